@@ -31,6 +31,8 @@ EXPORTS = [
     "b2q_vision_wait_submitted",
     "b2q_text_create", "b2q_text_destroy", "b2q_text_set_tensor", "b2q_text_reserve", "b2q_text_encode",
     "b2q_text_encode_host", "b2q_score_scratch_bytes", "b2q_score",
+    "b2q_kv_plan", "b2q_qk_norm_rope", "b2q_attention_paged_scratch_bytes", "b2q_attention_paged",
+    "b2q_weight_q4_register", "b2q_weight_q4_release", "b2q_mul_vec_q4",
     "b2q_gguf_open", "b2q_gguf_close", "b2q_gguf_n_tensors", "b2q_gguf_tensor", "b2q_gguf_scalar_f32",
     "b2q_vision_load_gguf", "b2q_text_load_gguf",
 ]
@@ -54,11 +56,18 @@ class TextConfig(C.Structure):
 
 POOL_MEAN, POOL_PROBE = 0, 1
 GGML_F32, GGML_Q8_0 = 0, 8
+GGML_F16, GGML_Q4_0, GGML_Q4_1, GGML_BF16 = 1, 2, 3, 30
 
 
 class Epilogue(C.Structure):
     _fields_ = [("kind", C.c_int), ("bias", C.c_void_p), ("residual", C.c_void_p),
                 ("act_out", C.c_void_p), ("ld_out", C.c_int64)]
+
+
+class KvCacheDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("n_kv_head", C.c_int32), ("d_head", C.c_int32),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64)]
 
 
 _lib = None
@@ -113,6 +122,16 @@ def lib():
         L.b2q_score_scratch_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int32]
         L.b2q_score_scratch_bytes.restype = C.c_size_t
         L.b2q_score.argtypes = [P, C.c_int32, P, C.c_int32, C.c_int32, C.c_float, C.c_float, P, P, P, P]
+        I32 = C.c_int32
+        L.b2q_kv_plan.argtypes = [P, P, I32, I32, P, I32, P, I64, I32, I32, P, P, P, P, P, P]
+        L.b2q_qk_norm_rope.argtypes = [P, I32, I64, I64, I32, P, P, C.c_float, P, I32, I32, I32, P, P, P, I64, P, P]
+        L.b2q_attention_paged_scratch_bytes.argtypes = [I32, I32, I32]
+        L.b2q_attention_paged_scratch_bytes.restype = C.c_size_t
+        L.b2q_attention_paged.argtypes = [P, I64, I64, I32, P, P, I64, I32, I32, P, P, C.c_float, I32, P, I32, I64, P,
+                                          P, P]
+        L.b2q_weight_q4_register.argtypes = [P, I32, I64, I64, I64, C.c_int, P, C.POINTER(P)]
+        L.b2q_weight_q4_release.argtypes = [P]
+        L.b2q_mul_vec_q4.argtypes = [P, P, I32, I64, I64, I64, P, I32, I64, P, P, P]
         L.b2q_gguf_open.argtypes = [C.c_char_p, C.POINTER(P)]
         L.b2q_gguf_close.argtypes = [P]
         L.b2q_gguf_n_tensors.argtypes = [P]
@@ -125,7 +144,7 @@ def lib():
         for name in EXPORTS:
             fn = getattr(L, name)
             if name not in ("b2q_last_error", "b2q_abi_version", "b2q_act_bytes", "b2q_attention_scratch_bytes",
-                            "b2q_launch_count", "b2q_graph_launch_count"):
+                            "b2q_attention_paged_scratch_bytes", "b2q_launch_count", "b2q_graph_launch_count"):
                 fn.restype = C.c_int
         _lib = L
     return _lib
@@ -446,6 +465,189 @@ def score(img, txt, logit_scale: float, logit_bias: float, logits=True, probs=Tr
     check(lib().b2q_score(_ptr(img), I, _ptr(txt), J, H, float(logit_scale), float(logit_bias), _ptr(lg), _ptr(pr),
                           _ptr(scratch), _stream(stream)))
     return lg, pr
+
+
+# ---- decoding over a paged key-value cache ---------------------------------
+def _type_of(t) -> int:
+    import torch
+    types = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
+    if t.dtype not in types:
+        raise B2QError(ERR_INVALID, f"element type {t.dtype} is not one of float32, float16, bfloat16")
+    return types[t.dtype]
+
+
+def _require(ok: bool, what: str):
+    if not ok:
+        raise B2QError(ERR_SHAPE, what)
+
+
+def _require_i32(n, **tensors):
+    """Contiguous int32 tensors on the device with n entries (None = any)."""
+    import torch
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or not t.is_cuda:
+            raise B2QError(ERR_INVALID, f"{name} must be an int32 CUDA tensor")
+        _require(t.is_contiguous() and (n is None or t.numel() == n), f"{name} must be contiguous with {n} entries")
+
+
+def _rows(t, width: int, name: str) -> int:
+    """Row stride of a [rows][width] tensor whose columns are contiguous."""
+    _require(t.dim() == 2 and t.shape[1] == width and (t.stride(1) == 1 or width == 1 or t.numel() == 0),
+             f"{name} must be [rows][{width}] with contiguous columns")
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+class KVCache:
+    """A layer's paged keys and values: k, v of shape [n_pages][n_kv_head]
+    [page_size][d_head] (fp16 or bf16), in any order of the first three
+    dimensions (a permuted view is described by its strides)."""
+
+    def __init__(self, k, v):
+        _require(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype,
+                 "k and v must be alike, [n_pages][n_kv_head][page_size][d_head]")
+        _require(k.stride(3) == 1, "the elements of a head must be contiguous")
+        self.k, self.v = k, v
+        self.n_pages, self.n_kv_head, self.page_size, self.d_head = k.shape
+        self.dtype = k.dtype
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _type_of(k), self.n_pages, self.page_size, self.n_kv_head,
+                                self.d_head, k.stride(0), k.stride(1), k.stride(2))
+        self.ref = C.addressof(self.desc)
+
+
+def kv_plan(ctx_len, new_len, page_size: int, free_pages, block_table, seq_of, pos, slot, kv_len, counts, stream=None):
+    """Block tables, positions and cache slots of a step (b2q_kv_plan).
+    ctx_len, new_len: int32 [n_seq]; block_table: int32 [n_seq][max_blocks],
+    entered in place; seq_of, pos, slot, kv_len: int32 [max_tokens] and counts
+    int32 [2], written."""
+    n, rows = ctx_len.numel(), seq_of.numel()
+    _require_i32(n, ctx_len=ctx_len, new_len=new_len)
+    _require_i32(rows, seq_of=seq_of, pos=pos, slot=slot, kv_len=kv_len)
+    _require_i32(None, free_pages=free_pages)
+    _require_i32(2, counts=counts)
+    _require(block_table.dim() == 2 and block_table.shape[0] == n, "block_table must be [n_seq][max_blocks]")
+    width = block_table.shape[1]
+    stride = _table(block_table)
+    check(lib().b2q_kv_plan(_ptr(ctx_len), _ptr(new_len), n, page_size, _ptr(free_pages), free_pages.numel(),
+                            _ptr(block_table), stride, width, rows, _ptr(seq_of), _ptr(pos), _ptr(slot), _ptr(kv_len),
+                            _ptr(counts), _stream(stream)))
+
+
+def _table(block_table) -> int:
+    import torch
+    if block_table.dtype != torch.int32 or not block_table.is_cuda:
+        raise B2QError(ERR_INVALID, "block_table must be an int32 CUDA tensor")
+    return _rows(block_table, block_table.shape[1], "block_table")
+
+
+def rope_table(n_pos: int, rot_dim: int, theta: float = 10000.0, device="cuda"):
+    """The rotation table that qk_norm_rope reads: fp32 [n_pos][rot_dim], the
+    cosines of pos * theta^(-2i / rot_dim), then the sines (angles in double)."""
+    import torch
+    inv = theta ** (-2.0 * torch.arange(rot_dim // 2, dtype=torch.float64, device=device) / max(rot_dim, 1))
+    ang = torch.arange(n_pos, dtype=torch.float64, device=device)[:, None] * inv[None]
+    return torch.cat([ang.cos(), ang.sin()], 1).float().contiguous()
+
+
+def qk_norm_rope(qkv, n_head: int, cache: KVCache, q_out, pos, slot, q_weight=None, k_weight=None, eps: float = 1e-6,
+                 rope=None, interleaved: bool = False, stream=None):
+    """Norm and rotation of the rows' query and key heads, keys and values to
+    their cache slots (b2q_qk_norm_rope).  qkv: [rows][(n_head + 2 n_kv_head)
+    d_head]; q_out: [rows][n_head d_head] of the cache's type; pos, slot: int32
+    [rows]; rope: fp32 [n_pos][rot_dim] (see rope_table)."""
+    import torch
+    rows, d = qkv.shape[0], cache.d_head
+    ld = _rows(qkv, (n_head + 2 * cache.n_kv_head) * d, "qkv")
+    ldq = _rows(q_out, n_head * d, "q_out")
+    _require(q_out.shape[0] == rows and q_out.dtype == cache.dtype, "q_out must have qkv's rows and the cache's type")
+    _require_i32(rows, pos=pos, slot=slot)
+    n_pos = rot = 0
+    if rope is not None:
+        _require(rope.dim() == 2 and rope.is_contiguous() and rope.dtype == torch.float32,
+                 "rope must be fp32 [n_pos][rot_dim]")
+        n_pos, rot = rope.shape
+    for w in (q_weight, k_weight):
+        _require(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == d),
+                 "norm weights must be fp32 [d_head]")
+    check(lib().b2q_qk_norm_rope(_ptr(qkv), _type_of(qkv), ld, rows, n_head, _ptr(q_weight), _ptr(k_weight), eps,
+                                 _ptr(rope), n_pos, rot, int(interleaved), _ptr(pos), _ptr(slot), _ptr(q_out), ldq,
+                                 cache.ref, _stream(stream)))
+
+
+def attention_paged_scratch(n_head: int, cache: KVCache):
+    """Zeroed scratch for attention_paged with this cache (one per stream)."""
+    import torch
+    nbytes = int(lib().b2q_attention_paged_scratch_bytes(n_head, cache.n_kv_head, cache.d_head))
+    _require(nbytes > 0, "n_head must be a multiple of n_kv_head")
+    return torch.zeros(nbytes, dtype=torch.uint8, device=cache.k.device)
+
+
+def attention_paged(q, cache: KVCache, block_table, kv_len, out, scratch, seq_of=None, scale: float | None = None,
+                    window: int = 0, lse=None, stream=None):
+    """Attention of each row's token over its request's cached keys
+    (b2q_attention_paged).  q: [rows][n_head d_head] of the cache's type; out
+    the same shape, fp32 or the cache's type; block_table: int32 [requests]
+    [max_blocks]; kv_len (and seq_of): int32 [rows]; lse: fp32 [rows][n_head]."""
+    import torch
+    rows, d = q.shape[0], cache.d_head
+    n_head = q.shape[1] // d
+    ldq, ldo = _rows(q, n_head * d, "q"), _rows(out, n_head * d, "out")
+    _require(out.shape[0] == rows and q.dtype == cache.dtype, "q and out need the same rows, q the cache's type")
+    _require_i32(rows, kv_len=kv_len)
+    if seq_of is not None:
+        _require_i32(rows, seq_of=seq_of)
+    if lse is not None:
+        _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == rows * n_head,
+                 "lse must be fp32 [rows][n_head]")
+    _require(n_head % cache.n_kv_head == 0 and scratch.numel() >= lib().b2q_attention_paged_scratch_bytes(
+        n_head, cache.n_kv_head, d), "scratch smaller than attention_paged_scratch, or n_head not a multiple of n_kv_head")
+    check(lib().b2q_attention_paged(_ptr(q), ldq, rows, n_head, cache.ref, _ptr(block_table), _table(block_table),
+                                    block_table.shape[1], block_table.shape[0], _ptr(seq_of), _ptr(kv_len),
+                                    d ** -0.5 if scale is None else scale, window, _ptr(out), _type_of(out), ldo,
+                                    _ptr(lse), _ptr(scratch), _stream(stream)))
+
+
+class WeightQ4:
+    """A registered ggml Q4_0 / Q4_1 weight (N rows of K): a numpy array or a
+    CUDA tensor of its blocks' bytes, rows row_bytes apart."""
+
+    def __init__(self, blocks, n: int, k: int, ggml_type: int = GGML_Q4_0, row_bytes: int | None = None, stream=None):
+        self.handle = C.c_void_p()
+        row_bytes = row_bytes or k // 32 * (18 if ggml_type == GGML_Q4_0 else 20)
+        host = isinstance(blocks, np.ndarray)
+        buf = np.ascontiguousarray(blocks) if host else blocks
+        size = buf.nbytes if host else buf.numel() * buf.element_size()
+        _require(size >= n * row_bytes and (host or (buf.is_cuda and buf.is_contiguous())),
+                 "blocks must be contiguous and hold n rows")
+        check(lib().b2q_weight_q4_register(buf.ctypes.data if host else buf.data_ptr(), ggml_type, n, k, row_bytes,
+                                           int(host), _stream(stream), C.byref(self.handle)))
+        self.n, self.k, self.ggml_type = n, k, ggml_type
+
+    def release(self):
+        if self.handle:
+            lib().b2q_weight_q4_release(self.handle)
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.release()
+        except Exception:
+            pass
+
+
+def mul_vec_q4(w: WeightQ4, x, m: int, y, bias=None, residual=None, stream=None):
+    """y[m][n] = x @ w^T (+ bias) (+ residual) for few rows (b2q_mul_vec_q4).
+    x: [m][x_cols] fp32, fp16 or bf16 (x_cols rounds up to the weight's K); y:
+    [m][n] fp32 or x's type; bias fp32 [n]; residual fp32 like y."""
+    import torch
+    ldx, ldy = _rows(x, x.shape[1], "x"), _rows(y, w.n, "y")
+    _require(x.shape[0] >= m and y.shape[0] >= m, "x and y need m rows")
+    if bias is not None:
+        _require(bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == w.n, "bias must be fp32 [n]")
+    if residual is not None:
+        _require(residual.dtype == torch.float32 and _rows(residual, w.n, "residual") == ldy
+                 and residual.shape[0] >= m, "residual must be fp32 with y's rows and stride")
+    check(lib().b2q_mul_vec_q4(w.handle, _ptr(x), _type_of(x), m, x.shape[1], ldx, _ptr(y), _type_of(y), ldy,
+                               _ptr(bias), _ptr(residual), _stream(stream)))
 
 
 class Gguf:

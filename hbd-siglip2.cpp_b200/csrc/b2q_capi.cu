@@ -153,6 +153,12 @@ b2q_status b2q_check_device(void* stream, uint32_t* code_out) {
     if (code_out) *code_out = code;
     if (code == 5u)   // kDevBadTokenId
         return set_error(B2Q_ERR_DEVICE, "a token id outside the vocabulary (code 5)");
+    if (code == 6u)   // kDevBadPosition
+        return set_error(B2Q_ERR_DEVICE, "a position or a cache slot out of range (code 6)");
+    if (code == 7u)   // kDevBadPage
+        return set_error(B2Q_ERR_DEVICE, "a request, page or length outside the block table or the cache (code 7)");
+    if (code == 8u)   // kDevPlanFull
+        return set_error(B2Q_ERR_DEVICE, "a step that did not fit its pages, block table or rows (code 8)");
     if (code) return set_error(B2Q_ERR_DEVICE, "a kernel's bounded wait expired (code " + std::to_string(code) + ")");
     return B2Q_OK;
 }

@@ -38,7 +38,7 @@ enum : uint32_t {
     GGUF_U8 = 0, GGUF_I8 = 1, GGUF_U16 = 2, GGUF_I16 = 3, GGUF_U32 = 4, GGUF_I32 = 5, GGUF_F32 = 6,
     GGUF_BOOL = 7, GGUF_STRING = 8, GGUF_ARRAY = 9, GGUF_U64 = 10, GGUF_I64 = 11, GGUF_F64 = 12
 };
-enum : int32_t { T_F32 = 0, T_F16 = 1, T_Q8_0 = 8, T_BF16 = 30 };
+enum : int32_t { T_F32 = 0, T_F16 = 1, T_Q4_0 = 2, T_Q4_1 = 3, T_Q8_0 = 8, T_BF16 = 30 };
 
 struct TensorInfo {
     std::string name;
@@ -205,6 +205,13 @@ b2q_status bytes_of(const TensorInfo& t, size_t* out) {
             if (un / 32 > SIZE_MAX / 34) return set_error(B2Q_ERR_SHAPE, "GGUF: tensor " + t.name + " too large");
             *out = static_cast<size_t>(un / 32) * 34;
             return B2Q_OK;
+        case T_Q4_0: case T_Q4_1: {   // for b2q_weight_q4_register; no tower tensor has these types
+            const uint64_t block = t.type == T_Q4_0 ? 18 : 20;
+            if (t.ne[0] % 32) return set_error(B2Q_ERR_SHAPE, "GGUF: Q4 tensor " + t.name + " with ne0 % 32 != 0");
+            if (un / 32 > SIZE_MAX / block) return set_error(B2Q_ERR_SHAPE, "GGUF: tensor " + t.name + " too large");
+            *out = static_cast<size_t>(un / 32 * block);
+            return B2Q_OK;
+        }
         default:
             *out = 0;   // other types are listed but cannot be loaded into a tower
             return B2Q_OK;

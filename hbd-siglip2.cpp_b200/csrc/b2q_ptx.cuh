@@ -20,6 +20,9 @@ enum : uint32_t {
     kDevTimeoutTmemFull = 3,  // MMA result never committed
     kDevTimeoutTmemEmpty = 4, // epilogue never released an accumulator
     kDevBadTokenId = 5,       // a token id outside the vocabulary (replaced by 0)
+    kDevBadPosition = 6,      // a position outside the rotation table, a slot outside the cache
+    kDevBadPage = 7,          // a request, page or length outside the block table or the cache
+    kDevPlanFull = 8,         // a step that did not fit its pages, block table or rows
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

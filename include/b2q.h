@@ -101,7 +101,10 @@ b2q_status b2q_tune(int key, int64_t value);
 /* Reads (and clears) the device error word after synchronising `stream`;
  * B2Q_ERR_DEVICE when it was set: codes 1-4 = an in-kernel wait expired
  * (1 TMA data, 2 stage release, 3 MMA commit, 4 accumulator release),
- * 5 = a token id outside the vocabulary. */
+ * 5 = a token id outside the vocabulary, 6 = a position outside the rotation
+ * table or a slot outside the cache, 7 = a request, page or length outside the
+ * block table or the cache, 8 = a step that did not fit its pages, table or
+ * rows. */
 b2q_status b2q_check_device(void *stream, uint32_t *code_out);
 
 /* ---- weights -------------------------------------------------------------
@@ -300,6 +303,107 @@ b2q_status b2q_text_encode_host(b2q_text *t, const int32_t *ids_host, int32_t n_
 size_t b2q_score_scratch_bytes(int32_t n_image, int32_t n_text, int32_t hidden);
 b2q_status b2q_score(const float *img, int32_t n_image, const float *txt, int32_t n_text, int32_t hidden,
                      float logit_scale, float logit_bias, float *logits, float *probs, void *scratch, void *stream);
+
+/* ---- decoding over a paged key-value cache ----------------------------------
+ * What answering with tokens needs next to the towers (no counterpart in the
+ * reference, which only encodes): one decode step is b2q_kv_plan, then per
+ * layer b2q_mul_vec_q4 (QKV), b2q_qk_norm_rope, b2q_attention_paged and
+ * b2q_mul_vec_q4 (output).  Element types go by their ggml type ids. */
+enum { B2Q_TYPE_F32 = 0, B2Q_TYPE_F16 = 1, B2Q_TYPE_Q4_0 = 2, B2Q_TYPE_Q4_1 = 3, B2Q_TYPE_BF16 = 30 };
+
+/* Keys and values in pages of page_size tokens (a power of two, at most
+ * 1024): token slot s lives in page s / page_size, row s % page_size.  The
+ * element (page, head, row, d) of k and of v is at page * page_stride +
+ * head * head_stride + row * token_stride + d; strides are in elements,
+ * multiples of 8, and 0 means that of the contiguous order
+ * [n_pages][n_kv_head][page_size][d_head].  d_head: a multiple of 8 up to
+ * 256.  k and v are 16-byte aligned; n_pages * page_size fits an int32. */
+typedef struct b2q_kv_cache {
+    void *k, *v;
+    int32_t dtype;      /* B2Q_TYPE_F16 or B2Q_TYPE_BF16 */
+    int32_t n_pages, page_size, n_kv_head, d_head;
+    int64_t page_stride, head_stride, token_stride;
+} b2q_kv_cache;
+
+/* Block tables, positions and cache slots of a step, built on the device from
+ * the requests' lengths.  Request s has ctx_len[s] tokens cached and brings
+ * new_len[s]; block_table[s * bt_stride + b] (max_blocks entries) is the page
+ * of its tokens b * page_size ...  Pages that the new tokens need are taken
+ * from free_pages in order (requests in order, each request's pages in order)
+ * and entered into the table.  The new tokens of all requests back to back are
+ * the step's rows; row t receives
+ *   seq_of[t] its request, pos[t] its position, slot[t] its cache slot,
+ *   kv_len[t] = pos + 1 (what b2q_attention_paged reads for a causal row);
+ * rows from the number of tokens up to max_tokens get -1, -1, -1, 0, so that a
+ * captured step can run on fewer tokens.  counts[0] = tokens, counts[1] =
+ * pages taken.  n_seq up to 16384.  Where the pages, the table's width or
+ * max_tokens do not suffice, or a length is negative (read as 0), what fits
+ * is done, slots without a page are -1, and b2q_check_device reports code 8. */
+b2q_status b2q_kv_plan(const int32_t *ctx_len, const int32_t *new_len, int32_t n_seq, int32_t page_size,
+                       const int32_t *free_pages, int32_t n_free, int32_t *block_table, int64_t bt_stride,
+                       int32_t max_blocks, int32_t max_tokens, int32_t *seq_of, int32_t *pos, int32_t *slot,
+                       int32_t *kv_len, int32_t *counts, void *stream);
+
+/* One pass over the rows [Q | K | V] (n_head + 2 * n_kv_head heads of d_head,
+ * row stride ld elements, dtype F32, F16 or BF16): each query and key head h is
+ * normed, h * w / sqrt(mean(h^2) + eps) (q_weight, k_weight: fp32 [d_head],
+ * NULL = no norm), and its first rot_dim elements are rotated by row pos[t] of
+ * `rope` (fp32 [n_pos][rot_dim]: rot_dim/2 cosines, then rot_dim/2 sines;
+ * rot_dim even, 0 = no rotation and rope NULL).  Pairs are (i, i + rot_dim/2),
+ * or (2i, 2i + 1) with interleaved != 0:
+ *   y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin.
+ * Queries go to q_out (row stride ldq, the cache's type), keys and unchanged
+ * values to cache slot slot[t]; slot -1 stores none.  A row with pos -1 is
+ * padding: its q_out row is zeroed and nothing is cached.  Another position or
+ * slot out of range is reported through b2q_check_device (code 6; position 0 is
+ * used, nothing is stored).  Slots of one call are distinct.  q_out may be
+ * the Q columns of `qkv` itself when the types agree.  Arithmetic in fp32,
+ * rounded once. */
+b2q_status b2q_qk_norm_rope(const void *qkv, int32_t dtype, int64_t ld, int64_t n_rows, int32_t n_head,
+                            const float *q_weight, const float *k_weight, float eps, const float *rope, int32_t n_pos,
+                            int32_t rot_dim, int32_t interleaved, const int32_t *pos, const int32_t *slot,
+                            void *q_out, int64_t ldq, const b2q_kv_cache *cache, void *stream);
+
+/* Attention of single tokens over the cache, split over its length and joined
+ * in one launch.  Row r has n_head query heads of d_head (the cache's type, row
+ * stride ldq); head h reads key head h / (n_head / n_kv_head) of request
+ * seq_of[r] (NULL: request r; -1: an idle row) at the positions
+ * max(0, kv_len[r] - window) .. kv_len[r] - 1 (window 0: from 0), found through
+ * its block_table row (max_blocks entries, n_table_rows rows).  out[r][h*d_head
+ * + d] = sum softmax(scale q.k) v (out_dtype F32 or the cache's type, row
+ * stride ldo); a row with nothing to read gets zeros.  lse (fp32 [n_rows]
+ * [n_head], NULL = not wanted) receives log sum exp(scale q.k), -inf for such
+ * rows.  Nothing behind kv_len is read into a result, whatever bits it holds.
+ * A request, a page or a length out of range is reported through
+ * b2q_check_device (code 7) and its keys are left out.
+ * scratch: b2q_attention_paged_scratch_bytes(), 256-byte aligned, all zero
+ * before its first use; every call leaves it usable for the next call of any
+ * shape with the same n_head, n_kv_head and d_head (one stream at a time). */
+size_t b2q_attention_paged_scratch_bytes(int32_t n_head, int32_t n_kv_head, int32_t d_head);
+b2q_status b2q_attention_paged(const void *q, int64_t ldq, int64_t n_rows, int32_t n_head, const b2q_kv_cache *cache,
+                               const int32_t *block_table, int64_t bt_stride, int32_t max_blocks,
+                               int32_t n_table_rows, const int32_t *seq_of, const int32_t *kv_len, float scale,
+                               int32_t window, void *out, int32_t out_dtype, int64_t ldo, float *lse, void *scratch,
+                               void *stream);
+
+/* ---- matrix-vector products with 4-bit weights -------------------------------
+ * A registered ggml Q4_0 tensor (18-byte blocks of 32: fp16 d, 16 bytes of
+ * nibbles, low nibbles first; w = d (q - 8)) or Q4_1 (20 bytes: fp16 d, fp16
+ * m; w = d q + m): N rows of K (a multiple of 32), row stride row_bytes.
+ * Repacked once; the source is not retained. */
+typedef struct b2q_weight_q4 b2q_weight_q4;
+b2q_status b2q_weight_q4_register(const void *blocks, int32_t ggml_type, int64_t N, int64_t K, int64_t row_bytes,
+                                  int src_is_host, void *stream, b2q_weight_q4 **out);
+b2q_status b2q_weight_q4_release(b2q_weight_q4 *w);
+/* y[m][n] = sum_k w[n][k] x[m][k] (+ bias[n]) (+ residual[m][n]) for M rows
+ * x[M][ldx] (x_dtype F32, F16 or BF16) of x_cols columns, x_cols rounded up to
+ * 32 = K (columns x_cols..K-1 read as zero).  y (y_dtype F32 or x_dtype) and
+ * residual (fp32, may be y) have row stride ldy; bias and residual may be
+ * NULL.  The activations are not quantized: products and sums are in fp32,
+ * rounded once.  Meant for few rows (one weight pass per eight or so). */
+b2q_status b2q_mul_vec_q4(const b2q_weight_q4 *w, const void *x, int32_t x_dtype, int64_t M, int64_t x_cols,
+                          int64_t ldx, void *y, int32_t y_dtype, int64_t ldy, const float *bias,
+                          const float *residual, void *stream);
 
 /* ---- GGUF checkpoints -------------------------------------------------------
  * Counterpart of GGUFLoader (src/gguf_loader.cpp:205-337).  b2q_gguf_open maps
