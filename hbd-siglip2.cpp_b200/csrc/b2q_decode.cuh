@@ -62,6 +62,13 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], uint32_t
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// d = a * b, sums from zero.
+template <class T>
+__device__ __forceinline__ void mma_16816_from0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
+    d[0] = d[1] = d[2] = d[3] = 0.f;
+    mma_16816<T>(d, a0, a1, a2, a3, b0, b1);
+}
 // Two floats rounded to a pair of T (x in the low half), and what the rounding left of them.
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float x, float y);
@@ -89,6 +96,16 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
 __device__ __forceinline__ void cp_async_16(uint32_t smem, const void* gmem, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(valid ? 16u : 0u)
                  : "memory");
+}
+__device__ __forceinline__ uint4 lds_128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint2 lds_64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
