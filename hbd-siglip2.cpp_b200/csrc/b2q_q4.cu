@@ -1,31 +1,38 @@
 // b2q_q4.cu — products of few activation rows with ggml Q4_0 / Q4_1 weights
 // (b2q_weight_q4_*, b2q_mul_vec_q4).
 //
-// y[n] = sum_kb d[n,kb] S[n,kb] (+ m[n,kb] X[kb]), S the sum of (q - 8) x (Q4_1:
-// q x) over the 32 columns of block kb, X that of x.
+// y[n] = sum_kb d[n,kb] (S[n,kb] - 8 X[kb])   (Q4_1: d S + m X), S the sum of q x
+// over the 32 columns of block kb, X that of x.
 //
 // Bound: bytes, 18 (20) per 32 weights and at most once.  At the measured copy
 // rate that is 11.6 T weights/s, and the SMs issue about 36 T lane operations/s:
-// three instructions a weight for everything.  Unpacking alone takes more than
-// one, so even a single activation row goes to the tensor cores: mma.sync
-// (16 weight rows x 16 columns x 8 activation columns) does 8 of a lane's
-// products in one instruction and sums in fp32.
+// three instructions a weight for everything, which unpacking to floats and
+// multiplying alone would take.  So even a single activation row goes to the
+// tensor cores: one mma.sync (16 weight rows x 16 columns x 8 activation columns)
+// does 8 of a lane's products and sums in fp32, and almost nothing is unpacked:
 //
-//  * The nibbles become exact 16-bit integers: OR-ed into the mantissa of 2^7
-//    (bf16) or 2^10 (fp16), the power and the 8 subtracted again.
-//  * fp16 and bf16 activations are operands as they are.  An fp32 activation
-//    is the exact sum of three bf16 values (8 bits of its mantissa each), which
-//    take three of the eight activation columns: with one row they are free.
-//  * S leaves the tensor core once per block, is scaled by the fp32 value of d
-//    and summed in fp32, so nothing is rounded to 16 bits on the way.
+//  * A nibble masked out of its word is an fp16 number as it stands, the
+//    subnormal q 2^-24 (in bits 0-3 of a half) or q 2^-20 (bits 4-7); the factor
+//    between the two is put into the activations.  Five instructions unpack eight
+//    weights: four masks and one shift.  The 8 of Q4_0 goes into the sums' start
+//    value, -8 X.
+//  * An activation row is scaled by a power of two to a largest value in
+//    [2^14, 2^15) and becomes fp16 operands: fp16 and bf16 values one, an fp32 value
+//    three (11 bits of its mantissa each), in as many of the eight activation
+//    columns; with one or two rows they are free.  What this loses lies 2^-36
+//    below the row's largest value.  (As bf16 the three pieces would need no scale,
+//    but bf16 holds one nibble in its mantissa, which takes 11 instructions for
+//    eight weights: 65 against 35 us for 256000 x 1152.)
+//  * S - 8 X leaves the tensor core once per block, is scaled by the fp32 value of d
+//    and summed in fp32.
 //
 // The weights are laid out at registration in the order the lanes want them:
-// per 16 rows a run of units of 64 columns, each 512 bytes of nibbles (lane l of
-// the warp: 16 bytes) and the blocks' scales (64 bytes; Q4_1: 64 more for m).  A
-// warp streams units through a ring of asynchronous copies that runs on across
-// row tiles; the activations sit in shared memory for the whole launch (grid:
-// one CTA of 16 warps per SM).  kSplit warps share a row tile, each taking every
-// kSplit-th unit, and add up in a fixed order.
+// per 16 rows a run of units of 128 columns, each 1024 bytes of nibbles (lane l of
+// the warp: twice 16 bytes) and the blocks' scales (128 bytes; Q4_1: 128 more for
+// m).  A warp streams units through its own ring, one bulk copy each, which runs
+// on across row tiles; the activations sit in shared memory for the whole launch
+// (a fixed grid of one or two CTAs of 16 warps per SM).  `split` warps share a row
+// tile, each taking every split-th unit, and add up in a fixed order.
 #include "b2q_decode.cuh"
 
 #include <new>
@@ -34,8 +41,8 @@
 struct b2q_weight_q4 {
     int64_t N = 0, K = 0;
     int type = 0, device = -1;
-    int64_t tiles = 0, units = 0;   // of 16 rows; of 64 columns per row tile
-    uint8_t* packed = nullptr;      // [tiles][units][576 or 640 bytes]
+    int64_t tiles = 0, units = 0;   // of 16 rows; of 128 columns per row tile
+    uint8_t* packed = nullptr;      // [tiles][units][unit_bytes]
 };
 
 namespace b2q {
@@ -43,16 +50,21 @@ namespace {
 
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxK = 28672;        // three bf16 pieces of a row still fit shared memory next to the rings
-constexpr int kSmemMax = 227 * 1024 - 1024;
+constexpr int kMaxRows = 32;        // of one launch
+constexpr int kMaxK = 28672;        // three pieces of a row still fit shared memory next to the rings
+constexpr int kSmemMax = 227 * 1024 - 2048;   // next to the static part
+constexpr int kSmemHalf = 111 * 1024;   // two CTAs of an SM
 
-constexpr int unit_bytes(bool min) { return min ? 640 : 576; }
+constexpr int kMaxStages = 8;
+constexpr int unit_bytes(bool min) { return min ? 1280 : 1152; }
+constexpr int red_pitch(int n_tiles) { return 8 * n_tiles + 1; }   // odd: rows in different banks
 
 // ------------------------------------------------------------------ layout
-// Lane l = 4 g + t of a unit holds, for each of its two blocks, the columns
+// Lane l = 4 g + t of a unit holds, for each of its four blocks, the columns
 // 8 t .. 8 t + 7 of rows g and g + 8: one 32-bit word each, column 2 j in the
-// nibble at bit 4 j and column 2 j + 1 in that at bit 16 + 4 j, so that shifting
-// by 4 j and masking yields the operand pair (2 j, 2 j + 1).
+// nibble at bit 4 j and column 2 j + 1 in that at bit 16 + 4 j.  Blocks 0 and 1
+// fill the first 512 bytes, 2 and 3 the next; then per g the scales of
+// (block, row g), (block, row g + 8), ..., and in Q4_1 the same for m.
 __global__ void pack_q4_kernel(const uint8_t* __restrict__ raw, int64_t N, int64_t Kb, int64_t row_bytes, bool min,
                                int64_t tiles, int64_t units, uint8_t* __restrict__ out) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;   // one lane of one unit
@@ -60,9 +72,9 @@ __global__ void pack_q4_kernel(const uint8_t* __restrict__ raw, int64_t N, int64
     const int l = static_cast<int>(i & 31), g = l >> 2, t = l & 3;
     const int64_t unit = (i >> 5) % units, tile = (i >> 5) / units;
     uint8_t* dst = out + (i >> 5) * unit_bytes(min);
-    uint32_t w[4];
-    for (int x = 0; x < 4; ++x) {
-        const int64_t n = tile * 16 + g + 8 * (x & 1), kb = unit * 2 + (x >> 1);
+    uint32_t w[8];
+    for (int x = 0; x < 8; ++x) {
+        const int64_t n = tile * 16 + g + 8 * (x & 1), kb = unit * 4 + (x >> 1);
         w[x] = 0;
         uint16_t d = 0, m = 0;
         if (n < N && kb < Kb) {
@@ -77,270 +89,412 @@ __global__ void pack_q4_kernel(const uint8_t* __restrict__ raw, int64_t N, int64
             if (min) m = static_cast<uint16_t>(b[2] | (b[3] << 8));
         }
         if (t == 0) {
-            reinterpret_cast<uint16_t*>(dst + 512 + g * 8)[x] = d;
-            if (min) reinterpret_cast<uint16_t*>(dst + 576 + g * 8)[x] = m;
+            reinterpret_cast<uint16_t*>(dst + 1024 + g * 16)[x] = d;
+            if (min) reinterpret_cast<uint16_t*>(dst + 1152 + g * 16)[x] = m;
         }
     }
     *reinterpret_cast<uint4*>(dst + l * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(dst + 512 + l * 16) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 // ------------------------------------------------------------------ product
-template <class Tx>
 struct Q4Args {
     const uint8_t* w;
     int64_t N;
     int tiles, units, split;
-    const Tx* x;
+    const void* x;
+    int x_type, pieces;
     int rows;               // activation rows of this launch
     int64_t x_cols, ldx;
     void* y;
     int64_t ldy;
     bool y_f32;
     const float *bias, *residual;
-    int pitch, ring_at, red_at, sum_at;   // shared memory: row of an activation column, parts' offsets (bytes)
+    int pitch, ring_at, stages, red_at, sum_at;   // shared memory: bytes of an operand column, parts' offsets
+    uint64_t timeout_ns;
+    uint32_t* err;
 };
 
-// The word's four pairs as exact integers q - 8 (Q4_1: q).
-template <class T, bool kMin>
-__device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t (&r)[4]);
-#define B2Q_UNPACK_BF16(kMin)                                                                             \
-    template <>                                                                                           \
-    __device__ __forceinline__ void unpack_q4<__nv_bfloat16, kMin>(uint32_t w, uint32_t (&r)[4]) {        \
-        const __nv_bfloat162 off = __floats2bfloat162_rn(kMin ? -128.f : -136.f, kMin ? -128.f : -136.f); \
-        _Pragma("unroll") for (int j = 0; j < 4; ++j) {                                                   \
-            const uint32_t u = ((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u;                              \
-            const __nv_bfloat162 v = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&u), off);          \
-            r[j] = *reinterpret_cast<const uint32_t*>(&v);                                                \
-        }                                                                                                 \
-    }
-B2Q_UNPACK_BF16(false)
-B2Q_UNPACK_BF16(true)
-#undef B2Q_UNPACK_BF16
-// fp16 has room for a nibble at bit 4 as well (1024 + 16 q, scaled back in the
-// multiply-add), which saves two of the three shifts.
-#define B2Q_UNPACK_F16(kMin)                                                                      \
-    template <>                                                                                   \
-    __device__ __forceinline__ void unpack_q4<__half, kMin>(uint32_t w, uint32_t (&r)[4]) {       \
-        const __half2 off = __float2half2_rn(kMin ? -1024.f : -1032.f);                           \
-        const __half2 off16 = __float2half2_rn(kMin ? -64.f : -72.f), s16 = __float2half2_rn(0.0625f); \
-        _Pragma("unroll") for (int j = 0; j < 4; j += 2) {                                        \
-            const uint32_t s = w >> (4 * j);                                                      \
-            const uint32_t u = (s & 0x000F000Fu) | 0x64006400u, v = (s & 0x00F000F0u) | 0x64006400u; \
-            const __half2 a = __hadd2(*reinterpret_cast<const __half2*>(&u), off);                \
-            const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&v), s16, off16);         \
-            r[j] = *reinterpret_cast<const uint32_t*>(&a);                                        \
-            r[j + 1] = *reinterpret_cast<const uint32_t*>(&b);                                    \
-        }                                                                                         \
-    }
-B2Q_UNPACK_F16(false)
-B2Q_UNPACK_F16(true)
-#undef B2Q_UNPACK_F16
-
-// The leading 8 bits of x's mantissa (cut, so that what is left is exact and a
-// large x does not become infinite); infinities and NaN stay what they are.
-__device__ __forceinline__ float lead_bf16(float x) {
-    const uint32_t u = __float_as_uint(x) & 0xFFFF0000u;
-    return x != x ? x : __uint_as_float(u);
-}
-__device__ __forceinline__ float finite_or_0(float x) { return fabsf(x) <= 3.402823466e38f ? x : 0.f; }
-__device__ __forceinline__ uint32_t cut_pair(float x, float y) {
-    const uint32_t a = x != x ? 0x7FC0u : __float_as_uint(x) >> 16, b = y != y ? 0x7FC0u : __float_as_uint(y) >> 16;
-    return a | (b << 16);
+// The word's four pairs of a lane as fp16 operands: q 2^-24, q 2^-20, q 2^-24, q 2^-20.
+__device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t (&r)[4]) {
+    const uint32_t s = w >> 8;
+    r[0] = w & 0x000F000Fu;
+    r[1] = w & 0x00F000F0u;
+    r[2] = s & 0x000F000Fu;
+    r[3] = s & 0x00F000F0u;
 }
 
-// Activation rows into shared memory: per row its operand columns (fp32: three
-// bf16 pieces), and for Q4_1 the sums over each block.
-template <class Tx, bool kMin>
-__device__ __forceinline__ void stage_x(const Q4Args<Tx>& a, uint8_t* smem) {
-    constexpr int kPieces = std::is_same<Tx, float>::value ? 3 : 1;
-    const int chunks = a.units * 8;   // of 8 columns
-    const int total = a.rows * chunks;
-    const bool vec = (a.ldx * sizeof(Tx)) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
-    for (int base = 0; base < total; base += kThreads) {
-        const int i = base + threadIdx.x;
-        const bool in = i < total;
-        const int m = in ? i / chunks : 0, c = in ? i % chunks : 0;
-        const Tx* x = a.x + m * a.ldx + c * 8;
-        const int64_t left = in ? a.x_cols - c * 8 : 0;
-        Tx v[8];
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// What the rows' staging leaves in shared memory beside the operands.
+struct RowState {
+    uint32_t peak[kMaxRows];   // bits of the largest finite |x|
+    uint32_t odd;              // rows that hold an infinity or a NaN (left out of the operands)
+};
+// x 2^shift(peak) has its largest value in [2^14, 2^15); peaks below 2^-113 stay smaller.
+__device__ __forceinline__ int shift_of(uint32_t peak) { return min(141 - static_cast<int>(peak >> 23), 127); }
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
+
+// Eight values as they lie in memory.
+template <class Tx>
+struct Eight {
+    uint4 r[sizeof(Tx) / 2];
+    __device__ __forceinline__ void load(const Tx* x, int left, bool vec) {
         if (vec && left >= 8) {
 #pragma unroll
-            for (int j = 0; j < static_cast<int>(sizeof(Tx)) / 2; ++j)
-                reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(x)[j];
+            for (int j = 0; j < static_cast<int>(sizeof(Tx)) / 2; ++j) r[j] = reinterpret_cast<const uint4*>(x)[j];
         } else {
+            Tx* e = reinterpret_cast<Tx*>(r);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < left ? x[j] : from_f32<Tx>(0.f);
-        }
-        uint8_t* dst = smem + m * kPieces * a.pitch + c * 16;
-        if (in) {
-            if constexpr (kPieces == 1) {
-                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
-            } else {
-                uint32_t p[3][4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float e[2] = {v[2 * j], v[2 * j + 1]}, h[3][2];
-#pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        h[0][z] = lead_bf16(e[z]);
-                        const float r = finite_or_0(e[z] - h[0][z]);
-                        h[1][z] = lead_bf16(r);
-                        h[2][z] = r - h[1][z];
-                    }
-#pragma unroll
-                    for (int q = 0; q < 3; ++q) p[q][j] = cut_pair(h[q][0], h[q][1]);
-                }
-#pragma unroll
-                for (int q = 0; q < 3; ++q)
-                    *reinterpret_cast<uint4*>(dst + q * a.pitch) = make_uint4(p[q][0], p[q][1], p[q][2], p[q][3]);
-            }
-        }
-        if constexpr (kMin) {
-            float s = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s += to_f32(v[j]);
-            s += __shfl_xor_sync(0xffffffffu, s, 1);
-            s += __shfl_xor_sync(0xffffffffu, s, 2);
-            if (in && (c & 3) == 0) reinterpret_cast<float*>(smem + a.sum_at)[(c >> 2) * a.rows + m] = s;
+            for (int j = 0; j < 8; ++j) e[j] = j < left ? x[j] : from_f32<Tx>(0.f);
         }
     }
+    __device__ __forceinline__ float2 pair(int j) const {   // values 2 j, 2 j + 1
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(r);
+        if constexpr (sizeof(Tx) == 4) return make_float2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+        else return unpack2<Tx>(w[j]);
+    }
+    __device__ __forceinline__ uint32_t peak_bits() const {   // of the largest |x|, infinities and NaN on top
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(r);
+        uint32_t m = 0;
+        if constexpr (sizeof(Tx) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, w[j] & 0x7FFFFFFFu);
+            return m;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+            return __float_as_uint(unpack2<Tx>(max(m & 0xFFFFu, m >> 16)).x);
+        }
+    }
+};
+
+// Activation rows into shared memory: operand column p * rows + m holds piece p
+// of row m.  `sum_at` gets the sums X of each block's scaled values.  Q4_0: what
+// its products start from, -8 X 2^-24 in fp32, four blocks x two rows per unit and
+// pair of rows.  Q4_1: X 2^-5 as operands of the product with m, in three fp16
+// pieces side by side in k, four blocks x 8 bytes per unit and row.
+// A warp takes 256 columns of a row at a time, in two passes: the rows' peaks,
+// then the operands.
+template <class Tx, bool kMin>
+__device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState& st) {
+    constexpr int kPieces = std::is_same<Tx, float>::value ? 3 : 1;
+    constexpr int kBatch = kPieces == 3 ? 2 : 4;   // pieces of work whose loads are in flight together
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int chunks = a.units * 16, segs = (chunks + 31) / 32;   // of 8 columns; of 32 chunks
+    const int tasks = (a.rows * segs + kWarps - 1 - warp) / kWarps;
+    const Tx* px = static_cast<const Tx*>(a.x);
+    const bool vec = (a.ldx * sizeof(Tx)) % 16 == 0 && (reinterpret_cast<uintptr_t>(px) & 15) == 0;
+    struct Place {
+        int m, seg;
+    };
+    auto place = [&]() { return Place{warp / segs, warp % segs}; };
+    auto step = [&](Place& p) {
+        p.seg += kWarps;
+        while (p.seg >= segs) {
+            p.seg -= segs;
+            ++p.m;
+        }
+    };
+    Eight<Tx> v[kBatch];
+    auto load = [&](Place p, int n) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (b < n) {
+                const int c = p.seg * 32 + lane;
+                v[b].load(px + p.m * a.ldx + c * 8, static_cast<int>(a.x_cols) - c * 8, vec);
+                step(p);
+            }
+        }
+    };
+    Place p = place();
+    for (int i = 0; i < tasks; i += kBatch) {
+        load(p, tasks - i);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (i + b < tasks) {
+                uint32_t peak = v[b].peak_bits();
+                if (__any_sync(0xffffffffu, peak >= 0x7F800000u)) {
+                    if (lane == 0) atomicOr(&st.odd, 1u << p.m);
+                    peak = 0;
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 x = v[b].pair(j);
+                        if (is_finite(x.x)) peak = max(peak, __float_as_uint(fabsf(x.x)));
+                        if (is_finite(x.y)) peak = max(peak, __float_as_uint(fabsf(x.y)));
+                    }
+                }
+                peak = __reduce_max_sync(0xffffffffu, peak);
+                if (lane == 0) atomicMax(&st.peak[p.m], peak);
+                step(p);
+            }
+        }
+    }
+    __syncthreads();
+    const int pairs = (a.rows + 1) / 2;
+    const uint32_t any_odd = st.odd;
+    p = place();
+    for (int i = 0; i < tasks; i += kBatch) {
+        if (tasks > kBatch) load(p, tasks - i);   // else the first pass left them
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (i + b < tasks) {
+                const int c = p.seg * 32 + lane, m = p.m;
+                const float s = pow2(shift_of(st.peak[m])), s16 = s * 0.0625f;
+                float sum = 0.f;
+                uint32_t q[kPieces][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float2 x = v[b].pair(j);
+                    if (any_odd) {
+                        if (!is_finite(x.x)) x.x = 0.f;
+                        if (!is_finite(x.y)) x.y = 0.f;
+                    }
+                    sum = fmaf(x.x, s, fmaf(x.y, s, sum));
+                    x.x *= j & 1 ? s16 : s;   // where the nibble stands four bits higher
+                    x.y *= j & 1 ? s16 : s;
+#pragma unroll
+                    for (int z = 0; z < kPieces; ++z) {
+                        q[z][j] = pack2<__half>(x.x, x.y);
+                        if (z + 1 < kPieces) {
+                            const float2 h = unpack2<__half>(q[z][j]);
+                            x.x -= h.x;
+                            x.y -= h.y;
+                        }
+                    }
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (c < chunks) {
+                    uint8_t* dst = smem + m * a.pitch + c * 16;
+#pragma unroll
+                    for (int z = 0; z < kPieces; ++z)
+                        *reinterpret_cast<uint4*>(dst + z * a.rows * a.pitch) =
+                            make_uint4(q[z][0], q[z][1], q[z][2], q[z][3]);
+                    if ((c & 3) == 0) {
+                        const int unit = c >> 4, block = (c >> 2) & 3;
+                        if constexpr (kMin) {
+                            __half h[4];
+                            sum *= 0.03125f;
+#pragma unroll
+                            for (int z = 0; z < 3; ++z) {
+                                h[z] = __float2half_rn(sum);
+                                sum -= __half2float(h[z]);
+                            }
+                            h[3] = __float2half_rn(0.f);
+                            *reinterpret_cast<uint2*>(smem + a.sum_at + ((unit * a.rows + m) * 4 + block) * 8) =
+                                *reinterpret_cast<const uint2*>(h);
+                        } else {
+                            float* out = reinterpret_cast<float*>(smem + a.sum_at) +
+                                         ((unit * pairs + (m >> 1)) * 4 + block) * 2 + (m & 1);
+                            out[0] = sum * -4.76837158203125e-7f;
+                            if (m + 1 == a.rows && !(m & 1)) out[1] = 0.f;
+                        }
+                    }
+                }
+                step(p);
+            }
+        }
+    }
+    // what columns of other pieces take
+    if (threadIdx.x < 8)
+        reinterpret_cast<float*>(smem + a.sum_at)[a.units * (kMin ? a.rows : pairs) * 8 + threadIdx.x] = 0.f;
 }
 
-template <class Tx, bool kMin, int kN, int kStages>
-__global__ void __launch_bounds__(kThreads, 1) mul_vec_q4_kernel(Q4Args<Tx> a) {
-    using T = typename std::conditional<std::is_same<Tx, float>::value, __nv_bfloat16, Tx>::type;
-    constexpr int kPieces = std::is_same<Tx, float>::value ? 3 : 1;
+// w[n][k] as registered
+template <bool kMin>
+__device__ float weight_at(const Q4Args& a, int64_t n, int64_t k) {
+    const uint8_t* u = a.w + ((n >> 4) * a.units + (k >> 7)) * unit_bytes(kMin);
+    const int g = n & 7, high = (n >> 3) & 1, b = (k >> 5) & 3, t = (k >> 3) & 3, e = k & 7;
+    const uint32_t word = reinterpret_cast<const uint32_t*>(u)[(b >> 1) * 128 + (4 * g + t) * 4 + 2 * (b & 1) + high];
+    const int q = (word >> (4 * (e >> 1) + 16 * (e & 1))) & 15;
+    const float d = __half2float(reinterpret_cast<const __half*>(u + 1024)[8 * g + 2 * b + high]);
+    if (!kMin) return d * static_cast<float>(q - 8);
+    return d * static_cast<float>(q) + __half2float(reinterpret_cast<const __half*>(u + 1152)[8 * g + 2 * b + high]);
+}
+// What a row's infinities and NaN add to output n.
+template <bool kMin>
+__device__ __noinline__ float odd_terms(const Q4Args& a, int64_t n, int m) {
+    float v = 0.f;
+    for (int64_t k = 0; k < a.x_cols; ++k) {
+        const int64_t i = m * a.ldx + k;
+        const float x = a.x_type == B2Q_TYPE_F32   ? static_cast<const float*>(a.x)[i]
+                        : a.x_type == B2Q_TYPE_F16 ? to_f32(static_cast<const __half*>(a.x)[i])
+                                                   : to_f32(static_cast<const __nv_bfloat16*>(a.x)[i]);
+        if (!is_finite(x)) v += weight_at<kMin>(a, n, k) * x;
+    }
+    return v;
+}
+
+template <bool kMin, int kN>
+__global__ void __launch_bounds__(kThreads, kN == 1 ? 2 : 1) mul_vec_q4_kernel(const __grid_constant__ Q4Args a) {
     constexpr int kUnit = unit_bytes(kMin);
-    constexpr int kRedPitch = 8 * kN + 1, kRedWarp = 16 * kRedPitch + 1;   // odd: no bank conflicts either way
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ RowState st;
+    __shared__ uint64_t s_full[kWarps][kMaxStages];
+    __shared__ uint32_t s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int split = a.split, sub = warp % split, group = warp / split, groups = kWarps / split;
     const int first = blockIdx.x * groups + group, step = gridDim.x * groups;
     const int per_tile = (a.units - sub + split - 1) / split;   // units of this warp in each of its tiles
 
-    // ---- the weights' stream: unit `u` of tile `lt`, kStages - 1 units ahead ----
-    const uint32_t ring = smem_u32(smem + a.ring_at) + warp * kStages * kUnit;
-    const uint8_t* src = a.w;
-    int lt = first, lu = sub, slot = 0;
-    auto issue = [&]() {
-        if (lt < a.tiles) {
-            const uint8_t* p = src + (static_cast<int64_t>(lt) * a.units + lu) * kUnit + lane * 16;
-            const uint32_t dst = ring + slot * kUnit + lane * 16;
-            cp_async_16(dst, p, true);
-            if (lane < (kUnit - 512) / 16) cp_async_16(dst + 512, p + 512, true);
-            lu += split;
-            if (lu >= a.units) {
-                lu = sub;
-                lt += step;
-            }
+    // ---- the weights' stream: lane 0 asks for a unit as soon as its slot is free ----
+    const int ring_off = a.ring_at + warp * a.stages * kUnit;
+    const uint32_t full = smem_u32(s_full[warp]), ring = smem_u32(smem) + ring_off;
+    const uint8_t* src = a.w + (static_cast<int64_t>(first) * a.units + sub) * kUnit;
+    const int64_t unit_step = static_cast<int64_t>(split) * kUnit;
+    const int64_t tile_step = (static_cast<int64_t>(step) * a.units - static_cast<int64_t>(per_tile) * split) * kUnit;
+    int left = first < a.tiles ? (a.tiles - first + step - 1) / step * per_tile : 0;   // units still to ask for
+    int left_tile = per_tile;
+    auto issue = [&](int slot) {   // lane 0
+        if (left <= 0) return;
+        mbar_arrive_expect_tx(full + 8 * slot, kUnit);
+        bulk_load(ring + slot * kUnit, src, kUnit, full + 8 * slot);
+        --left;
+        src += unit_step;
+        if (--left_tile == 0) {
+            left_tile = per_tile;
+            src += tile_step;
         }
-        cp_commit();
-        slot = slot + 1 == kStages ? 0 : slot + 1;
     };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue();
-    stage_x<Tx, kMin>(a, smem);
+    if (lane == 0) {
+        for (int i = 0; i < a.stages; ++i) mbar_init(full + 8 * i, 1);
+        fence_barrier_init();
+        for (int i = 0; i < a.stages; ++i) issue(i);
+    }
+    if (tid < kMaxRows) st.peak[tid] = 0;
+    if (tid == 0) st.odd = s_abort = 0;
+    __syncthreads();
+    if (a.x_type == B2Q_TYPE_F32) stage_x<float, kMin>(a, smem, st);
+    else if (a.x_type == B2Q_TYPE_F16) stage_x<__half, kMin>(a, smem, st);
+    else stage_x<__nv_bfloat16, kMin>(a, smem, st);
     __syncthreads();
 
-    // this lane's operand columns and, for Q4_1, the sums that its outputs take
-    const int cols = a.rows * kPieces;
-    const float* sums = reinterpret_cast<const float*>(smem + a.sum_at);
-    uint32_t xb[kN];
-    bool has[kN];
+    // This lane's operand columns.  A column that no row has computes on the
+    // first one's values; its results are not read.
+    const int cols = a.rows * a.pieces, pairs = (a.rows + 1) / 2;
+    int x0[kN], sum0[kN], sum_step[kN];   // sums: Q4_0 of columns 2 t, 2 t + 1, Q4_1 of this lane's column, block t
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-        has[n] = n * 8 + g < cols;
-        xb[n] = smem_u32(smem) + (has[n] ? n * 8 + g : 0) * a.pitch + t * 16;
+        const int col = n * 8 + g < cols ? n * 8 + g : 0, pair = n * 4 + t;
+        x0[n] = col * a.pitch + t * 16 + sub * 256;
+        if constexpr (kMin) {
+            const bool own = n * 8 + g < a.rows;
+            sum_step[n] = own ? a.rows * 32 : 0;
+            sum0[n] = a.sum_at + (own ? (sub * a.rows + col) * 32 : a.units * a.rows * 32) + t * 8;
+        } else {
+            sum_step[n] = pair < pairs ? pairs * 32 : 0;
+            sum0[n] = a.sum_at + (pair < pairs ? (sub * pairs + pair) * 32 : a.units * pairs * 32);
+        }
     }
-    int out_slot = 0;
-    for (int tile = first; tile < a.tiles; tile += step) {
-        float acc[kN][4] = {};
-        int u = sub;
-        for (int j = 0; j < per_tile; ++j, u += split) {
-            issue();
-            cp_wait<kStages - 1>();
-            __syncwarp();
-            const uint32_t at = ring + out_slot * kUnit;
-            out_slot = out_slot + 1 == kStages ? 0 : out_slot + 1;
-            const uint4 w4 = lds_128(at + lane * 16);
-            const uint2 d4 = lds_64(at + 512 + g * 8);
-            uint2 m4 = make_uint2(0, 0);
-            if constexpr (kMin) m4 = lds_64(at + 576 + g * 8);
+    int slot = 0, buf = 0;
+    uint32_t phase = 0;
+    for (int tile = first; tile < a.tiles; tile += step, buf ^= 1) {
+        float acc[kN][4] = {}, accm[kN][4] = {};   // sums with d, sums with m
+        int xo = 0, so[kN];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                uint32_t lo[4], hi[4];
-                unpack_q4<T, kMin>(b ? w4.z : w4.x, lo);
-                unpack_q4<T, kMin>(b ? w4.w : w4.y, hi);
-                const float2 d = unpack2<__half>(b ? d4.y : d4.x);
-                const float2 mn = unpack2<__half>(b ? m4.y : m4.x);
+        for (int n = 0; n < kN; ++n) so[n] = sum0[n];
+        for (int j = 0; j < per_tile; ++j, xo += split * 256) {
+            // A copy that never comes is reported; the warp goes on over what the slot
+            // holds, so that no other warp waits for it.
+            if (!mbar_test_wait(full + 8 * slot, phase) && !mbar_wait(full + 8 * slot, phase, &s_abort, a.timeout_ns)) {
+                report(a.err, kDevTimeoutFull);
+                *static_cast<volatile uint32_t*>(&s_abort) = 1;
+                left = 0;
+            }
+            const uint8_t* use = smem + ring_off + slot * kUnit;
+            const uint4 wa = *reinterpret_cast<const uint4*>(use + lane * 16);
+            const uint4 wb = *reinterpret_cast<const uint4*>(use + 512 + lane * 16);
+            const uint4 dd = *reinterpret_cast<const uint4*>(use + 1024 + g * 16);
+            uint32_t mm = 0;
+            if constexpr (kMin) mm = *reinterpret_cast<const uint32_t*>(use + 1152 + g * 16 + t * 4);
+            __syncwarp();   // all lanes have their words: the slot may be filled again
+            if (lane == 0) issue(slot);
+            if (++slot == a.stages) {
+                slot = 0;
+                phase ^= 1;
+            }
+            const uint32_t w8[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+            const uint32_t d4[4] = {dd.x, dd.y, dd.z, dd.w};
+            if constexpr (kMin) {   // block t's m three times in k, against the pieces of its X
+                const uint32_t m0 = __byte_perm(mm, 0, 0x1010), m8 = __byte_perm(mm, 0, 0x3232);
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
-                    uint4 x4 = make_uint4(0, 0, 0, 0);
-                    if (has[n]) x4 = lds_128(xb[n] + (2 * u + b) * 64);
+                    const uint2 xp = *reinterpret_cast<const uint2*>(smem + so[n]);
+                    mma_16816<__half>(accm[n], m0, m8, m0, m8, xp.x, xp.y);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                uint32_t lo[4], hi[4];
+                unpack_q4(w8[2 * b], lo);
+                unpack_q4(w8[2 * b + 1], hi);
+                const float2 d = unpack2<__half>(d4[b]);
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+                    const uint4 xv = *reinterpret_cast<const uint4*>(smem + x0[n] + xo + b * 64);
+                    float2 x = make_float2(0.f, 0.f);
+                    if constexpr (!kMin) x = *reinterpret_cast<const float2*>(smem + so[n] + b * 8);
                     float s[4];
-                    mma_16816_from0<T>(s, lo[0], hi[0], lo[1], hi[1], x4.x, x4.y);
-                    mma_16816<T>(s, lo[2], hi[2], lo[3], hi[3], x4.z, x4.w);
+                    mma_16816_start(s, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y, x.x, x.y);
+                    mma_16816<__half>(s, lo[2], hi[2], lo[3], hi[3], xv.z, xv.w);
                     acc[n][0] = fmaf(d.x, s[0], acc[n][0]);
                     acc[n][1] = fmaf(d.x, s[1], acc[n][1]);
                     acc[n][2] = fmaf(d.y, s[2], acc[n][2]);
                     acc[n][3] = fmaf(d.y, s[3], acc[n][3]);
-                    if constexpr (kMin) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int col = n * 8 + 2 * t + e;
-                            if (col < cols && col % kPieces == 0) {
-                                const float xs = sums[(2 * u + b) * a.rows + col / kPieces];
-                                acc[n][e] = fmaf(mn.x, xs, acc[n][e]);
-                                acc[n][2 + e] = fmaf(mn.y, xs, acc[n][2 + e]);
-                            }
-                        }
-                    }
                 }
             }
-            __syncwarp();   // the slot may be filled again
+#pragma unroll
+            for (int n = 0; n < kN; ++n) so[n] += split * sum_step[n];
         }
-        // ---- add up the warps of the tile and the pieces, in order ----
-        float* red = reinterpret_cast<float*>(smem + a.red_at) + warp * kRedWarp;
+        // ---- add up the tile's warps and the pieces, in order; two buffers, so that
+        // one meeting a tile suffices ----
+        constexpr int kRedPitch = red_pitch(kN), kRedWarp = 16 * kRedPitch;
+        float* all = reinterpret_cast<float*>(smem + a.red_at) + (buf * kWarps + group * split) * kRedWarp;
+        float* red = all + sub * kRedWarp + g * kRedPitch + 2 * t;
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) red[(g + 8 * (e >> 1)) * kRedPitch + n * 8 + 2 * t + (e & 1)] = acc[n][e];
-        auto meet = [&]() {
-            if (split == 1) __syncwarp();
-            else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(split * 32) : "memory");
-        };
-        meet();
-        const float* all = reinterpret_cast<const float*>(smem + a.red_at) + group * split * kRedWarp;
-        const int e = tid - group * split * 32, part = e % split;
-        for (int base = 0; base < 16 * a.rows; base += 32) {
-            const int o = base + e / split, row = o & 15, m = o >> 4;
-            const int64_t n = static_cast<int64_t>(tile) * 16 + row;
-            const bool in = o < 16 * a.rows && n < a.N;
-            float v = 0.f;
-            if (in)
-#pragma unroll
-                for (int p = 0; p < kPieces; ++p) v += all[part * kRedWarp + row * kRedPitch + m * kPieces + p];
-            for (int x = 1; x < split; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
-            if (in && part == 0) {
-                if (a.bias) v += a.bias[n];
-                if (a.residual) v += a.residual[m * a.ldy + n];
-                if (a.y_f32) static_cast<float*>(a.y)[m * a.ldy + n] = v;
-                else static_cast<Tx*>(a.y)[m * a.ldy + n] = from_f32<Tx>(v);
+            for (int e = 0; e < 4; ++e) {
+                // Q4_1: the operands of m were scaled by 2^-5, those of d by 2^-24
+                const float v = kMin ? fmaf(accm[n][e], 1.9073486328125e-6f, acc[n][e]) : acc[n][e];
+                red[8 * (e >> 1) * kRedPitch + n * 8 + (e & 1)] = v;
             }
+        if (split == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(split * 32) : "memory");
+        for (int o = tid - group * split * 32; o < 16 * a.rows; o += split * 32) {
+            const int row = o & 15, m = o >> 4, n = tile * 16 + row;
+            if (n >= a.N) continue;
+            const float* p = all + row * kRedPitch + m;
+            float v = 0.f;
+#pragma unroll 4
+            for (int w = 0; w < split; ++w, p += kRedWarp) {
+                float s = p[0];
+                if (a.pieces == 3) s += p[a.rows] + p[2 * a.rows];
+                v += s;
+            }
+            const int e = 24 - shift_of(st.peak[m]);
+            v = v * pow2(e >> 1) * pow2(e - (e >> 1));
+            if ((st.odd >> m) & 1) v += odd_terms<kMin>(a, n, m);
+            const int64_t at = m * a.ldy + n;
+            if (a.bias) v += a.bias[n];
+            if (a.residual) v += a.residual[at];
+            if (a.y_f32) static_cast<float*>(a.y)[at] = v;
+            else if (a.x_type == B2Q_TYPE_F16) static_cast<__half*>(a.y)[at] = from_f32<__half>(v);
+            else static_cast<__nv_bfloat16*>(a.y)[at] = from_f32<__nv_bfloat16>(v);
         }
-        meet();
     }
 }
 
 // ------------------------------------------------------------------ launch
-// Warps per row tile: the split whose slowest warp streams the fewest units;
-// of equal ones the smallest, which meets least often.
-int split_of(int64_t tiles, int units, int sms) {
+// Warps per row tile: the split whose slowest warp has the least to do, in half
+// units: two a unit that it streams, and per tile one for its end, two where
+// warps meet there.
+int split_of(int64_t tiles, int units, int ctas) {
     int best = 1;
     int64_t best_cost = INT64_MAX;
     for (int s = 1; s <= kWarps && s <= units; s *= 2) {
-        const int64_t groups = static_cast<int64_t>(sms) * (kWarps / s);
-        const int64_t cost = (tiles + groups - 1) / groups * ((units + s - 1) / s);
+        const int64_t groups = static_cast<int64_t>(ctas) * (kWarps / s);
+        const int64_t cost = (tiles + groups - 1) / groups * (2 * ((units + s - 1) / s) + (s > 1 ? 2 : 1));
         if (cost < best_cost) {
             best = s;
             best_cost = cost;
@@ -350,25 +504,29 @@ int split_of(int64_t tiles, int units, int sms) {
 }
 
 struct Q4Plan {
-    int stages, pitch, ring_at, red_at, sum_at, bytes;
+    int stages, ctas, pitch, ring_at, red_at, sum_at, bytes;
 };
-// Shared memory of a launch over `rows` activation rows; stages 0 where it does not fit.
+// Shared memory of a launch over `rows` activation rows; stages 0 where it does
+// not fit.  Two CTAs of an SM hide more than one, so they come first where the
+// registers allow them (n_tiles 1) and three stages of each ring fit.
 Q4Plan plan_of(int rows, int pieces, int n_tiles, int units, bool min) {
-    for (int stages : {8, 4}) {
-        Q4Plan p;
-        p.stages = stages;
-        p.pitch = units * 128 + 64;   // 64 bytes off a multiple of 128: eight columns' chunks miss one another's banks
-        p.ring_at = static_cast<int>(round_up(rows * pieces * p.pitch, 128));
-        p.red_at = p.ring_at + kWarps * stages * unit_bytes(min);
-        p.sum_at = p.red_at + static_cast<int>(round_up(kWarps * (16 * (8 * n_tiles + 1) + 1) * 4, 128));
-        p.bytes = p.sum_at + (min ? units * 2 * rows * 4 : 0);
-        if (p.bytes <= kSmemMax) return p;
-    }
-    return Q4Plan{};
+    Q4Plan p{};
+    p.pitch = units * 256 + 64;   // 64 bytes off a multiple of 128: eight columns' chunks miss one another's banks
+    p.red_at = static_cast<int>(round_up(rows * pieces * p.pitch, 128));
+    p.sum_at = p.red_at + static_cast<int>(round_up(2 * kWarps * 16 * red_pitch(n_tiles) * 4, 128));
+    const int sums = (units * (min ? rows : (rows + 1) / 2) + 1) * 32;
+    p.ring_at = p.sum_at + static_cast<int>(round_up(sums, 128));
+    const int stage = kWarps * unit_bytes(min);
+    p.ctas = n_tiles == 1 && p.ring_at + 3 * stage <= kSmemHalf ? 2 : 1;
+    const int room = ((p.ctas == 2 ? kSmemHalf : kSmemMax) - p.ring_at) / stage;
+    p.stages = room < kMaxStages ? room : kMaxStages;
+    if (p.stages < 1) p.stages = 0;
+    p.bytes = p.ring_at + p.stages * stage;
+    return p;
 }
 // Operand tiles (of 8 columns) that a launch over `rows` rows is built for, 0 = too many.
 int n_tiles_of(int rows, int pieces) {
-    const int n = (rows * pieces + 7) / 8;
+    const int n = rows <= kMaxRows ? (rows * pieces + 7) / 8 : 5;
     return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 0;
 }
 
@@ -398,7 +556,7 @@ b2q_status b2q_weight_q4_register(const void* blocks, int32_t ggml_type, int64_t
     w->type = ggml_type;
     w->device = ds->device;
     w->tiles = (N + 15) / 16;
-    w->units = (K + 63) / 64;
+    w->units = (K + 127) / 128;
     void* staged = nullptr;
     const size_t src_bytes = static_cast<size_t>(N - 1) * row_bytes + K / 32 * (min ? 20 : 18);
     b2q_status st = B2Q_OK;
@@ -465,25 +623,24 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
     // the most rows that a launch takes (operand tiles and shared memory), then as even launches as that allows
     int most = 1;
     while (most < M && n_tiles_of(most + 1, pieces) &&
-           plan_of(most + 1, pieces, n_tiles_of(most + 1, pieces), units, min).stages)
+           plan_of(most + 1, pieces, n_tiles_of(most + 1, pieces), units, min).stages >= 2)
         ++most;
     const int64_t launches = (M + most - 1) / most;
-    const int split = split_of(w->tiles, units, ds->num_sms);
-    const int groups = kWarps / split;
-    const int64_t want = (w->tiles + groups - 1) / groups;
-    const unsigned grid = static_cast<unsigned>(want < ds->num_sms ? want : ds->num_sms);
     for (int64_t i = 0, m0 = 0; i < launches; ++i) {
         const int rows = static_cast<int>((M - m0 + launches - i - 1) / (launches - i));
         const int n_tiles = n_tiles_of(rows, pieces);
         const Q4Plan p = plan_of(rows, pieces, n_tiles, units, min);
         if (!p.stages) return set_error(B2Q_ERR_SHAPE, "an activation row does not fit shared memory");
-        auto go = [&](auto tx, auto mn, auto nt, auto stages) {
-            using Tx = decltype(tx);
-            Q4Args<Tx> a{w->packed, w->N, static_cast<int>(w->tiles), units, split,
-                         reinterpret_cast<const Tx*>(static_cast<const uint8_t*>(x) + m0 * ldx * es), rows, x_cols, ldx,
-                         static_cast<uint8_t*>(y) + m0 * ldy * ys, ldy, y_dtype == B2Q_TYPE_F32, bias,
-                         residual ? residual + m0 * ldy : nullptr, p.pitch, p.ring_at, p.red_at, p.sum_at};
-            auto* kernel = mul_vec_q4_kernel<Tx, decltype(mn)::value, decltype(nt)::value, decltype(stages)::value>;
+        const int split = split_of(w->tiles, units, ds->num_sms * p.ctas);
+        const int64_t want = (w->tiles + kWarps / split - 1) / (kWarps / split);
+        const unsigned grid = static_cast<unsigned>(want < ds->num_sms * p.ctas ? want : ds->num_sms * p.ctas);
+        const Q4Args a{w->packed, w->N, static_cast<int>(w->tiles), units, split,
+                       static_cast<const uint8_t*>(x) + m0 * ldx * es, x_dtype, pieces, rows, x_cols, ldx,
+                       static_cast<uint8_t*>(y) + m0 * ldy * ys, ldy, y_dtype == B2Q_TYPE_F32, bias,
+                       residual ? residual + m0 * ldy : nullptr, p.pitch, p.ring_at, p.stages, p.red_at, p.sum_at,
+                       ds->timeout_ns, ds->err};
+        auto go = [&](auto mn, auto nt) {
+            auto* kernel = mul_vec_q4_kernel<decltype(mn)::value, decltype(nt)::value>;
             b2q_status st = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                             kSmemMax), "4-bit product shared memory");
             if (st) return st;
@@ -491,21 +648,12 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
             count_launch();
             return cuda_check(cudaGetLastError(), "4-bit product launch");
         };
-        auto with_stages = [&](auto tx, auto mn, auto nt) {
-            return p.stages == 8 ? go(tx, mn, nt, std::integral_constant<int, 8>{})
-                                 : go(tx, mn, nt, std::integral_constant<int, 4>{});
+        auto with_tiles = [&](auto mn) {
+            return n_tiles == 1   ? go(mn, std::integral_constant<int, 1>{})
+                   : n_tiles == 2 ? go(mn, std::integral_constant<int, 2>{})
+                                  : go(mn, std::integral_constant<int, 4>{});
         };
-        auto with_tiles = [&](auto tx, auto mn) {
-            return n_tiles == 1   ? with_stages(tx, mn, std::integral_constant<int, 1>{})
-                   : n_tiles == 2 ? with_stages(tx, mn, std::integral_constant<int, 2>{})
-                                  : with_stages(tx, mn, std::integral_constant<int, 4>{});
-        };
-        auto with_min = [&](auto tx) {
-            return min ? with_tiles(tx, std::true_type{}) : with_tiles(tx, std::false_type{});
-        };
-        const b2q_status st = x_dtype == B2Q_TYPE_F32   ? with_min(float{})
-                              : x_dtype == B2Q_TYPE_F16 ? with_min(__half{})
-                                                        : with_min(__nv_bfloat16{});
+        const b2q_status st = min ? with_tiles(std::true_type{}) : with_tiles(std::false_type{});
         if (st) return st;
         m0 += rows;
     }
