@@ -29,9 +29,10 @@
 // The weights are laid out at registration in the order the lanes want them:
 // per 16 rows a run of units of 128 columns, each 1024 bytes of nibbles (lane l of
 // the warp: twice 16 bytes) and the blocks' scales (128 bytes; Q4_1: 128 more for
-// m).  A warp streams units through its own ring, one bulk copy each, which runs
-// on across row tiles; the activations sit in shared memory for the whole launch
-// (a fixed grid of one or two CTAs of 16 warps per SM).  `split` warps share a row
+// m).  A warp streams units through its own ring of asynchronous copies, which runs
+// on across row tiles (with one bulk copy and a barrier per unit the stream took 64
+// of 176 instructions a unit); the activations sit in shared memory for the whole
+// launch (a fixed grid of one or two CTAs of 16 warps per SM).  `split` warps share a row
 // tile, each taking every split-th unit, and add up in a fixed order.
 #include "b2q_decode.cuh"
 
@@ -52,10 +53,9 @@ constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxRows = 32;        // of one launch
 constexpr int kMaxK = 28672;        // three pieces of a row still fit shared memory next to the rings
-constexpr int kSmemMax = 227 * 1024 - 2048;   // next to the static part
+constexpr int kSmemMax = 227 * 1024 - 512;   // next to the static part
 constexpr int kSmemHalf = 111 * 1024;   // two CTAs of an SM
 
-constexpr int kMaxStages = 8;
 constexpr int unit_bytes(bool min) { return min ? 1280 : 1152; }
 constexpr int red_pitch(int n_tiles) { return 8 * n_tiles + 1; }   // odd: rows in different banks
 
@@ -110,9 +110,7 @@ struct Q4Args {
     int64_t ldy;
     bool y_f32;
     const float *bias, *residual;
-    int pitch, ring_at, stages, red_at, sum_at;   // shared memory: bytes of an operand column, parts' offsets
-    uint64_t timeout_ns;
-    uint32_t* err;
+    int pitch, ring_at, red_at, sum_at;   // shared memory: bytes of an operand column, parts' offsets
 };
 
 // The word's four pairs of a lane as fp16 operands: q 2^-24, q 2^-20, q 2^-24, q 2^-20.
@@ -325,44 +323,42 @@ __device__ __noinline__ float odd_terms(const Q4Args& a, int64_t n, int m) {
     return v;
 }
 
-template <bool kMin, int kN>
+template <bool kMin, int kN, int kStages>
 __global__ void __launch_bounds__(kThreads, kN == 1 ? 2 : 1) mul_vec_q4_kernel(const __grid_constant__ Q4Args a) {
     constexpr int kUnit = unit_bytes(kMin);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ RowState st;
-    __shared__ uint64_t s_full[kWarps][kMaxStages];
-    __shared__ uint32_t s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int split = a.split, sub = warp % split, group = warp / split, groups = kWarps / split;
     const int first = blockIdx.x * groups + group, step = gridDim.x * groups;
     const int per_tile = (a.units - sub + split - 1) / split;   // units of this warp in each of its tiles
 
-    // ---- the weights' stream: lane 0 asks for a unit as soon as its slot is free ----
-    const int ring_off = a.ring_at + warp * a.stages * kUnit;
-    const uint32_t full = smem_u32(s_full[warp]), ring = smem_u32(smem) + ring_off;
-    const uint8_t* src = a.w + (static_cast<int64_t>(first) * a.units + sub) * kUnit;
+    // ---- the weights' stream: a unit is asked for as soon as its slot is free ----
+    const int ring = a.ring_at + warp * kStages * kUnit;
+    const uint8_t* src = a.w + (static_cast<int64_t>(first) * a.units + sub) * kUnit + lane * 16;
     const int64_t unit_step = static_cast<int64_t>(split) * kUnit;
     const int64_t tile_step = (static_cast<int64_t>(step) * a.units - static_cast<int64_t>(per_tile) * split) * kUnit;
     int left = first < a.tiles ? (a.tiles - first + step - 1) / step * per_tile : 0;   // units still to ask for
     int left_tile = per_tile;
-    auto issue = [&](int slot) {   // lane 0
-        if (left <= 0) return;
-        mbar_arrive_expect_tx(full + 8 * slot, kUnit);
-        bulk_load(ring + slot * kUnit, src, kUnit, full + 8 * slot);
-        --left;
-        src += unit_step;
-        if (--left_tile == 0) {
-            left_tile = per_tile;
-            src += tile_step;
+    auto issue = [&](int slot) {
+        if (left > 0) {
+            const uint32_t dst = smem_u32(smem) + slot + lane * 16;
+            cp_async_16(dst, src, true);
+            cp_async_16(dst + 512, src + 512, true);
+            if (lane < (kUnit - 1024) / 16) cp_async_16(dst + 1024, src + 1024, true);
+            --left;
+            src += unit_step;
+            if (--left_tile == 0) {
+                left_tile = per_tile;
+                src += tile_step;
+            }
         }
+        cp_commit();
     };
-    if (lane == 0) {
-        for (int i = 0; i < a.stages; ++i) mbar_init(full + 8 * i, 1);
-        fence_barrier_init();
-        for (int i = 0; i < a.stages; ++i) issue(i);
-    }
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) issue(ring + i * kUnit);
     if (tid < kMaxRows) st.peak[tid] = 0;
-    if (tid == 0) st.odd = s_abort = 0;
+    if (tid == 0) st.odd = 0;
     __syncthreads();
     if (a.x_type == B2Q_TYPE_F32) stage_x<float, kMin>(a, smem, st);
     else if (a.x_type == B2Q_TYPE_F16) stage_x<__half, kMin>(a, smem, st);
@@ -386,33 +382,25 @@ __global__ void __launch_bounds__(kThreads, kN == 1 ? 2 : 1) mul_vec_q4_kernel(c
             sum0[n] = a.sum_at + (pair < pairs ? (sub * pairs + pair) * 32 : a.units * pairs * 32);
         }
     }
-    int slot = 0, buf = 0;
-    uint32_t phase = 0;
+    int slot = ring, buf = 0;
     for (int tile = first; tile < a.tiles; tile += step, buf ^= 1) {
         float acc[kN][4] = {}, accm[kN][4] = {};   // sums with d, sums with m
         int xo = 0, so[kN];
 #pragma unroll
         for (int n = 0; n < kN; ++n) so[n] = sum0[n];
         for (int j = 0; j < per_tile; ++j, xo += split * 256) {
-            // A copy that never comes is reported; the warp goes on over what the slot
-            // holds, so that no other warp waits for it.
-            if (!mbar_test_wait(full + 8 * slot, phase) && !mbar_wait(full + 8 * slot, phase, &s_abort, a.timeout_ns)) {
-                report(a.err, kDevTimeoutFull);
-                *static_cast<volatile uint32_t*>(&s_abort) = 1;
-                left = 0;
-            }
-            const uint8_t* use = smem + ring_off + slot * kUnit;
+            cp_wait<kStages - 1>();
+            __syncwarp();   // every lane's part of the unit has come
+            const uint8_t* use = smem + slot;
             const uint4 wa = *reinterpret_cast<const uint4*>(use + lane * 16);
             const uint4 wb = *reinterpret_cast<const uint4*>(use + 512 + lane * 16);
             const uint4 dd = *reinterpret_cast<const uint4*>(use + 1024 + g * 16);
             uint32_t mm = 0;
             if constexpr (kMin) mm = *reinterpret_cast<const uint32_t*>(use + 1152 + g * 16 + t * 4);
             __syncwarp();   // all lanes have their words: the slot may be filled again
-            if (lane == 0) issue(slot);
-            if (++slot == a.stages) {
-                slot = 0;
-                phase ^= 1;
-            }
+            issue(slot);
+            slot += kUnit;
+            if (slot == ring + kStages * kUnit) slot = ring;
             const uint32_t w8[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
             const uint32_t d4[4] = {dd.x, dd.y, dd.z, dd.w};
             if constexpr (kMin) {   // block t's m three times in k, against the pieces of its X
@@ -507,8 +495,8 @@ struct Q4Plan {
     int stages, ctas, pitch, ring_at, red_at, sum_at, bytes;
 };
 // Shared memory of a launch over `rows` activation rows; stages 0 where it does
-// not fit.  Two CTAs of an SM hide more than one, so they come first where the
-// registers allow them (n_tiles 1) and three stages of each ring fit.
+// not fit.  Two CTAs of an SM with four stages hide more than one with eight, so
+// they come first where the registers allow them (n_tiles 1).
 Q4Plan plan_of(int rows, int pieces, int n_tiles, int units, bool min) {
     Q4Plan p{};
     p.pitch = units * 256 + 64;   // 64 bytes off a multiple of 128: eight columns' chunks miss one another's banks
@@ -516,12 +504,15 @@ Q4Plan plan_of(int rows, int pieces, int n_tiles, int units, bool min) {
     p.sum_at = p.red_at + static_cast<int>(round_up(2 * kWarps * 16 * red_pitch(n_tiles) * 4, 128));
     const int sums = (units * (min ? rows : (rows + 1) / 2) + 1) * 32;
     p.ring_at = p.sum_at + static_cast<int>(round_up(sums, 128));
-    const int stage = kWarps * unit_bytes(min);
-    p.ctas = n_tiles == 1 && p.ring_at + 3 * stage <= kSmemHalf ? 2 : 1;
-    const int room = ((p.ctas == 2 ? kSmemHalf : kSmemMax) - p.ring_at) / stage;
-    p.stages = room < kMaxStages ? room : kMaxStages;
-    if (p.stages < 1) p.stages = 0;
-    p.bytes = p.ring_at + p.stages * stage;
+    for (int variant = n_tiles == 1 ? 0 : 1; variant < 4; ++variant) {
+        constexpr int kStagesOf[] = {4, 8, 4, 2};   // the last for the longest rows only
+        p.bytes = p.ring_at + kWarps * unit_bytes(min) * kStagesOf[variant];
+        p.ctas = variant == 0 ? 2 : 1;
+        if (p.bytes <= (p.ctas == 2 ? kSmemHalf : kSmemMax)) {
+            p.stages = kStagesOf[variant];
+            break;
+        }
+    }
     return p;
 }
 // Operand tiles (of 8 columns) that a launch over `rows` rows is built for, 0 = too many.
@@ -623,7 +614,7 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
     // the most rows that a launch takes (operand tiles and shared memory), then as even launches as that allows
     int most = 1;
     while (most < M && n_tiles_of(most + 1, pieces) &&
-           plan_of(most + 1, pieces, n_tiles_of(most + 1, pieces), units, min).stages >= 2)
+           plan_of(most + 1, pieces, n_tiles_of(most + 1, pieces), units, min).stages >= 4)
         ++most;
     const int64_t launches = (M + most - 1) / most;
     for (int64_t i = 0, m0 = 0; i < launches; ++i) {
@@ -637,10 +628,9 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
         const Q4Args a{w->packed, w->N, static_cast<int>(w->tiles), units, split,
                        static_cast<const uint8_t*>(x) + m0 * ldx * es, x_dtype, pieces, rows, x_cols, ldx,
                        static_cast<uint8_t*>(y) + m0 * ldy * ys, ldy, y_dtype == B2Q_TYPE_F32, bias,
-                       residual ? residual + m0 * ldy : nullptr, p.pitch, p.ring_at, p.stages, p.red_at, p.sum_at,
-                       ds->timeout_ns, ds->err};
-        auto go = [&](auto mn, auto nt) {
-            auto* kernel = mul_vec_q4_kernel<decltype(mn)::value, decltype(nt)::value>;
+                       residual ? residual + m0 * ldy : nullptr, p.pitch, p.ring_at, p.red_at, p.sum_at};
+        auto go = [&](auto mn, auto nt, auto stages) {
+            auto* kernel = mul_vec_q4_kernel<decltype(mn)::value, decltype(nt)::value, decltype(stages)::value>;
             b2q_status st = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                             kSmemMax), "4-bit product shared memory");
             if (st) return st;
@@ -648,10 +638,15 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
             count_launch();
             return cuda_check(cudaGetLastError(), "4-bit product launch");
         };
+        auto with_stages = [&](auto mn, auto nt) {
+            return p.stages == 8   ? go(mn, nt, std::integral_constant<int, 8>{})
+                   : p.stages == 4 ? go(mn, nt, std::integral_constant<int, 4>{})
+                                   : go(mn, nt, std::integral_constant<int, 2>{});
+        };
         auto with_tiles = [&](auto mn) {
-            return n_tiles == 1   ? go(mn, std::integral_constant<int, 1>{})
-                   : n_tiles == 2 ? go(mn, std::integral_constant<int, 2>{})
-                                  : go(mn, std::integral_constant<int, 4>{});
+            return n_tiles == 1   ? with_stages(mn, std::integral_constant<int, 1>{})
+                   : n_tiles == 2 ? with_stages(mn, std::integral_constant<int, 2>{})
+                                  : with_stages(mn, std::integral_constant<int, 4>{});
         };
         const b2q_status st = min ? with_tiles(std::true_type{}) : with_tiles(std::false_type{});
         if (st) return st;
