@@ -2,6 +2,7 @@
 // cache as a kernel sees it, and the check of a caller's cache description.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -125,6 +126,18 @@ struct CacheView {
     int64_t page_stride, head_stride, token_stride;
     int n_pages, page_shift, page_mask;
 };
+
+// Lets `kernel` use `bytes` of dynamic shared memory: once per device, `done` (one
+// per kernel, device d its bit d) keeps the call off the launch path.
+template <class Kernel>
+inline b2q_status allow_smem(Kernel* kernel, int bytes, std::atomic<uint64_t>& done, int device) {
+    const uint64_t bit = uint64_t(1) << device;
+    if (done.load(std::memory_order_acquire) & bit) return B2Q_OK;
+    const b2q_status st = cuda_check(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory of a kernel");
+    if (!st) done.fetch_or(bit, std::memory_order_release);
+    return st;
+}
 
 // B2Q_OK and the strides filled in, or the error of a bad description.
 inline b2q_status check_cache(const b2q_kv_cache* in, b2q_kv_cache* c) {

@@ -607,8 +607,8 @@ b2q_status b2q_attention_paged(const void* q, int64_t ldq, int64_t n_rows, int32
                            static_cast<uint32_t*>(scratch),
                            reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + kCounterBytes), ds->err};
             auto* kernel = paged_kernel<T, To, DP, kRows>;
-            b2q_status s = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                           static_cast<int>(smem)), "paged attention shared memory");
+            static std::atomic<uint64_t> allowed{0};
+            const b2q_status s = allow_smem(kernel, static_cast<int>(smem), allowed, ds->device);
             if (s) return s;
             kernel<<<grid_of(ds->num_sms, Shape<DP>::kCtas), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
             count_launch();

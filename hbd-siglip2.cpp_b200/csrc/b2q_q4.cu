@@ -32,7 +32,7 @@
 // m).  A warp streams units through its own ring of asynchronous copies, which runs
 // on across row tiles (with one bulk copy and a barrier per unit the stream took 64
 // of 176 instructions a unit); the activations sit in shared memory for the whole
-// launch (a fixed grid of one or two CTAs of 16 warps per SM).  `split` warps share a row
+// launch (a fixed grid of one CTA of 16 or 32 warps per SM).  `split` warps share a row
 // tile, each taking every split-th unit, and add up in a fixed order.
 #include "b2q_decode.cuh"
 
@@ -49,15 +49,16 @@ struct b2q_weight_q4 {
 namespace b2q {
 namespace {
 
-constexpr int kWarps = 16;
-constexpr int kThreads = kWarps * 32;
+// Warps of a CTA (one per SM): 32 where 64 registers suffice (one operand tile) and
+// an SM has more than four units for each of 16 warps; else 16, whose start takes
+// 0.7 us less (1 x 1152 x 4320: 5.8 against 7.0 us).
+int warps_of(int n_tiles, int64_t units_per_sm) { return n_tiles == 1 && units_per_sm > 64 ? 32 : 16; }
 constexpr int kMaxRows = 32;        // of one launch
 constexpr int kMaxK = 28672;        // three pieces of a row still fit shared memory next to the rings
-constexpr int kSmemMax = 227 * 1024 - 512;   // next to the static part
-constexpr int kSmemHalf = 111 * 1024;   // two CTAs of an SM
+constexpr int kSmemMax = 227 * 1024 - 1024;   // next to the static part
 
 constexpr int unit_bytes(bool min) { return min ? 1280 : 1152; }
-constexpr int red_pitch(int n_tiles) { return 8 * n_tiles + 1; }   // odd: rows in different banks
+inline __host__ __device__ int red_pitch(int cols) { return cols | 1; }   // odd: rows in different banks
 
 // ------------------------------------------------------------------ layout
 // Lane l = 4 g + t of a unit holds, for each of its four blocks, the columns
@@ -102,6 +103,7 @@ struct Q4Args {
     const uint8_t* w;
     int64_t N;
     int tiles, units, split;
+    int part_log2;          // 2^part_log2 lanes add up the warps of an output
     const void* x;
     int x_type, pieces;
     int rows;               // activation rows of this launch
@@ -127,10 +129,12 @@ __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823
 // What the rows' staging leaves in shared memory beside the operands.
 struct RowState {
     uint32_t peak[kMaxRows];   // bits of the largest finite |x|
+    int shift[kMaxRows];       // the operands are x 2^shift
+    float back[kMaxRows][2];   // factors that take a row's sums back: 2^(24 - shift), in two
     uint32_t odd;              // rows that hold an infinity or a NaN (left out of the operands)
 };
-// x 2^shift(peak) has its largest value in [2^14, 2^15); peaks below 2^-113 stay smaller.
-__device__ __forceinline__ int shift_of(uint32_t peak) { return min(141 - static_cast<int>(peak >> 23), 127); }
+// x 2^top_shift(peak) has its largest value in [2^14, 2^15); peaks below 2^-113 stay smaller.
+__device__ __forceinline__ int top_shift(uint32_t peak) { return min(141 - static_cast<int>(peak >> 23), 127); }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
 
 // Eight values as they lie in memory.
@@ -172,130 +176,143 @@ struct Eight {
 // its products start from, -8 X 2^-24 in fp32, four blocks x two rows per unit and
 // pair of rows.  Q4_1: X 2^-5 as operands of the product with m, in three fp16
 // pieces side by side in k, four blocks x 8 bytes per unit and row.
-// A warp takes 256 columns of a row at a time, in two passes: the rows' peaks,
-// then the operands.
-template <class Tx, bool kMin>
-__device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState& st) {
+// A warp takes 256 columns of a row at a time.  A row's power of two is a guess
+// from its first 32 values, the largest of them taken to [2^9, 2^10): that leaves
+// the row's largest value a factor of 32, and loses no more than 2^-30 of it.  The
+// same pass takes the peaks; a row that needs more room is staged again with the
+// power that its peak gives (`again`).
+template <class Tx, bool kMin, int kWarps>
+__device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState& st, bool again) {
     constexpr int kPieces = std::is_same<Tx, float>::value ? 3 : 1;
-    constexpr int kBatch = kPieces == 3 ? 2 : 4;   // pieces of work whose loads are in flight together
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int chunks = a.units * 16, segs = (chunks + 31) / 32;   // of 8 columns; of 32 chunks
-    const int tasks = (a.rows * segs + kWarps - 1 - warp) / kWarps;
     const Tx* px = static_cast<const Tx*>(a.x);
     const bool vec = (a.ldx * sizeof(Tx)) % 16 == 0 && (reinterpret_cast<uintptr_t>(px) & 15) == 0;
-    struct Place {
-        int m, seg;
+    const int pairs = (a.rows + 1) / 2, row_step = kWarps / segs, seg_step = kWarps % segs;
+    int m = warp / segs, seg = warp % segs;
+    Eight<Tx> next;
+    Tx next_sample = from_f32<Tx>(0.f);
+    auto load = [&]() {
+        const Tx* row = px + m * a.ldx;
+        const int c = seg * 32 + lane;
+        next.load(row + c * 8, static_cast<int>(a.x_cols) - c * 8, vec);
+        if (lane < a.x_cols) next_sample = row[lane];
     };
-    auto place = [&]() { return Place{warp / segs, warp % segs}; };
-    auto step = [&](Place& p) {
-        p.seg += kWarps;
-        while (p.seg >= segs) {
-            p.seg -= segs;
-            ++p.m;
+    if (m < a.rows) load();
+#pragma unroll 1
+    while (m < a.rows) {
+        const Eight<Tx> v = next;
+        const Tx sample = next_sample;
+        const int row = m, c = seg * 32 + lane;
+        m += row_step;
+        seg += seg_step;
+        if (seg >= segs) {
+            seg -= segs;
+            ++m;
         }
-    };
-    Eight<Tx> v[kBatch];
-    auto load = [&](Place p, int n) {
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            if (b < n) {
-                const int c = p.seg * 32 + lane;
-                v[b].load(px + p.m * a.ldx + c * 8, static_cast<int>(a.x_cols) - c * 8, vec);
-                step(p);
-            }
-        }
-    };
-    Place p = place();
-    for (int i = 0; i < tasks; i += kBatch) {
-        load(p, tasks - i);
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            if (i + b < tasks) {
-                uint32_t peak = v[b].peak_bits();
-                if (__any_sync(0xffffffffu, peak >= 0x7F800000u)) {
-                    if (lane == 0) atomicOr(&st.odd, 1u << p.m);
-                    peak = 0;
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 x = v[b].pair(j);
-                        if (is_finite(x.x)) peak = max(peak, __float_as_uint(fabsf(x.x)));
-                        if (is_finite(x.y)) peak = max(peak, __float_as_uint(fabsf(x.y)));
-                    }
+        if (m < a.rows) load();
+        uint32_t peak = __reduce_max_sync(0xffffffffu, v.peak_bits());
+        const bool odd = peak >= 0x7F800000u;
+        int shift;
+        if (again) {
+            shift = st.shift[row];
+        } else {
+            if (odd) {
+                peak = 0;
+                for (int j = 0; j < 4; ++j) {
+                    const float2 x = v.pair(j);
+                    if (is_finite(x.x)) peak = max(peak, __float_as_uint(fabsf(x.x)));
+                    if (is_finite(x.y)) peak = max(peak, __float_as_uint(fabsf(x.y)));
                 }
                 peak = __reduce_max_sync(0xffffffffu, peak);
-                if (lane == 0) atomicMax(&st.peak[p.m], peak);
-                step(p);
+            }
+            const float f = fabsf(to_f32(sample));
+            shift = top_shift(__reduce_max_sync(0xffffffffu, is_finite(f) ? __float_as_uint(f) : 0u)) - 5;
+            if (lane == 0) {
+                atomicMax(&st.peak[row], peak);
+                if (odd) atomicOr(&st.odd, 1u << row);
+                st.shift[row] = shift;   // every warp of the row finds the same
             }
         }
-    }
-    __syncthreads();
-    const int pairs = (a.rows + 1) / 2;
-    const uint32_t any_odd = st.odd;
-    p = place();
-    for (int i = 0; i < tasks; i += kBatch) {
-        if (tasks > kBatch) load(p, tasks - i);   // else the first pass left them
+        const float s = pow2(shift), s16 = s * 0.0625f;
+        float sum = 0.f;
+        uint32_t p[kPieces][4];
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            if (i + b < tasks) {
-                const int c = p.seg * 32 + lane, m = p.m;
-                const float s = pow2(shift_of(st.peak[m])), s16 = s * 0.0625f;
-                float sum = 0.f;
-                uint32_t q[kPieces][4];
+        for (int j = 0; j < 4; ++j) {
+            float2 x = v.pair(j);
+            if (odd) {
+                if (!is_finite(x.x)) x.x = 0.f;
+                if (!is_finite(x.y)) x.y = 0.f;
+            }
+            sum = fmaf(x.x, s, fmaf(x.y, s, sum));
+            x.x *= j & 1 ? s16 : s;   // where the nibble stands four bits higher
+            x.y *= j & 1 ? s16 : s;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float2 x = v[b].pair(j);
-                    if (any_odd) {
-                        if (!is_finite(x.x)) x.x = 0.f;
-                        if (!is_finite(x.y)) x.y = 0.f;
-                    }
-                    sum = fmaf(x.x, s, fmaf(x.y, s, sum));
-                    x.x *= j & 1 ? s16 : s;   // where the nibble stands four bits higher
-                    x.y *= j & 1 ? s16 : s;
-#pragma unroll
-                    for (int z = 0; z < kPieces; ++z) {
-                        q[z][j] = pack2<__half>(x.x, x.y);
-                        if (z + 1 < kPieces) {
-                            const float2 h = unpack2<__half>(q[z][j]);
-                            x.x -= h.x;
-                            x.y -= h.y;
-                        }
-                    }
+            for (int z = 0; z < kPieces; ++z) {
+                p[z][j] = pack2<__half>(x.x, x.y);
+                if (z + 1 < kPieces) {
+                    const float2 h = unpack2<__half>(p[z][j]);
+                    x.x -= h.x;
+                    x.y -= h.y;
                 }
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (c < chunks) {
-                    uint8_t* dst = smem + m * a.pitch + c * 16;
+            }
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (c < chunks) {
+            uint8_t* dst = smem + row * a.pitch + c * 16;
 #pragma unroll
-                    for (int z = 0; z < kPieces; ++z)
-                        *reinterpret_cast<uint4*>(dst + z * a.rows * a.pitch) =
-                            make_uint4(q[z][0], q[z][1], q[z][2], q[z][3]);
-                    if ((c & 3) == 0) {
-                        const int unit = c >> 4, block = (c >> 2) & 3;
-                        if constexpr (kMin) {
-                            __half h[4];
-                            sum *= 0.03125f;
+            for (int z = 0; z < kPieces; ++z)
+                *reinterpret_cast<uint4*>(dst + z * a.rows * a.pitch) = make_uint4(p[z][0], p[z][1], p[z][2], p[z][3]);
+            if ((c & 3) == 0) {
+                const int unit = c >> 4, block = (c >> 2) & 3;
+                if constexpr (kMin) {
+                    __half h[4];
+                    sum *= 0.03125f;
 #pragma unroll
-                            for (int z = 0; z < 3; ++z) {
-                                h[z] = __float2half_rn(sum);
-                                sum -= __half2float(h[z]);
-                            }
-                            h[3] = __float2half_rn(0.f);
-                            *reinterpret_cast<uint2*>(smem + a.sum_at + ((unit * a.rows + m) * 4 + block) * 8) =
-                                *reinterpret_cast<const uint2*>(h);
-                        } else {
-                            float* out = reinterpret_cast<float*>(smem + a.sum_at) +
-                                         ((unit * pairs + (m >> 1)) * 4 + block) * 2 + (m & 1);
-                            out[0] = sum * -4.76837158203125e-7f;
-                            if (m + 1 == a.rows && !(m & 1)) out[1] = 0.f;
-                        }
+                    for (int z = 0; z < 3; ++z) {
+                        h[z] = __float2half_rn(sum);
+                        sum -= __half2float(h[z]);
                     }
+                    h[3] = __float2half_rn(0.f);
+                    *reinterpret_cast<uint2*>(smem + a.sum_at + ((unit * a.rows + row) * 4 + block) * 8) =
+                        *reinterpret_cast<const uint2*>(h);
+                } else {
+                    float* out = reinterpret_cast<float*>(smem + a.sum_at) +
+                                 ((unit * pairs + (row >> 1)) * 4 + block) * 2 + (row & 1);
+                    out[0] = sum * -4.76837158203125e-7f;
+                    if (row + 1 == a.rows && !(row & 1)) out[1] = 0.f;
                 }
-                step(p);
             }
         }
     }
     // what columns of other pieces take
     if (threadIdx.x < 8)
         reinterpret_cast<float*>(smem + a.sum_at)[a.units * (kMin ? a.rows : pairs) * 8 + threadIdx.x] = 0.f;
+}
+
+template <bool kMin, int kWarps>
+__device__ __forceinline__ void stage_rows(const Q4Args& a, uint8_t* smem, RowState& st) {
+    const int tid = threadIdx.x;
+    if (tid < kMaxRows) st.peak[tid] = 0;
+    if (tid == 0) st.odd = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+        if (a.x_type == B2Q_TYPE_F32) stage_x<float, kMin, kWarps>(a, smem, st, pass);
+        else if (a.x_type == B2Q_TYPE_F16) stage_x<__half, kMin, kWarps>(a, smem, st, pass);
+        else stage_x<__nv_bfloat16, kMin, kWarps>(a, smem, st, pass);
+        __syncthreads();
+        const bool mine = pass == 0 && tid < a.rows;
+        const bool over = mine && st.shift[tid] > top_shift(st.peak[tid]);
+        if (over) st.shift[tid] = top_shift(st.peak[tid]);
+        if (mine) {
+            const int e = 24 - st.shift[tid];
+            st.back[tid][0] = pow2(e >> 1);
+            st.back[tid][1] = pow2(e - (e >> 1));
+        }
+        if (!__syncthreads_or(over)) break;
+    }
 }
 
 // w[n][k] as registered
@@ -323,14 +340,14 @@ __device__ __noinline__ float odd_terms(const Q4Args& a, int64_t n, int m) {
     return v;
 }
 
-template <bool kMin, int kN, int kStages>
-__global__ void __launch_bounds__(kThreads, kN == 1 ? 2 : 1) mul_vec_q4_kernel(const __grid_constant__ Q4Args a) {
+template <bool kMin, int kN, int kStages, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid_constant__ Q4Args a) {
     constexpr int kUnit = unit_bytes(kMin);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ RowState st;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int split = a.split, sub = warp % split, group = warp / split, groups = kWarps / split;
-    const int first = blockIdx.x * groups + group, step = gridDim.x * groups;
+    const int first = group * gridDim.x + blockIdx.x, step = gridDim.x * groups;   // every SM gets its share of the tiles
     const int per_tile = (a.units - sub + split - 1) / split;   // units of this warp in each of its tiles
 
     // ---- the weights' stream: a unit is asked for as soon as its slot is free ----
@@ -357,13 +374,7 @@ __global__ void __launch_bounds__(kThreads, kN == 1 ? 2 : 1) mul_vec_q4_kernel(c
     };
 #pragma unroll
     for (int i = 0; i < kStages; ++i) issue(ring + i * kUnit);
-    if (tid < kMaxRows) st.peak[tid] = 0;
-    if (tid == 0) st.odd = 0;
-    __syncthreads();
-    if (a.x_type == B2Q_TYPE_F32) stage_x<float, kMin>(a, smem, st);
-    else if (a.x_type == B2Q_TYPE_F16) stage_x<__half, kMin>(a, smem, st);
-    else stage_x<__nv_bfloat16, kMin>(a, smem, st);
-    __syncthreads();
+    stage_rows<kMin, kWarps>(a, smem, st);
 
     // This lane's operand columns.  A column that no row has computes on the
     // first one's values; its results are not read.
@@ -436,32 +447,33 @@ __global__ void __launch_bounds__(kThreads, kN == 1 ? 2 : 1) mul_vec_q4_kernel(c
         }
         // ---- add up the tile's warps and the pieces, in order; two buffers, so that
         // one meeting a tile suffices ----
-        constexpr int kRedPitch = red_pitch(kN), kRedWarp = 16 * kRedPitch;
-        float* all = reinterpret_cast<float*>(smem + a.red_at) + (buf * kWarps + group * split) * kRedWarp;
-        float* red = all + sub * kRedWarp + g * kRedPitch + 2 * t;
+        const int pitch = red_pitch(cols), part_floats = 16 * pitch;
+        float* all = reinterpret_cast<float*>(smem + a.red_at) + (buf * kWarps + group * split) * part_floats;
+        float* red = all + sub * part_floats + g * pitch + 2 * t;
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 // Q4_1: the operands of m were scaled by 2^-5, those of d by 2^-24
                 const float v = kMin ? fmaf(accm[n][e], 1.9073486328125e-6f, acc[n][e]) : acc[n][e];
-                red[8 * (e >> 1) * kRedPitch + n * 8 + (e & 1)] = v;
+                if (n * 8 + 2 * t + (e & 1) < cols) red[8 * (e >> 1) * pitch + n * 8 + (e & 1)] = v;
             }
         if (split == 1) __syncwarp();
-        else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(split * 32) : "memory");
-        for (int o = tid - group * split * 32; o < 16 * a.rows; o += split * 32) {
-            const int row = o & 15, m = o >> 4, n = tile * 16 + row;
-            if (n >= a.N) continue;
-            const float* p = all + row * kRedPitch + m;
+        else asm volatile("bar.sync %0, %1;" ::"r"(group), "r"(split * 32) : "memory");
+        // 2^part_log2 neighbouring lanes take an output, each some of its warps' parts
+        const int me = tid - group * split * 32, part = me & ((1 << a.part_log2) - 1);
+        for (int base = 0; base < 16 * a.rows; base += split * 32 >> a.part_log2) {
+            const int o = base + (me >> a.part_log2), row = o & 15, m = o >> 4, n = tile * 16 + row;
+            const bool in = m < a.rows;
             float v = 0.f;
-#pragma unroll 4
-            for (int w = 0; w < split; ++w, p += kRedWarp) {
-                float s = p[0];
-                if (a.pieces == 3) s += p[a.rows] + p[2 * a.rows];
-                v += s;
+            if (in) {
+                const float* p = all + part * part_floats + row * pitch + m;
+                for (int w = part; w < split; w += 1 << a.part_log2, p += part_floats << a.part_log2)
+                    v += a.pieces == 3 ? p[0] + (p[a.rows] + p[2 * a.rows]) : p[0];
             }
-            const int e = 24 - shift_of(st.peak[m]);
-            v = v * pow2(e >> 1) * pow2(e - (e >> 1));
+            for (int x = 1 << a.part_log2 >> 1; x; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+            if (!in || part || n >= a.N) continue;
+            v = v * st.back[m][0] * st.back[m][1];
             if ((st.odd >> m) & 1) v += odd_terms<kMin>(a, n, m);
             const int64_t at = m * a.ldy + n;
             if (a.bias) v += a.bias[n];
@@ -474,15 +486,16 @@ __global__ void __launch_bounds__(kThreads, kN == 1 ? 2 : 1) mul_vec_q4_kernel(c
 }
 
 // ------------------------------------------------------------------ launch
-// Warps per row tile: the split whose slowest warp has the least to do, in half
-// units: two a unit that it streams, and per tile one for its end, two where
-// warps meet there.
-int split_of(int64_t tiles, int units, int ctas) {
+// Warps per row tile: the split whose warps on the fullest SM have the least to
+// do, in half units: two a unit that they stream, and per tile three for its end,
+// four where warps meet there.
+int split_of(int64_t tiles, int units, int sms, int warps) {
     int best = 1;
     int64_t best_cost = INT64_MAX;
-    for (int s = 1; s <= kWarps && s <= units; s *= 2) {
-        const int64_t groups = static_cast<int64_t>(ctas) * (kWarps / s);
-        const int64_t cost = (tiles + groups - 1) / groups * (2 * ((units + s - 1) / s) + (s > 1 ? 2 : 1));
+    const int64_t per_sm = (tiles + sms - 1) / sms;
+    for (int s = 1; s <= warps && s <= units; s *= 2) {
+        const int64_t rounds = (per_sm * s + warps - 1) / warps;
+        const int64_t cost = rounds * (2 * ((units + s - 1) / s) + (s > 1 ? 4 : 3));
         if (cost < best_cost) {
             best = s;
             best_cost = cost;
@@ -490,26 +503,30 @@ int split_of(int64_t tiles, int units, int ctas) {
     }
     return best;
 }
+// log2 of the lanes that share an output at a tile's end: all warps' parts side by
+// side where the outputs leave that many lanes.
+int part_log2_of(int split, int rows) {
+    int l = 0;
+    while ((2 << l) <= split && 16 * rows * (2 << l) <= split * 32) ++l;
+    return l;
+}
 
 struct Q4Plan {
-    int stages, ctas, pitch, ring_at, red_at, sum_at, bytes;
+    int stages, pitch, ring_at, red_at, sum_at, bytes;
 };
-// Shared memory of a launch over `rows` activation rows; stages 0 where it does
-// not fit.  Two CTAs of an SM with four stages hide more than one with eight, so
-// they come first where the registers allow them (n_tiles 1).
-Q4Plan plan_of(int rows, int pieces, int n_tiles, int units, bool min) {
+// Shared memory of a launch over `rows` activation rows, with as deep a ring as
+// it holds; stages 0 where it does not fit.
+Q4Plan plan_of(int rows, int pieces, int warps, int units, bool min) {
     Q4Plan p{};
     p.pitch = units * 256 + 64;   // 64 bytes off a multiple of 128: eight columns' chunks miss one another's banks
     p.red_at = static_cast<int>(round_up(rows * pieces * p.pitch, 128));
-    p.sum_at = p.red_at + static_cast<int>(round_up(2 * kWarps * 16 * red_pitch(n_tiles) * 4, 128));
+    p.sum_at = p.red_at + static_cast<int>(round_up(2 * warps * 16 * red_pitch(rows * pieces) * 4, 128));
     const int sums = (units * (min ? rows : (rows + 1) / 2) + 1) * 32;
     p.ring_at = p.sum_at + static_cast<int>(round_up(sums, 128));
-    for (int variant = n_tiles == 1 ? 0 : 1; variant < 4; ++variant) {
-        constexpr int kStagesOf[] = {4, 8, 4, 2};   // the last for the longest rows only
-        p.bytes = p.ring_at + kWarps * unit_bytes(min) * kStagesOf[variant];
-        p.ctas = variant == 0 ? 2 : 1;
-        if (p.bytes <= (p.ctas == 2 ? kSmemHalf : kSmemMax)) {
-            p.stages = kStagesOf[variant];
+    for (int stages : {4, 2, 1}) {
+        p.bytes = p.ring_at + warps * unit_bytes(min) * stages;
+        if (p.bytes <= kSmemMax) {
+            p.stages = stages;
             break;
         }
     }
@@ -611,42 +628,49 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
     const int units = static_cast<int>(w->units);
     const int pieces = x_dtype == B2Q_TYPE_F32 ? 3 : 1;
     const size_t es = pieces == 3 ? 4 : 2, ys = y_dtype == B2Q_TYPE_F32 ? 4 : 2;
+    const int64_t per_sm = (w->tiles + ds->num_sms - 1) / ds->num_sms * units;
+    auto plan_rows = [&](int rows) {
+        const int n = n_tiles_of(rows, pieces);
+        return n ? plan_of(rows, pieces, warps_of(n, per_sm), units, min) : Q4Plan{};
+    };
     // the most rows that a launch takes (operand tiles and shared memory), then as even launches as that allows
     int most = 1;
-    while (most < M && n_tiles_of(most + 1, pieces) &&
-           plan_of(most + 1, pieces, n_tiles_of(most + 1, pieces), units, min).stages >= 4)
-        ++most;
+    while (most < M && plan_rows(most + 1).stages >= 2) ++most;
     const int64_t launches = (M + most - 1) / most;
     for (int64_t i = 0, m0 = 0; i < launches; ++i) {
         const int rows = static_cast<int>((M - m0 + launches - i - 1) / (launches - i));
-        const int n_tiles = n_tiles_of(rows, pieces);
-        const Q4Plan p = plan_of(rows, pieces, n_tiles, units, min);
+        const int n_tiles = n_tiles_of(rows, pieces), warps = warps_of(n_tiles, per_sm);
+        const Q4Plan p = plan_rows(rows);
         if (!p.stages) return set_error(B2Q_ERR_SHAPE, "an activation row does not fit shared memory");
-        const int split = split_of(w->tiles, units, ds->num_sms * p.ctas);
-        const int64_t want = (w->tiles + kWarps / split - 1) / (kWarps / split);
-        const unsigned grid = static_cast<unsigned>(want < ds->num_sms * p.ctas ? want : ds->num_sms * p.ctas);
+        const int split = split_of(w->tiles, units, ds->num_sms, warps);
+        const unsigned grid = static_cast<unsigned>(w->tiles < ds->num_sms ? w->tiles : ds->num_sms);
         const Q4Args a{w->packed, w->N, static_cast<int>(w->tiles), units, split,
+                       part_log2_of(split, rows),
                        static_cast<const uint8_t*>(x) + m0 * ldx * es, x_dtype, pieces, rows, x_cols, ldx,
                        static_cast<uint8_t*>(y) + m0 * ldy * ys, ldy, y_dtype == B2Q_TYPE_F32, bias,
                        residual ? residual + m0 * ldy : nullptr, p.pitch, p.ring_at, p.red_at, p.sum_at};
-        auto go = [&](auto mn, auto nt, auto stages) {
-            auto* kernel = mul_vec_q4_kernel<decltype(mn)::value, decltype(nt)::value, decltype(stages)::value>;
-            b2q_status st = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                            kSmemMax), "4-bit product shared memory");
+        auto go = [&](auto mn, auto nt, auto stages, auto wp) {
+            auto* kernel = mul_vec_q4_kernel<decltype(mn)::value, decltype(nt)::value, decltype(stages)::value,
+                                             decltype(wp)::value>;
+            static std::atomic<uint64_t> allowed{0};
+            const b2q_status st = allow_smem(kernel, kSmemMax, allowed, ds->device);
             if (st) return st;
-            kernel<<<grid, kThreads, p.bytes, s>>>(a);
+            kernel<<<grid, warps * 32, p.bytes, s>>>(a);
             count_launch();
             return cuda_check(cudaGetLastError(), "4-bit product launch");
         };
-        auto with_stages = [&](auto mn, auto nt) {
-            return p.stages == 8   ? go(mn, nt, std::integral_constant<int, 8>{})
-                   : p.stages == 4 ? go(mn, nt, std::integral_constant<int, 4>{})
-                                   : go(mn, nt, std::integral_constant<int, 2>{});
+        auto with_stages = [&](auto mn, auto nt, auto wp) {
+            return p.stages == 4   ? go(mn, nt, std::integral_constant<int, 4>{}, wp)
+                   : p.stages == 2 ? go(mn, nt, std::integral_constant<int, 2>{}, wp)
+                                   : go(mn, nt, std::integral_constant<int, 1>{}, wp);
         };
+        constexpr std::integral_constant<int, 16> w16{};
+        constexpr std::integral_constant<int, 32> w32{};
         auto with_tiles = [&](auto mn) {
-            return n_tiles == 1   ? with_stages(mn, std::integral_constant<int, 1>{})
-                   : n_tiles == 2 ? with_stages(mn, std::integral_constant<int, 2>{})
-                                  : with_stages(mn, std::integral_constant<int, 4>{});
+            return n_tiles == 1   ? (warps == 32 ? with_stages(mn, std::integral_constant<int, 1>{}, w32)
+                                                 : with_stages(mn, std::integral_constant<int, 1>{}, w16))
+                   : n_tiles == 2 ? with_stages(mn, std::integral_constant<int, 2>{}, w16)
+                                  : with_stages(mn, std::integral_constant<int, 4>{}, w16);
         };
         const b2q_status st = min ? with_tiles(std::true_type{}) : with_tiles(std::false_type{});
         if (st) return st;
