@@ -287,7 +287,7 @@ def block_sums(w: Weight, act, m: int, out, stream=None):
     check(lib().b2q_block_sums(w.handle, _ptr(act), m, _ptr(out), _stream(stream)))
 
 
-def _i32(a):
+def _host_i32(a):
     arr = np.ascontiguousarray(np.asarray(a, dtype=np.int32))
     return arr, arr.ctypes.data_as(C.POINTER(C.c_int32))
 
@@ -295,7 +295,7 @@ def _i32(a):
 def attention(q, ldq, k, ldk, v, ldv, q_off, q_len, k_off, k_len, o_off, n_head, out, ldo, stream=None):
     """Packed-sequence attention (head_dim 72); q/k/v fp16 torch tensors, out fp32."""
     import torch
-    keep = [_i32(x) for x in (q_off, q_len, k_off, k_len, o_off)]
+    keep = [_host_i32(x) for x in (q_off, q_len, k_off, k_len, o_off)]
     n_seq = len(keep[0][0])
     nbytes = int(lib().b2q_attention_scratch_bytes(keep[1][1], n_seq))
     scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
@@ -344,7 +344,7 @@ class VisionTower:
     def encode(self, patches, grids, pooling=POOL_PROBE, out=None, stream=None):
         """patches: torch CUDA fp32 [T][patch_dim] (images back to back); grids: [(h, w), ...]."""
         import torch
-        g, gp = _i32(np.asarray(grids, np.int32).reshape(-1))
+        g, gp = _host_i32(np.asarray(grids, np.int32).reshape(-1))
         n = len(grids)
         if out is None:
             out = torch.empty((n, self.cfg.hidden), dtype=torch.float32, device="cuda")
@@ -354,7 +354,7 @@ class VisionTower:
     def encode_host(self, patches: np.ndarray, grids, pooling=POOL_PROBE, out: np.ndarray | None = None,
                     stream=None):
         """Host in, host out (patch upload and embedding download included)."""
-        g, gp = _i32(np.asarray(grids, np.int32).reshape(-1))
+        g, gp = _host_i32(np.asarray(grids, np.int32).reshape(-1))
         n = len(grids)
         if out is None:
             out = np.empty((n, self.cfg.hidden), np.float32)
@@ -366,7 +366,7 @@ class VisionTower:
         """Pipelined host entry point (b2q_vision_submit_host): patches and out
         are pinned host tensors (or any host buffers exposing data_ptr / the
         array interface); returns without waiting, see wait()."""
-        g, gp = _i32(np.asarray(grids, np.int32).reshape(-1))
+        g, gp = _host_i32(np.asarray(grids, np.int32).reshape(-1))
         # the last two submissions' buffers stay referenced until their copies have run
         self._keep = (getattr(self, "_keep", ((), ()))[-1], (g, patches, out))
         check(lib().b2q_vision_submit_host(self.handle, _host_ptr(patches), gp, len(grids), pooling, _host_ptr(out),
@@ -468,33 +468,91 @@ def score(img, txt, logit_scale: float, logit_bias: float, logits=True, probs=Tr
 
 
 # ---- decoding over a paged key-value cache ---------------------------------
+# A decode step calls these once per layer on small tensors, so the common case
+# (contiguous tensors on the current device) is checked in few steps.
+_TYPE_IDS: dict = {}
+_INT32 = None
+_raw = None          # (current device, raw stream of a device): torch's cheap forms
+
+
+def _setup():
+    global _INT32, _raw
+    import torch
+    _INT32 = torch.int32
+    _TYPE_IDS.update({torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16})
+    _raw = (torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+
+
 def _type_of(t) -> int:
-    import torch
-    types = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
-    if t.dtype not in types:
-        raise B2QError(ERR_INVALID, f"element type {t.dtype} is not one of float32, float16, bfloat16")
-    return types[t.dtype]
+    try:
+        return _TYPE_IDS[t.dtype]
+    except KeyError:
+        _setup()
+        if t.dtype not in _TYPE_IDS:
+            raise B2QError(ERR_INVALID, f"element type {t.dtype} is not one of float32, float16, bfloat16") from None
+        return _TYPE_IDS[t.dtype]
 
 
-def _require(ok: bool, what: str):
+def _require(ok: bool, what: str, status: int = ERR_SHAPE):
     if not ok:
-        raise B2QError(ERR_SHAPE, what)
-
-
-def _require_i32(n, **tensors):
-    """Contiguous int32 tensors on the device with n entries (None = any)."""
-    import torch
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or not t.is_cuda:
-            raise B2QError(ERR_INVALID, f"{name} must be an int32 CUDA tensor")
-        _require(t.is_contiguous() and (n is None or t.numel() == n), f"{name} must be contiguous with {n} entries")
+        raise B2QError(status, what)
 
 
 def _rows(t, width: int, name: str) -> int:
     """Row stride of a [rows][width] tensor whose columns are contiguous."""
-    _require(t.dim() == 2 and t.shape[1] == width and (t.stride(1) == 1 or width == 1 or t.numel() == 0),
-             f"{name} must be [rows][{width}] with contiguous columns")
-    return t.stride(0) if t.shape[0] > 1 else width
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != width:
+        raise B2QError(ERR_SHAPE, f"{name} must be [rows][{width}]")
+    if t.is_contiguous():
+        return width
+    ld, step = t.stride()
+    if step != 1 and width > 1:
+        raise B2QError(ERR_SHAPE, f"{name} must have contiguous columns")
+    return ld if shape[0] > 1 else width
+
+
+def _on(stream, *tensors):
+    """The stream to launch on; every tensor (None skipped) is on the current device."""
+    if _raw is None:
+        _setup()
+    dev = _raw[0]()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise B2QError(ERR_INVALID, f"a tensor on {t.device}, the current device is cuda:{dev}")
+    return stream.cuda_stream if stream is not None else _raw[1](dev)
+
+
+def _i32(t, n, name: str) -> int:
+    """Address of a contiguous int32 tensor of n entries (None = any number)."""
+    if t.dtype is not _INT32:
+        _setup()
+        if t.dtype is not _INT32:
+            raise B2QError(ERR_INVALID, f"{name} must be int32")
+    if not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise B2QError(ERR_SHAPE, f"{name} must be contiguous with {n} entries")
+    return t.data_ptr()
+
+
+def _f32(t, n: int, name: str):
+    """Address of a contiguous fp32 tensor of n entries, None for None."""
+    if t is None:
+        return None
+    if _type_of(t) != GGML_F32 or not t.is_contiguous() or t.numel() != n:
+        raise B2QError(ERR_SHAPE, f"{name} must be fp32 with {n} entries")
+    return t.data_ptr()
+
+
+def _table(t):
+    """(address, row stride, entries of a row, rows) of a block table."""
+    if t.dtype is not _INT32:
+        _setup()
+        if t.dtype is not _INT32:
+            raise B2QError(ERR_INVALID, "block_table must be int32")
+    shape = t.shape
+    if len(shape) != 2:
+        raise B2QError(ERR_SHAPE, "block_table must be [requests][max_blocks]")
+    width = shape[1]
+    return t.data_ptr(), width if t.is_contiguous() else _rows(t, width, "block_table"), width, shape[0]
 
 
 class KVCache:
@@ -512,6 +570,7 @@ class KVCache:
         self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _type_of(k), self.n_pages, self.page_size, self.n_kv_head,
                                 self.d_head, k.stride(0), k.stride(1), k.stride(2))
         self.ref = C.addressof(self.desc)
+        self.scratch_bytes: dict[int, int] = {}   # attention_paged scratch by n_head
 
 
 def kv_plan(ctx_len, new_len, page_size: int, free_pages, block_table, seq_of, pos, slot, kv_len, counts, stream=None):
@@ -520,23 +579,14 @@ def kv_plan(ctx_len, new_len, page_size: int, free_pages, block_table, seq_of, p
     entered in place; seq_of, pos, slot, kv_len: int32 [max_tokens] and counts
     int32 [2], written."""
     n, rows = ctx_len.numel(), seq_of.numel()
-    _require_i32(n, ctx_len=ctx_len, new_len=new_len)
-    _require_i32(rows, seq_of=seq_of, pos=pos, slot=slot, kv_len=kv_len)
-    _require_i32(None, free_pages=free_pages)
-    _require_i32(2, counts=counts)
-    _require(block_table.dim() == 2 and block_table.shape[0] == n, "block_table must be [n_seq][max_blocks]")
-    width = block_table.shape[1]
-    stride = _table(block_table)
-    check(lib().b2q_kv_plan(_ptr(ctx_len), _ptr(new_len), n, page_size, _ptr(free_pages), free_pages.numel(),
-                            _ptr(block_table), stride, width, rows, _ptr(seq_of), _ptr(pos), _ptr(slot), _ptr(kv_len),
-                            _ptr(counts), _stream(stream)))
-
-
-def _table(block_table) -> int:
-    import torch
-    if block_table.dtype != torch.int32 or not block_table.is_cuda:
-        raise B2QError(ERR_INVALID, "block_table must be an int32 CUDA tensor")
-    return _rows(block_table, block_table.shape[1], "block_table")
+    table, stride, width, requests = _table(block_table)
+    _require(requests == n, "block_table must be [n_seq][max_blocks]")
+    check(lib().b2q_kv_plan(_i32(ctx_len, n, "ctx_len"), _i32(new_len, n, "new_len"), n, page_size,
+                            _i32(free_pages, None, "free_pages"), free_pages.numel(), table, stride, width,
+                            rows, _i32(seq_of, rows, "seq_of"), _i32(pos, rows, "pos"),
+                            _i32(slot, rows, "slot"), _i32(kv_len, rows, "kv_len"),
+                            _i32(counts, 2, "counts"),
+                            _on(stream, ctx_len, new_len, free_pages, block_table, seq_of, pos, slot, kv_len, counts)))
 
 
 def rope_table(n_pos: int, rot_dim: int, theta: float = 10000.0, device="cuda"):
@@ -554,31 +604,37 @@ def qk_norm_rope(qkv, n_head: int, cache: KVCache, q_out, pos, slot, q_weight=No
     their cache slots (b2q_qk_norm_rope).  qkv: [rows][(n_head + 2 n_kv_head)
     d_head]; q_out: [rows][n_head d_head] of the cache's type; pos, slot: int32
     [rows]; rope: fp32 [n_pos][rot_dim] (see rope_table)."""
-    import torch
-    rows, d = qkv.shape[0], cache.d_head
+    d = cache.d_head
     ld = _rows(qkv, (n_head + 2 * cache.n_kv_head) * d, "qkv")
     ldq = _rows(q_out, n_head * d, "q_out")
-    _require(q_out.shape[0] == rows and q_out.dtype == cache.dtype, "q_out must have qkv's rows and the cache's type")
-    _require_i32(rows, pos=pos, slot=slot)
+    rows = qkv.shape[0]
+    if q_out.shape[0] != rows or q_out.dtype is not cache.dtype:
+        raise B2QError(ERR_SHAPE, "q_out must have qkv's rows and the cache's type")
     n_pos = rot = 0
     if rope is not None:
-        _require(rope.dim() == 2 and rope.is_contiguous() and rope.dtype == torch.float32,
-                 "rope must be fp32 [n_pos][rot_dim]")
+        if rope.dim() != 2 or not rope.is_contiguous() or _type_of(rope) != GGML_F32:
+            raise B2QError(ERR_SHAPE, "rope must be fp32 [n_pos][rot_dim]")
         n_pos, rot = rope.shape
-    for w in (q_weight, k_weight):
-        _require(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == d),
-                 "norm weights must be fp32 [d_head]")
-    check(lib().b2q_qk_norm_rope(_ptr(qkv), _type_of(qkv), ld, rows, n_head, _ptr(q_weight), _ptr(k_weight), eps,
-                                 _ptr(rope), n_pos, rot, int(interleaved), _ptr(pos), _ptr(slot), _ptr(q_out), ldq,
-                                 cache.ref, _stream(stream)))
+    check(lib().b2q_qk_norm_rope(qkv.data_ptr(), _type_of(qkv), ld, rows, n_head, _f32(q_weight, d, "q_weight"),
+                                 _f32(k_weight, d, "k_weight"), eps, rope.data_ptr() if rot else None, n_pos, rot,
+                                 interleaved, _i32(pos, rows, "pos"), _i32(slot, rows, "slot"),
+                                 q_out.data_ptr(), ldq, cache.ref,
+                                 _on(stream, qkv, q_out, pos, slot, q_weight, k_weight, rope, cache.k)))
+
+
+def _paged_scratch_bytes(n_head: int, cache: KVCache) -> int:
+    n = cache.scratch_bytes.get(n_head)
+    if n is None:
+        n = int(lib().b2q_attention_paged_scratch_bytes(n_head, cache.n_kv_head, cache.d_head))
+        _require(n > 0, "n_head must be a multiple of n_kv_head")
+        cache.scratch_bytes[n_head] = n
+    return n
 
 
 def attention_paged_scratch(n_head: int, cache: KVCache):
     """Zeroed scratch for attention_paged with this cache (one per stream)."""
     import torch
-    nbytes = int(lib().b2q_attention_paged_scratch_bytes(n_head, cache.n_kv_head, cache.d_head))
-    _require(nbytes > 0, "n_head must be a multiple of n_kv_head")
-    return torch.zeros(nbytes, dtype=torch.uint8, device=cache.k.device)
+    return torch.zeros(_paged_scratch_bytes(n_head, cache), dtype=torch.uint8, device=cache.k.device)
 
 
 def attention_paged(q, cache: KVCache, block_table, kv_len, out, scratch, seq_of=None, scale: float | None = None,
@@ -587,23 +643,22 @@ def attention_paged(q, cache: KVCache, block_table, kv_len, out, scratch, seq_of
     (b2q_attention_paged).  q: [rows][n_head d_head] of the cache's type; out
     the same shape, fp32 or the cache's type; block_table: int32 [requests]
     [max_blocks]; kv_len (and seq_of): int32 [rows]; lse: fp32 [rows][n_head]."""
-    import torch
-    rows, d = q.shape[0], cache.d_head
-    n_head = q.shape[1] // d
-    ldq, ldo = _rows(q, n_head * d, "q"), _rows(out, n_head * d, "out")
-    _require(out.shape[0] == rows and q.dtype == cache.dtype, "q and out need the same rows, q the cache's type")
-    _require_i32(rows, kv_len=kv_len)
-    if seq_of is not None:
-        _require_i32(rows, seq_of=seq_of)
-    if lse is not None:
-        _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == rows * n_head,
-                 "lse must be fp32 [rows][n_head]")
-    _require(n_head % cache.n_kv_head == 0 and scratch.numel() >= lib().b2q_attention_paged_scratch_bytes(
-        n_head, cache.n_kv_head, d), "scratch smaller than attention_paged_scratch, or n_head not a multiple of n_kv_head")
-    check(lib().b2q_attention_paged(_ptr(q), ldq, rows, n_head, cache.ref, _ptr(block_table), _table(block_table),
-                                    block_table.shape[1], block_table.shape[0], _ptr(seq_of), _ptr(kv_len),
-                                    d ** -0.5 if scale is None else scale, window, _ptr(out), _type_of(out), ldo,
-                                    _ptr(lse), _ptr(scratch), _stream(stream)))
+    d = cache.d_head
+    shape = q.shape
+    if len(shape) != 2 or out.shape != shape or q.dtype is not cache.dtype:
+        raise B2QError(ERR_SHAPE, "q and out must be [rows][n_head d_head], q of the cache's type")
+    rows, width = shape
+    n_head = width // d
+    ldq, ldo = _rows(q, n_head * d, "q"), _rows(out, width, "out")
+    if scratch.numel() < _paged_scratch_bytes(n_head, cache):
+        raise B2QError(ERR_SHAPE, "scratch smaller than attention_paged_scratch")
+    table, stride, blocks, requests = _table(block_table)
+    check(lib().b2q_attention_paged(q.data_ptr(), ldq, rows, n_head, cache.ref, table, stride, blocks, requests,
+                                    None if seq_of is None else _i32(seq_of, rows, "seq_of"),
+                                    _i32(kv_len, rows, "kv_len"), d ** -0.5 if scale is None else scale, window,
+                                    out.data_ptr(), _type_of(out), ldo, _f32(lse, rows * n_head, "lse"),
+                                    scratch.data_ptr(),
+                                    _on(stream, q, cache.k, block_table, kv_len, out, scratch, seq_of, lse)))
 
 
 class WeightQ4:
@@ -638,16 +693,19 @@ def mul_vec_q4(w: WeightQ4, x, m: int, y, bias=None, residual=None, stream=None)
     """y[m][n] = x @ w^T (+ bias) (+ residual) for few rows (b2q_mul_vec_q4).
     x: [m][x_cols] fp32, fp16 or bf16 (x_cols rounds up to the weight's K); y:
     [m][n] fp32 or x's type; bias fp32 [n]; residual fp32 like y."""
-    import torch
-    ldx, ldy = _rows(x, x.shape[1], "x"), _rows(y, w.n, "y")
-    _require(x.shape[0] >= m and y.shape[0] >= m, "x and y need m rows")
-    if bias is not None:
-        _require(bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == w.n, "bias must be fp32 [n]")
-    if residual is not None:
-        _require(residual.dtype == torch.float32 and _rows(residual, w.n, "residual") == ldy
-                 and residual.shape[0] >= m, "residual must be fp32 with y's rows and stride")
-    check(lib().b2q_mul_vec_q4(w.handle, _ptr(x), _type_of(x), m, x.shape[1], ldx, _ptr(y), _type_of(y), ldy,
-                               _ptr(bias), _ptr(residual), _stream(stream)))
+    n = w.n
+    if x.dim() != 2:
+        raise B2QError(ERR_SHAPE, "x must be [m][x_cols]")
+    x_rows, x_cols = x.shape
+    ldx, ldy = _rows(x, x_cols, "x"), _rows(y, n, "y")
+    if x_rows < m or y.shape[0] < m:
+        raise B2QError(ERR_SHAPE, "x and y need m rows")
+    if residual is not None and (_type_of(residual) != GGML_F32 or residual.shape != y.shape
+                                 or _rows(residual, n, "residual") != ldy):
+        raise B2QError(ERR_SHAPE, "residual must be fp32 with y's rows and stride")
+    check(lib().b2q_mul_vec_q4(w.handle, x.data_ptr(), _type_of(x), m, x_cols, ldx, y.data_ptr(), _type_of(y), ldy,
+                               _f32(bias, n, "bias"), None if residual is None else residual.data_ptr(),
+                               _on(stream, x, y, bias, residual)))
 
 
 class Gguf:
