@@ -1,6 +1,20 @@
 // b2q_rope.cu — RMS norm of query and key heads, rotation by position, and the
 // keys' and values' way into the paged cache, in one pass (b2q_qk_norm_rope).
+//
+// Bound: bytes; every element is read and written once, about six operations
+// apart.  Norm, rotation and the cache write in one pass because each of them
+// alone would read and write the same bytes.
+//
+// A head belongs to a group of 4 to 32 lanes, each with two pieces of kVec elements
+// loaded before either is used: in the half-and-half pairing a piece and the one
+// half a rotation further, so that a lane holds both elements of its pairs and the
+// only exchange is the sum of squares.  With d_head 128 a lane moves 2 x 16 bytes each
+// way.  One head per group and enough CTAs that an SM has 64 KB on its way: that
+// hides the latency without a pipeline.  The rotation rows are read by every head of
+// a row and stay in L1.
 #include "b2q_decode.cuh"
+
+#include <type_traits>
 
 namespace b2q {
 namespace {
@@ -22,9 +36,179 @@ struct RopeArgs {
     uint32_t* err;
 };
 
-// One warp per (row, head); element d of the head in lane d % 32.
+// Where a row's head goes and what may be done with it.
 template <class Tin, class Tc>
-__global__ void __launch_bounds__(kRopeWarps * 32) rope_kernel(RopeArgs<Tin, Tc> a) {
+struct Head {
+    int pos;
+    bool pad, stored;   // a padding row; whether there is a place for the head
+    Tc* dst;
+};
+template <class Tin, class Tc>
+__device__ __forceinline__ Head<Tin, Tc> head_of(const RopeArgs<Tin, Tc>& a, int64_t t, int h, bool reports) {
+    Head<Tin, Tc> o;
+    int pos = a.pos[t], slot = a.slot[t];
+    o.pad = pos == -1;
+    if (!o.pad && a.rot && (pos < 0 || pos >= a.n_pos)) {
+        if (reports) report(a.err, kDevBadPosition);
+        pos = 0;
+        slot = -1;
+    }
+    if (slot < -1 || slot >= a.n_slots) {
+        if (reports) report(a.err, kDevBadPosition);
+        slot = -1;
+    }
+    if (o.pad) {
+        pos = 0;
+        slot = -1;
+    }
+    o.pos = pos;
+    o.stored = true;
+    if (h < a.n_head) {
+        o.dst = a.q + t * a.ldq + static_cast<int64_t>(h) * a.d;
+    } else {
+        const bool is_v = h >= a.n_head + a.n_kv;
+        const int hk = h - a.n_head - (is_v ? a.n_kv : 0);
+        o.stored = slot >= 0;
+        o.dst = (is_v ? a.c.v : a.c.k) + (slot >> a.c.page_shift) * a.c.page_stride + hk * a.c.head_stride +
+                (slot & a.c.page_mask) * a.c.token_stride;
+    }
+    return o;
+}
+
+// kVec elements in 16-byte (or 8-byte) accesses
+template <class T, int kVec>
+struct Piece {
+    static constexpr int kWords = kVec * sizeof(T) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kWords >= 4) {
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) {
+                const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
+        } else {
+            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
+            w[0] = v.x, w[1] = v.y;
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[kVec]) const {
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) {
+            float2 f;
+            if constexpr (sizeof(T) == 4) f = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+            else f = unpack2<T>(w[i]);
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    }
+};
+template <class T, int kVec>
+__device__ __forceinline__ void store_piece(T* p, const float (&x)[kVec]) {
+    uint32_t w[kVec / 2];
+#pragma unroll
+    for (int i = 0; i < kVec / 2; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+    if constexpr (kVec == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+template <int kN>
+__device__ __forceinline__ void load_f32(const float* p, float (&x)[kN]) {
+    if constexpr (kN == 2) {
+        const float2 v = __ldg(reinterpret_cast<const float2*>(p));
+        x[0] = v.x, x[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN / 4; ++i) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
+            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+        }
+    }
+}
+
+// Lane s of a head's group holds pieces s and s + half/kVec of the rotated part,
+// the lanes after those two neighbouring pieces each of what is left.
+template <class Tin, class Tc, int kVec>
+__global__ void __launch_bounds__(kRopeWarps * 32) rope_kernel(RopeArgs<Tin, Tc> a, int group_log2) {
+    const int group = 1 << group_log2, heads = a.n_head + 2 * a.n_kv;
+    const int per_cta = kRopeWarps * 32 >> group_log2, s = threadIdx.x & (group - 1);
+    const int64_t item0 = static_cast<int64_t>(blockIdx.x) * per_cta;
+    const int64_t row0 = item0 / heads;
+    const int in = static_cast<int>(item0 - row0 * heads) + (threadIdx.x >> group_log2);
+    const int64_t t = row0 + in / heads;
+    const int h = in % heads;
+    const bool live = t < a.n_rows;
+    const int pieces = a.d / kVec, paired = a.interleaved ? 0 : a.rot / (2 * kVec);
+    const int pa = s < paired ? s : 2 * s, pb = s < paired ? s + paired : 2 * s + 1;   // (2 paired + 2 (s - paired))
+    const bool has_a = live && pa < pieces, has_b = live && pb < pieces;
+    Piece<Tin, kVec> ra{}, rb{};
+    const Tin* src = a.x + t * a.ld + static_cast<int64_t>(h) * a.d;
+    if (has_a) ra.load(src + pa * kVec);
+    if (has_b) rb.load(src + pb * kVec);
+    Head<Tin, Tc> o{};
+    if (live) o = head_of(a, t, h, s == 0);
+    const bool turned = live && h < a.n_head + a.n_kv && !o.pad;
+    float xa[kVec], xb[kVec];
+    ra.get(xa);
+    rb.get(xb);
+    const float* w = h < a.n_head ? a.qw : a.kw;
+    if (a.qw || a.kw) {   // (uniform: every lane takes part in the sum)
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
+        for (int x = group >> 1; x; x >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, x);
+        if (turned && w) {
+            const float r = 1.0f / sqrtf(ss / a.d + a.eps);
+            float wa[kVec], wb[kVec];
+            if (has_a) load_f32(w + pa * kVec, wa);
+            if (has_b) load_f32(w + pb * kVec, wb);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                xa[i] = has_a ? xa[i] * r * wa[i] : 0.f;
+                xb[i] = has_b ? xb[i] * r * wb[i] : 0.f;
+            }
+        }
+    }
+    if (!live || !o.stored) return;
+    if (o.pad) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) xa[i] = xb[i] = 0.f;
+    } else if (turned && a.rot) {
+        const float* cs = a.rope + static_cast<int64_t>(o.pos) * a.rot;
+        const int half = a.rot / 2;
+        if (s < paired) {
+            float c[kVec], sn[kVec];
+            load_f32(cs + pa * kVec, c);
+            load_f32(cs + half + pa * kVec, sn);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                const float u = xa[i], v = xb[i];
+                xa[i] = u * c[i] - v * sn[i];
+                xb[i] = v * c[i] + u * sn[i];
+            }
+        } else if (a.interleaved) {
+            auto turn = [&](float(&x)[kVec], int piece) {
+                if (piece * kVec >= a.rot) return;
+                float c[kVec / 2], sn[kVec / 2];
+                load_f32(cs + piece * (kVec / 2), c);
+                load_f32(cs + half + piece * (kVec / 2), sn);
+#pragma unroll
+                for (int i = 0; i < kVec / 2; ++i) {
+                    const float u = x[2 * i], v = x[2 * i + 1];
+                    x[2 * i] = u * c[i] - v * sn[i];
+                    x[2 * i + 1] = v * c[i] + u * sn[i];
+                }
+            };
+            turn(xa, pa);
+            turn(xb, pb);
+        }
+    }
+    if (has_a) store_piece<Tc, kVec>(o.dst + pa * kVec, xa);
+    if (has_b) store_piece<Tc, kVec>(o.dst + pb * kVec, xb);
+}
+
+// Any alignment and any even rotation: one warp per (row, head), element d of the
+// head in lane d % 32.
+template <class Tin, class Tc>
+__global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(RopeArgs<Tin, Tc> a) {
     __shared__ float sx[kRopeWarps][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int heads = a.n_head + 2 * a.n_kv;
@@ -32,47 +216,27 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_kernel(RopeArgs<Tin, Tc>
     if (item >= a.n_rows * heads) return;
     const int64_t t = item / heads;
     const int h = static_cast<int>(item % heads);
-    int pos = a.pos[t], slot = a.slot[t];
-    const bool pad = pos == -1;
-    if (!pad && a.rot && (pos < 0 || pos >= a.n_pos)) {
-        if (lane == 0) report(a.err, kDevBadPosition);
-        pos = 0;
-        slot = -1;
-    }
-    if (slot < -1 || slot >= a.n_slots) {
-        if (lane == 0) report(a.err, kDevBadPosition);
-        slot = -1;
-    }
-    if (pad) slot = -1;
-    Tc* dst;
-    if (h < a.n_head) {
-        dst = a.q + t * a.ldq + static_cast<int64_t>(h) * a.d;
-    } else {
-        if (slot < 0) return;
-        const bool is_v = h >= a.n_head + a.n_kv;
-        const int hk = h - a.n_head - (is_v ? a.n_kv : 0);
-        dst = (is_v ? a.c.v : a.c.k) + (slot >> a.c.page_shift) * a.c.page_stride + hk * a.c.head_stride +
-              (slot & a.c.page_mask) * a.c.token_stride;
-    }
+    const Head<Tin, Tc> o = head_of(a, t, h, lane == 0);
+    if (!o.stored) return;
     const Tin* src = a.x + t * a.ld + static_cast<int64_t>(h) * a.d;
     float* x = sx[warp];
     float ss = 0.f;
     for (int i = lane; i < a.d; i += 32) {
-        const float v = pad ? 0.f : to_f32(src[i]);
+        const float v = o.pad ? 0.f : to_f32(src[i]);
         x[i] = v;
         ss = fmaf(v, v, ss);
     }
     __syncwarp();
-    const bool turned = h < a.n_head + a.n_kv && !pad;
+    const bool turned = h < a.n_head + a.n_kv && !o.pad;
     const float* w = h < a.n_head ? a.qw : a.kw;
     if (turned && w) {
-        for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        for (int k = 16; k; k >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, k);
         const float r = 1.0f / sqrtf(ss / a.d + a.eps);
         for (int i = lane; i < a.d; i += 32) x[i] = x[i] * r * w[i];
         __syncwarp();
     }
     const int half = a.rot / 2;
-    const float* cs = a.rope + static_cast<int64_t>(pad ? 0 : pos) * a.rot;
+    const float* cs = a.rope + static_cast<int64_t>(o.pos) * a.rot;
     for (int i = lane; i < a.d; i += 32) {
         float y = x[i];
         if (turned && i < a.rot) {
@@ -81,14 +245,38 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_kernel(RopeArgs<Tin, Tc>
             const float other = x[a.interleaved ? i ^ 1 : (second ? i - half : i + half)];
             y = second ? y * cs[p] + other * cs[half + p] : y * cs[p] - other * cs[half + p];
         }
-        dst[i] = from_f32<Tc>(y);
+        o.dst[i] = from_f32<Tc>(y);
     }
 }
 
+// Pieces of 8 elements where every row, cache row and rotation half is made of
+// whole aligned ones, of 4 where that holds for 4 (halves such as 36 of 72), else the
+// element-wise kernel.
 template <class Tin, class Tc>
 cudaError_t launch(const RopeArgs<Tin, Tc>& a, cudaStream_t s) {
     const int64_t items = a.n_rows * (a.n_head + 2 * a.n_kv);
-    rope_kernel<Tin, Tc><<<static_cast<unsigned>((items + kRopeWarps - 1) / kRopeWarps), kRopeWarps * 32, 0, s>>>(a);
+    auto fits = [&](int vec) {
+        const size_t in = vec * sizeof(Tin) < 16 ? vec * sizeof(Tin) : 16, out = vec * 2;
+        const int unit = a.interleaved ? vec : 2 * vec;
+        return a.rot % unit == 0 && a.d / vec <= 64 && ptr_aligned(a.x, in) && a.ld * sizeof(Tin) % in == 0 &&
+               ptr_aligned(a.q, out) && a.ldq * 2 % out == 0 && ptr_aligned(a.qw, 16) && ptr_aligned(a.kw, 16) &&
+               ptr_aligned(a.rope, 16);
+    };
+    auto go = [&](auto vec) {
+        constexpr int kVec = decltype(vec)::value;
+        const int pieces = a.d / kVec, paired = a.interleaved ? 0 : a.rot / (2 * kVec);
+        const int lanes = paired + (pieces - 2 * paired + 1) / 2;
+        int log2 = 0;
+        while ((1 << log2) < lanes) ++log2;
+        const int per_cta = kRopeWarps * 32 >> log2;
+        rope_kernel<Tin, Tc, kVec><<<static_cast<unsigned>((items + per_cta - 1) / per_cta), kRopeWarps * 32, 0, s>>>(
+            a, log2);
+    };
+    if (fits(8)) go(std::integral_constant<int, 8>{});
+    else if (fits(4)) go(std::integral_constant<int, 4>{});
+    else
+        rope_any_kernel<Tin, Tc>
+            <<<static_cast<unsigned>((items + kRopeWarps - 1) / kRopeWarps), kRopeWarps * 32, 0, s>>>(a);
     count_launch();
     return cudaGetLastError();
 }
