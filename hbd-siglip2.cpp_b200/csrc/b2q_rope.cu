@@ -5,13 +5,17 @@
 // apart.  Norm, rotation and the cache write in one pass because each of them
 // alone would read and write the same bytes.
 //
-// A head belongs to a group of 4 to 32 lanes, each with two pieces of kVec elements
-// loaded before either is used: in the half-and-half pairing a piece and the one
-// half a rotation further, so that a lane holds both elements of its pairs and the
-// only exchange is the sum of squares.  With d_head 128 a lane moves 2 x 16 bytes each
-// way.  One head per group and enough CTAs that an SM has 64 KB on its way: that
-// hides the latency without a pipeline.  The rotation rows are read by every head of
-// a row and stay in L1.
+// A head belongs to a group of up to 32 lanes, each with two pieces of kVec
+// elements: in the half-and-half pairing a piece and the one half a rotation
+// further, so that a lane holds both elements of its pairs and the only exchange is
+// the sum of squares.  A group takes two heads of its row, both loaded before the
+// first is used; the row's position, slot and rotation values are fetched once for
+// both.  Norm and pairing are compiled in and lanes without a piece read the first
+// one's: instructions, not bytes, were the limit before (19 an element).
+// Measured on one B200, 20,011 rows of 24 + 2 x 4 heads of 128, fp16, half rotated,
+// 333 MB: 61 us, 5.46 TB/s (one head a group 67, four 69); 20,000 rows of 32 + 2 x 8
+// heads, bf16, normed and rotated, 502 MB: 102 us, 4.92 TB/s (141, 153).  Heads of 72
+// (36 pairs: pieces of 4, 9 of 16 lanes at work) reach 2.9 TB/s.
 #include "b2q_decode.cuh"
 
 #include <type_traits>
@@ -36,41 +40,27 @@ struct RopeArgs {
     uint32_t* err;
 };
 
-// Where a row's head goes and what may be done with it.
-template <class Tin, class Tc>
-struct Head {
-    int pos;
-    bool pad, stored;   // a padding row; whether there is a place for the head
-    Tc* dst;
+// A row's position and slot, checked; pad: a padding row.
+struct RowPlace {
+    int pos, slot;
+    bool pad;
 };
 template <class Tin, class Tc>
-__device__ __forceinline__ Head<Tin, Tc> head_of(const RopeArgs<Tin, Tc>& a, int64_t t, int h, bool reports) {
-    Head<Tin, Tc> o;
-    int pos = a.pos[t], slot = a.slot[t];
-    o.pad = pos == -1;
-    if (!o.pad && a.rot && (pos < 0 || pos >= a.n_pos)) {
+__device__ __forceinline__ RowPlace place_of(const RopeArgs<Tin, Tc>& a, int64_t t, bool reports) {
+    RowPlace o{a.pos[t], a.slot[t], false};
+    o.pad = o.pos == -1;
+    if (!o.pad && a.rot && (o.pos < 0 || o.pos >= a.n_pos)) {
         if (reports) report(a.err, kDevBadPosition);
-        pos = 0;
-        slot = -1;
+        o.pos = 0;
+        o.slot = -1;
     }
-    if (slot < -1 || slot >= a.n_slots) {
+    if (o.slot < -1 || o.slot >= a.n_slots) {
         if (reports) report(a.err, kDevBadPosition);
-        slot = -1;
+        o.slot = -1;
     }
     if (o.pad) {
-        pos = 0;
-        slot = -1;
-    }
-    o.pos = pos;
-    o.stored = true;
-    if (h < a.n_head) {
-        o.dst = a.q + t * a.ldq + static_cast<int64_t>(h) * a.d;
-    } else {
-        const bool is_v = h >= a.n_head + a.n_kv;
-        const int hk = h - a.n_head - (is_v ? a.n_kv : 0);
-        o.stored = slot >= 0;
-        o.dst = (is_v ? a.c.v : a.c.k) + (slot >> a.c.page_shift) * a.c.page_stride + hk * a.c.head_stride +
-                (slot & a.c.page_mask) * a.c.token_stride;
+        o.pos = 0;
+        o.slot = -1;
     }
     return o;
 }
@@ -124,85 +114,126 @@ __device__ __forceinline__ void load_f32(const float* p, float (&x)[kN]) {
     }
 }
 
-// Lane s of a head's group holds pieces s and s + half/kVec of the rotated part,
-// the lanes after those two neighbouring pieces each of what is left.
-template <class Tin, class Tc, int kVec>
-__global__ void __launch_bounds__(kRopeWarps * 32) rope_kernel(RopeArgs<Tin, Tc> a, int group_log2) {
-    const int group = 1 << group_log2, heads = a.n_head + 2 * a.n_kv;
-    const int per_cta = kRopeWarps * 32 >> group_log2, s = threadIdx.x & (group - 1);
-    const int64_t item0 = static_cast<int64_t>(blockIdx.x) * per_cta;
-    const int64_t row0 = item0 / heads;
-    const int in = static_cast<int>(item0 - row0 * heads) + (threadIdx.x >> group_log2);
-    const int64_t t = row0 + in / heads;
-    const int h = in % heads;
+// Block (lanes of a group, groups of a row, rows), grid (rows, runs of heads).
+// Lane s of a group holds pieces s and s + half/kVec of the rotated part, the lanes
+// after those two neighbouring pieces each of what is left.
+template <class Tin, class Tc, int kVec, int kHeads, bool kNorm, bool kInter>
+__global__ void __launch_bounds__(256, kHeads == 2 ? 4 : 1) rope_kernel(RopeArgs<Tin, Tc> a) {
+    const int group = blockDim.x, s = threadIdx.x, heads = a.n_head + 2 * a.n_kv, n_turned = a.n_head + a.n_kv;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.z + threadIdx.z;
+    const int step = blockDim.y, h0 = blockIdx.y * step * kHeads + threadIdx.y;
     const bool live = t < a.n_rows;
-    const int pieces = a.d / kVec, paired = a.interleaved ? 0 : a.rot / (2 * kVec);
-    const int pa = s < paired ? s : 2 * s, pb = s < paired ? s + paired : 2 * s + 1;   // (2 paired + 2 (s - paired))
-    const bool has_a = live && pa < pieces, has_b = live && pb < pieces;
-    Piece<Tin, kVec> ra{}, rb{};
-    const Tin* src = a.x + t * a.ld + static_cast<int64_t>(h) * a.d;
-    if (has_a) ra.load(src + pa * kVec);
-    if (has_b) rb.load(src + pb * kVec);
-    Head<Tin, Tc> o{};
-    if (live) o = head_of(a, t, h, s == 0);
-    const bool turned = live && h < a.n_head + a.n_kv && !o.pad;
-    float xa[kVec], xb[kVec];
-    ra.get(xa);
-    rb.get(xb);
-    const float* w = h < a.n_head ? a.qw : a.kw;
-    if (a.qw || a.kw) {   // (uniform: every lane takes part in the sum)
-        float ss = 0.f;
+    const int pieces = a.d / kVec, paired = kInter ? 0 : a.rot / (2 * kVec);
+    int pa = s < paired ? s : 2 * s, pb = s < paired ? s + paired : 2 * s + 1;   // (2 paired + 2 (s - paired))
+    const bool has_a = pa < pieces, has_b = pb < pieces;   // a lane without a piece reads the first and stores none
+    if (!has_a) pa = 0;
+    if (!has_b) pb = 0;
+    Piece<Tin, kVec> ra[kHeads], rb[kHeads];
+    const Tin* src = a.x + (live ? t : a.n_rows - 1) * a.ld;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
-        for (int x = group >> 1; x; x >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, x);
-        if (turned && w) {
-            const float r = 1.0f / sqrtf(ss / a.d + a.eps);
-            float wa[kVec], wb[kVec];
-            if (has_a) load_f32(w + pa * kVec, wa);
-            if (has_b) load_f32(w + pb * kVec, wb);
+    for (int k = 0; k < kHeads; ++k) {
+        const Tin* p = src + min(h0 + k * step, heads - 1) * a.d;
+        ra[k].load(p + pa * kVec);
+        rb[k].load(p + pb * kVec);
+    }
+    const RowPlace o = live ? place_of(a, t, s == 0 && h0 == 0) : RowPlace{0, -1, true};
+    // this lane's rotation values: of piece a and b in the interleaved pairing, of their pairs in the other;
+    // (1, 0) where nothing turns
+    const float* cs = a.rope + static_cast<int64_t>(o.pos) * a.rot;
+    const int half = a.rot / 2;
+    float c[kVec], sn[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+        c[i] = 1.f;
+        sn[i] = 0.f;
+    }
+    if constexpr (kInter) {
+        constexpr int kHalf = kVec / 2;
+        float u[kHalf];
+        if (pa * kVec < a.rot) {
+            load_f32(cs + pa * kHalf, u);
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) c[i] = u[i];
+            load_f32(cs + half + pa * kHalf, u);
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) sn[i] = u[i];
+        }
+        if (pb * kVec < a.rot) {
+            load_f32(cs + pb * kHalf, u);
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) c[kHalf + i] = u[i];
+            load_f32(cs + half + pb * kHalf, u);
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) sn[kHalf + i] = u[i];
+        }
+    } else if (s < paired) {
+        load_f32(cs + pa * kVec, c);
+        load_f32(cs + half + pa * kVec, sn);
+    }
+    const int64_t cache_row = (o.slot >> a.c.page_shift) * a.c.page_stride + (o.slot & a.c.page_mask) * a.c.token_stride;
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+        const int h = h0 + k * step;
+        float xa[kVec], xb[kVec];
+        ra[k].get(xa);
+        rb[k].get(xb);
+        if constexpr (kNorm) {   // (every lane takes part in the sum)
+            float sa = 0.f, sb = 0.f;
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                xa[i] = has_a ? xa[i] * r * wa[i] : 0.f;
-                xb[i] = has_b ? xb[i] * r * wb[i] : 0.f;
+                sa = fmaf(xa[i], xa[i], sa);
+                sb = fmaf(xb[i], xb[i], sb);
+            }
+            float ss = (has_a ? sa : 0.f) + (has_b ? sb : 0.f);
+            for (int x = group >> 1; x; x >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, x);
+            const float* w = h < a.n_head ? a.qw : a.kw;
+            if (h < n_turned && w) {
+                const float r = 1.0f / sqrtf(ss / a.d + a.eps);
+                float v[kVec];
+                load_f32(w + pa * kVec, v);
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) xa[i] = xa[i] * r * v[i];
+                load_f32(w + pb * kVec, v);
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) xb[i] = xb[i] * r * v[i];
             }
         }
-    }
-    if (!live || !o.stored) return;
-    if (o.pad) {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) xa[i] = xb[i] = 0.f;
-    } else if (turned && a.rot) {
-        const float* cs = a.rope + static_cast<int64_t>(o.pos) * a.rot;
-        const int half = a.rot / 2;
-        if (s < paired) {
-            float c[kVec], sn[kVec];
-            load_f32(cs + pa * kVec, c);
-            load_f32(cs + half + pa * kVec, sn);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                const float u = xa[i], v = xb[i];
-                xa[i] = u * c[i] - v * sn[i];
-                xb[i] = v * c[i] + u * sn[i];
-            }
-        } else if (a.interleaved) {
-            auto turn = [&](float(&x)[kVec], int piece) {
-                if (piece * kVec >= a.rot) return;
-                float c[kVec / 2], sn[kVec / 2];
-                load_f32(cs + piece * (kVec / 2), c);
-                load_f32(cs + half + piece * (kVec / 2), sn);
+        if (!live || h >= heads) continue;
+        Tc* dst;
+        if (h < a.n_head) {
+            dst = a.q + t * a.ldq + h * a.d;
+        } else {
+            if (o.slot < 0) continue;
+            dst = h < n_turned ? a.c.k + (h - a.n_head) * a.c.head_stride : a.c.v + (h - n_turned) * a.c.head_stride;
+            dst += cache_row;
+        }
+        if (h < n_turned) {
+            if constexpr (kInter) {
 #pragma unroll
                 for (int i = 0; i < kVec / 2; ++i) {
-                    const float u = x[2 * i], v = x[2 * i + 1];
-                    x[2 * i] = u * c[i] - v * sn[i];
-                    x[2 * i + 1] = v * c[i] + u * sn[i];
+                    float u = xa[2 * i], v = xa[2 * i + 1];
+                    xa[2 * i] = u * c[i] - v * sn[i];
+                    xa[2 * i + 1] = v * c[i] + u * sn[i];
+                    u = xb[2 * i], v = xb[2 * i + 1];
+                    xb[2 * i] = u * c[kVec / 2 + i] - v * sn[kVec / 2 + i];
+                    xb[2 * i + 1] = v * c[kVec / 2 + i] + u * sn[kVec / 2 + i];
                 }
-            };
-            turn(xa, pa);
-            turn(xb, pb);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) {
+                    const float u = xa[i], v = xb[i];
+                    xa[i] = u * c[i] - v * sn[i];
+                    xb[i] = v * c[i] + u * sn[i];
+                }
+            }
+            if (o.pad) {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) xa[i] = xb[i] = 0.f;
+            }
         }
+        if (has_a) store_piece<Tc, kVec>(dst + pa * kVec, xa);
+        if (has_b) store_piece<Tc, kVec>(dst + pb * kVec, xb);
     }
-    if (has_a) store_piece<Tc, kVec>(o.dst + pa * kVec, xa);
-    if (has_b) store_piece<Tc, kVec>(o.dst + pb * kVec, xb);
 }
 
 // Any alignment and any even rotation: one warp per (row, head), element d of the
@@ -216,8 +247,16 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(RopeArgs<Tin,
     if (item >= a.n_rows * heads) return;
     const int64_t t = item / heads;
     const int h = static_cast<int>(item % heads);
-    const Head<Tin, Tc> o = head_of(a, t, h, lane == 0);
-    if (!o.stored) return;
+    const RowPlace o = place_of(a, t, lane == 0);
+    Tc* dst;
+    if (h < a.n_head) {
+        dst = a.q + t * a.ldq + static_cast<int64_t>(h) * a.d;
+    } else {
+        if (o.slot < 0) return;
+        const bool is_v = h >= a.n_head + a.n_kv;
+        dst = (is_v ? a.c.v + (h - a.n_head - a.n_kv) * a.c.head_stride : a.c.k + (h - a.n_head) * a.c.head_stride) +
+              (o.slot >> a.c.page_shift) * a.c.page_stride + (o.slot & a.c.page_mask) * a.c.token_stride;
+    }
     const Tin* src = a.x + t * a.ld + static_cast<int64_t>(h) * a.d;
     float* x = sx[warp];
     float ss = 0.f;
@@ -245,7 +284,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(RopeArgs<Tin,
             const float other = x[a.interleaved ? i ^ 1 : (second ? i - half : i + half)];
             y = second ? y * cs[p] + other * cs[half + p] : y * cs[p] - other * cs[half + p];
         }
-        o.dst[i] = from_f32<Tc>(y);
+        dst[i] = from_f32<Tc>(y);
     }
 }
 
@@ -262,15 +301,33 @@ cudaError_t launch(const RopeArgs<Tin, Tc>& a, cudaStream_t s) {
                ptr_aligned(a.q, out) && a.ldq * 2 % out == 0 && ptr_aligned(a.qw, 16) && ptr_aligned(a.kw, 16) &&
                ptr_aligned(a.rope, 16);
     };
+    const int heads = a.n_head + 2 * a.n_kv;
     auto go = [&](auto vec) {
         constexpr int kVec = decltype(vec)::value;
         const int pieces = a.d / kVec, paired = a.interleaved ? 0 : a.rot / (2 * kVec);
         const int lanes = paired + (pieces - 2 * paired + 1) / 2;
-        int log2 = 0;
-        while ((1 << log2) < lanes) ++log2;
-        const int per_cta = kRopeWarps * 32 >> log2;
-        rope_kernel<Tin, Tc, kVec><<<static_cast<unsigned>((items + per_cta - 1) / per_cta), kRopeWarps * 32, 0, s>>>(
-            a, log2);
+        int group = 1;
+        while (group < lanes) group *= 2;
+        auto with = [&](auto n_heads, auto norm, auto inter) {
+            constexpr int kHeads = decltype(n_heads)::value;
+            // whole warps: 32 / group rows, and at most 8 groups a row; as few runs of heads as that allows
+            const int runs = (heads + 8 * kHeads - 1) / (8 * kHeads);
+            const int groups = (heads + runs * kHeads - 1) / (runs * kHeads);
+            const dim3 block(group, groups, 32 / group);
+            const dim3 grid(static_cast<unsigned>((a.n_rows + block.z - 1) / block.z), runs);
+            rope_kernel<Tin, Tc, kVec, kHeads, decltype(norm)::value, decltype(inter)::value><<<grid, block, 0, s>>>(a);
+        };
+        auto with_heads = [&](auto norm, auto inter) {
+            // one head a group until the lanes fill the GPU (half a million), for the shorter wait
+            if (items * group < (1 << 19)) with(std::integral_constant<int, 1>{}, norm, inter);
+            else with(std::integral_constant<int, 2>{}, norm, inter);
+        };
+        auto with_norm = [&](auto inter) {
+            if (a.qw || a.kw) with_heads(std::true_type{}, inter);
+            else with_heads(std::false_type{}, inter);
+        };
+        if (a.interleaved) with_norm(std::true_type{});
+        else with_norm(std::false_type{});
     };
     if (fits(8)) go(std::integral_constant<int, 8>{});
     else if (fits(4)) go(std::integral_constant<int, 4>{});
