@@ -16,15 +16,17 @@
 // and hundreds of ragged ones load every SM alike, lengths are read on the
 // device, and a captured launch stays valid as they grow.  A CTA's share holds
 // the end of one group, whole groups, and the start of another; what is not
-// whole goes to scratch as a partial result, and the last CTA to arrive at a
-// group joins its parts in their order (so the bits repeat).  Nobody waits.
+// whole goes to scratch as a partial result.  At its end the CTA reports its one or
+// two partial groups, and the last to report a group joins the parts in their order
+// (so the bits repeat).  Nobody waits.
 //
 // Inside a CTA each of four warps takes 16 keys of every tile and keeps its own
-// ref, sum and output; they meet only where a group ends.  Keys and values
-// come by 16-byte asynchronous copies, each warp filling its own ring of
-// stages, so loads run on across tiles, groups and rows with no block barrier.
-// Shared rows have an odd number of 16-byte chunks, which keeps ldmatrix free of
-// bank conflicts for every head width.
+// ref, sum and output; they meet only where a group ends, each leaving its output
+// in the ring slot that it has just read.  Keys and values come by 16-byte
+// asynchronous copies, each warp filling its own ring of stages, so loads run on
+// across tiles, groups and rows with no block barrier; page ids are looked up a tile
+// before they are needed.  Shared rows have an odd number of 16-byte chunks, which
+// keeps ldmatrix free of bank conflicts for every head width.
 //
 // Products run on mma.sync (16 query rows x 8 keys): a decode step has 1 to 16
 // query rows per key head, far from the 64 to 128 of a tcgen05 tile, and the
@@ -45,25 +47,28 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16 * kWarps;     // keys of a unit
-constexpr int kMaxCtas = 1024;         // join counters at the start of the scratch
-constexpr size_t kCounterBytes = kMaxCtas * sizeof(uint32_t);
+constexpr int kMaxCtas = 444;          // three per SM of a full GPU (148)
+constexpr size_t kCounterBytes = 2048;   // a join counter per CTA, at the start of the scratch
 
 // Per head width (padded to DP): stages of the ring and CTAs per SM, as many as
-// the 227 KB of shared memory hold next to the join buffer.
+// the 227 KB of shared memory hold.
 template <int DP>
 struct Shape {
     static constexpr int kChunks = (DP / 8) | 1;            // 16-byte chunks of a shared row
     static constexpr int kPitch = kChunks * 16;
     static constexpr int kStageBytes = 2 * 16 * kPitch;     // one warp's keys and values
-    static constexpr int kStages = DP > 128 ? 3 : 3;
+    static constexpr int kStages = 3;
     static constexpr int kCtas = DP > 128 ? 1 : (DP > 64 ? 2 : 3);
     static constexpr int kLanes = DP <= 64 ? 8 : (DP <= 128 ? 16 : 32);   // lanes that copy one row
     static constexpr int kOutPitch = DP + 8;
+    static_assert(16 * kOutPitch * 4 <= kStageBytes, "a warp's output fits the ring slot that it has just read");
 };
+// The ring, which at the end also holds a join's weights, sums and half-way outputs.
 template <int DP, int kRows>
-constexpr size_t smem_bytes() {
-    return static_cast<size_t>(kWarps) * Shape<DP>::kStages * Shape<DP>::kStageBytes +
-           static_cast<size_t>(kRows) * Shape<DP>::kOutPitch * 4;
+constexpr int smem_bytes() {
+    constexpr int ring = kWarps * Shape<DP>::kStages * Shape<DP>::kStageBytes;
+    constexpr int join = 2 * kRows * kMaxCtas * 4 + kThreads * 16;
+    return ring > join ? ring : join;
 }
 // floats of one partial result: output rows, then refs and sums
 template <int DP, int kRows>
@@ -127,8 +132,62 @@ __device__ __forceinline__ void next_unit(const PagedArgs<T>& a, Cursor& c, int 
     while (c.s.nt == 0 && ++c.r < a.n_rows) c.s = span_of(a, c.r);
 }
 
-template <class To>
-__device__ __forceinline__ void store_out(To* p, float v) { *p = from_f32<To>(v); }
+// x / y for y that fits an int: 32-bit wherever x does too (64-bit division is some
+// hundred dependent instructions, and the start of a short call waits for it).
+__device__ __forceinline__ long long divide(long long x, int y) {
+    return x <= 0xFFFFFFFFll ? static_cast<long long>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y)) : x / y;
+}
+// `total` units dealt to `ctas` CTAs in contiguous shares that differ by one at most.
+struct Shares {
+    long long each;
+    int more, ctas;   // the first `more` CTAs have one unit more
+    __device__ __forceinline__ void init(long long total, int grid) {
+        ctas = total < grid ? static_cast<int>(total) : grid;
+        each = ctas ? divide(total, ctas) : 0;
+        more = static_cast<int>(total - each * ctas);
+    }
+    __device__ __forceinline__ long long start(int cta) const { return each * cta + min(cta, more); }
+    __device__ __forceinline__ int owner(long long u) const {
+        const long long first = (each + 1) * more;   // units of the longer shares
+        if (each > 0x7FFFFFFEll) return static_cast<int>(u < first ? u / (each + 1) : more + (u - first) / each);
+        return static_cast<int>(u < first ? divide(u, static_cast<int>(each) + 1)
+                                          : more + divide(u - first, static_cast<int>(each)));
+    }
+};
+struct Start {
+    int r;
+    long long in_row;   // units before the share within row r
+    Span s;
+};
+struct Partial {
+    int live, r, head0, rows, nt;
+    long long u0;       // the group's first unit
+    int c0;             // and the CTA that has it
+};
+
+__device__ __forceinline__ uint32_t add_acq_rel(uint32_t* p, uint32_t v) {
+    uint32_t old;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+    return old;
+}
+
+template <class To, class T>
+__device__ __forceinline__ void write_out(const PagedArgs<T>& a, int r, int head, int c, float4 v, float l) {
+    if (c >= a.d) return;   // d is a multiple of 8
+    const float f = l == 0.f ? 0.f : 1.0f / l;
+    To* o = static_cast<To*>(a.out) + r * a.ldo + static_cast<int64_t>(head) * a.d + c;
+    v = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+    o[0] = from_f32<To>(v.x);
+    o[1] = from_f32<To>(v.y);
+    o[2] = from_f32<To>(v.z);
+    o[3] = from_f32<To>(v.w);
+}
+template <class T>
+__device__ __forceinline__ void write_lse(const PagedArgs<T>& a, int r, int head, float ref, float l) {
+    if (a.lse)
+        a.lse[static_cast<int64_t>(r) * a.n_head + head] =
+            l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.69314718055994531f;
+}
 
 template <class T, class To, int DP, int kRows>
 __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(PagedArgs<T> a) {
@@ -143,28 +202,36 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
 
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t s_valid[kWarps][S::kStages];
-    __shared__ float s_ref[kWarps][16], s_sum[kWarps][16], s_row_ref[16], s_row_sum[16];
+    __shared__ float s_ref[kWarps][16], s_sum[kWarps][16];
     __shared__ long long s_base[kWarps];
-    __shared__ long long s_u0;
-    __shared__ int s_row;
-    __shared__ uint32_t s_last;
+    __shared__ Start s_start;
+    __shared__ Partial s_partial[2];
+    __shared__ uint32_t s_last[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
     const int per_row = (a.n_head / a.group) * a.row_blocks;
-    float* s_out = reinterpret_cast<float*>(smem + kWarps * S::kStages * S::kStageBytes);
-    const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStageBytes;
+    const int ring_at = warp * S::kStages * S::kStageBytes;
+    const uint32_t ring = smem_u32(smem) + ring_at;
+    constexpr int kPart = part_floats<DP, kRows>();
 
     // columns d..DP-1 of the shared rows stay zero for good
-    if (a.d < DP)
-        for (int i = tid; i < kWarps * S::kStages * S::kStageBytes / 16; i += kThreads)
-            reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    if (a.d < DP) {
+        const int from = a.d / 8, n = S::kChunks - from;
+        for (int i = tid; i < kWarps * S::kStages * 32 * n; i += kThreads)
+            *reinterpret_cast<uint4*>(smem + i / n * S::kPitch + (from + i % n) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    if (tid < 2) s_partial[tid].live = 0;
 
     // ---- the units of all rows, and this CTA's share ----
     const int per = (a.n_rows + kThreads - 1) / kThreads;
     const int r0 = min(tid * per, a.n_rows), r1 = min(r0 + per, a.n_rows);
+    Span mine_span{};
     long long mine = 0;
-    for (int r = r0; r < r1; ++r) mine += span_of(a, r).nt;
+    for (int r = r0; r < r1; ++r) {
+        mine_span = span_of(a, r);
+        mine += mine_span.nt;
+    }
     long long incl = mine;
     for (int o = 1; o < 32; o <<= 1) {
         const long long v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -177,354 +244,411 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
         if (w < warp) base += s_base[w];
         total += s_base[w];
     }
-    total *= per_row;
+    Shares sh;
+    sh.init(total * per_row, gridDim.x);
+    const bool works = static_cast<int>(blockIdx.x) < sh.ctas;
+    const long long u0 = sh.start(blockIdx.x), u1 = sh.start(blockIdx.x + 1);
     base *= per_row;
-    mine *= per_row;
-    const long long ctas = min(static_cast<long long>(gridDim.x), total), cta = blockIdx.x;
+    if (works && u0 >= base && u0 < base + mine * per_row) {   // exactly one thread
+        for (int r = r0; r < r1; ++r) {
+            if (per > 1) mine_span = span_of(a, r);
+            const long long n = static_cast<long long>(mine_span.nt) * per_row;
+            if (u0 < base + n) {
+                s_start = Start{r, u0 - base, mine_span};
+                break;
+            }
+            base += n;
+        }
+    }
+    __syncthreads();
+
+    if (works) {
+        Cursor ld;
+        ld.r = s_start.r;
+        ld.s = s_start.s;
+        ld.hm = static_cast<int>(divide(s_start.in_row, ld.s.nt));
+        ld.t = static_cast<int>(s_start.in_row - static_cast<long long>(ld.hm) * ld.s.nt);
+        Cursor cu = ld;
+        const int n_units = static_cast<int>(min(u1 - u0, 0x7FFFFFFFll));
+        long long group_u0 = u0 - cu.t;           // first unit of the current group
+
+        // ---- loading: a warp's 16 keys are looked up one tile ahead of their copies ----
+        struct Pending {
+            int page;        // of lane's key (of all 16 where a page holds that many), -1 = none
+            uint32_t live;   // the 16 keys that are the row's
+            int64_t rest;    // offset of head and row within the page: of lane's key, or of the first
+        };
+        const bool one_page = a.c.page_mask >= 15;
+        int looked = 0;
+        auto look_up = [&]() {
+            Pending p{-1, 0u, 0};
+            if (looked < n_units) {
+                ++looked;
+                const int key0 = (ld.s.t0 + ld.t) * kTile + warp * 16;
+                const int lo = max(ld.s.first - key0, 0), hi = min(ld.s.len - key0, 16);
+                if (lo < hi) p.live = ((1u << hi) - 1) & ~((1u << lo) - 1);
+                const int key = key0 + (one_page ? 0 : lane);
+                const bool mine = one_page ? p.live != 0 : lane < 16 && ((p.live >> lane) & 1);
+                if (mine) p.page = a.table[ld.s.seq * a.bt_stride + (key >> a.c.page_shift)];
+                const int head = a.row_blocks == 1 ? ld.hm : ld.hm / a.row_blocks;
+                p.rest = head * a.c.head_stride + (key & a.c.page_mask) * a.c.token_stride;
+                next_unit(a, ld, per_row);
+            }
+            return p;
+        };
+        const int chunk = lane % S::kLanes, row_of_lane = lane / S::kLanes;
+        const bool copies = chunk * 8 < a.d;
+        auto issue = [&](const Pending& p, int stage) {
+            const bool ok = p.page >= 0 && p.page < a.c.n_pages;
+            const int64_t off = (ok ? p.page : 0) * a.c.page_stride + p.rest;
+            uint32_t valid = p.live;
+            if (one_page) {
+                if (!ok && valid) {
+                    if (lane == 0) report(a.err, kDevBadPage);
+                    valid = 0;
+                }
+            } else {
+                if (!ok && lane < 16 && ((p.live >> lane) & 1)) report(a.err, kDevBadPage);
+                valid &= __ballot_sync(0xffffffffu, ok);
+            }
+            if (lane == 0) s_valid[warp][stage] = valid;
+            if (valid) {
+                const uint32_t dst = ring + stage * S::kStageBytes + row_of_lane * S::kPitch + chunk * 16;
+                constexpr int kStep = 32 / S::kLanes;   // rows of one copy instruction
+                if (one_page) {
+                    const T* k = a.c.k + off + row_of_lane * a.c.token_stride + chunk * 8;
+                    const T* v = a.c.v + off + row_of_lane * a.c.token_stride + chunk * 8;
+#pragma unroll
+                    for (int row = 0; row < 16; row += kStep) {
+                        const bool in = (valid >> (row + row_of_lane)) & 1;
+                        if (copies) {
+                            cp_async_16(dst + row * S::kPitch, k, in);
+                            cp_async_16(dst + (16 + row) * S::kPitch, v, in);
+                        }
+                        k += kStep * a.c.token_stride;
+                        v += kStep * a.c.token_stride;
+                    }
+                } else {
+#pragma unroll
+                    for (int row = 0; row < 16; row += kStep) {
+                        const int64_t o = __shfl_sync(0xffffffffu, off, row + row_of_lane);
+                        const bool in = (valid >> (row + row_of_lane)) & 1;
+                        if (copies) {   // (a row that is not read is named by the cache's first)
+                            cp_async_16(dst + row * S::kPitch, a.c.k + (in ? o : 0) + chunk * 8, in);
+                            cp_async_16(dst + (16 + row) * S::kPitch, a.c.v + (in ? o : 0) + chunk * 8, in);
+                        }
+                    }
+                }
+            }
+            cp_commit();
+        };
+        Pending first[S::kStages];
+#pragma unroll
+        for (int i = 0; i < S::kStages; ++i) first[i] = look_up();
+#pragma unroll
+        for (int i = 0; i < S::kStages - 1; ++i) issue(first[i], i);
+        Pending next = first[S::kStages - 1];
+
+        uint32_t qf[kSteps][4];
+        float o[kCols][4];
+        float ref[2], sum[2];
+        bool fresh = true;
+        int stage = 0;
+
+        for (int i = 0; i < n_units; ++i) {
+            issue(next, stage == 0 ? S::kStages - 1 : stage - 1);
+            next = look_up();
+            if (fresh) {   // a new group: its queries, empty sums
+                fresh = false;
+                const int hk = cu.hm / a.row_blocks, q0 = (cu.hm % a.row_blocks) * kRows;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int row = q0 + g + 8 * x;
+                    const bool in = row < a.group && (x == 0 || !kPacked);
+                    const T* q = a.q + cu.r * a.ldq + static_cast<int64_t>(hk * a.group + (in ? row : 0)) * a.d;
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const int col = k * 16 + y * 8 + 2 * t4;
+                            qf[k][x + 2 * y] = in && col < a.d ? *reinterpret_cast<const uint32_t*>(q + col) : 0u;
+                        }
+                    ref[x] = -INFINITY;
+                    sum[x] = 0.f;
+                }
+#pragma unroll
+                for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[n][x] = 0.f;
+            }
+            cp_wait<S::kStages - 1>();
+            __syncwarp();
+            const uint32_t valid = s_valid[warp][stage];
+            if (valid) {
+                const uint32_t sk = ring + stage * S::kStageBytes, sv = sk + 16 * S::kPitch;
+                float s[2][4] = {};
+                const uint32_t ka = sk + ((lane & 7) + (lane >> 4) * 8) * S::kPitch + ((lane >> 3) & 1) * 16;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    uint32_t b[4];
+                    ldsm_x4(b, ka + k * 32);
+                    mma_16816<T>(s[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
+                    mma_16816<T>(s[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+                }
+                constexpr int kHalves = kPacked ? 1 : 2;
+                bool moved = false;
+                float factor[2] = {1.f, 1.f};
+#pragma unroll
+                for (int x = 0; x < kHalves; ++x) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float& v = s[n][2 * x + e];
+                            v = (valid >> (n * 8 + 2 * t4 + e)) & 1 ? v * a.scale_log2 : -INFINITY;
+                            mx = fmaxf(mx, v);
+                        }
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float nr = fmaxf(ref[x], mx - kLift);
+                    if (nr > ref[x]) {
+                        factor[x] = exp2_approx(ref[x] - nr);
+                        ref[x] = nr;
+                        moved = true;
+                    }
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int n = 0; n < kCols; ++n) {
+                        o[n][0] *= factor[0];
+                        o[n][1] *= factor[0];
+                        o[n][2] *= factor[kPacked ? 0 : 1];
+                        o[n][3] *= factor[kPacked ? 0 : 1];
+                    }
+                    sum[0] *= factor[0];
+                    sum[1] *= factor[1];
+                }
+                // p = 2^(s - ref), split into 16-bit pieces in operand order
+                uint32_t hi[4], lo[4], th[4];
+#pragma unroll
+                for (int x = 0; x < kHalves; ++x) {
+                    const float rf = ref[x] == -INFINITY ? 0.f : ref[x];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const float p0 = exp2_approx(s[n][2 * x] - rf), p1 = exp2_approx(s[n][2 * x + 1] - rf);
+                        sum[x] += p0 + p1;
+                        const uint32_t h = pack2<T>(p0, p1);
+                        const float2 hf = unpack2<T>(h);
+                        const float d0 = p0 - hf.x, d1 = p1 - hf.y;
+                        const uint32_t l = pack2<T>(d0, d1);
+                        hi[x + 2 * n] = h;
+                        lo[x + 2 * n] = l;
+                        if constexpr (kThird) {
+                            const float2 lf = unpack2<T>(l);
+                            th[x + 2 * n] = pack2<T>(d0 - lf.x, d1 - lf.y);
+                        }
+                    }
+                }
+                const uint32_t va = sv + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::kPitch + (lane >> 4) * 16;
+#pragma unroll
+                for (int n = 0; n < kCols; n += 2) {
+                    uint32_t b[4];
+                    ldsm_x4_trans(b, va + n * 16);
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const uint32_t b0 = b[2 * y], b1 = b[2 * y + 1];
+                        if constexpr (kPacked) {
+                            mma_16816<T>(o[n + y], hi[0], lo[0], hi[2], lo[2], b0, b1);
+                            if constexpr (kThird) mma_16816<T>(o[n + y], th[0], 0u, th[2], 0u, b0, b1);
+                        } else {
+                            mma_16816<T>(o[n + y], hi[0], hi[1], hi[2], hi[3], b0, b1);
+                            mma_16816<T>(o[n + y], lo[0], lo[1], lo[2], lo[3], b0, b1);
+                            if constexpr (kThird) mma_16816<T>(o[n + y], th[0], th[1], th[2], th[3], b0, b1);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+
+            // ---- the end of a group, or of the share: join the warps ----
+            const bool group_end = cu.t + 1 == cu.s.nt;
+            if (group_end || i + 1 == n_units) {
+                // into the slot that has just been read: nothing fills it before the next tile
+                const int slot_at = stage * S::kStageBytes;
+                float* so = reinterpret_cast<float*>(smem + ring_at + slot_at) + g * S::kOutPitch + 2 * t4;
+#pragma unroll
+                for (int n = 0; n < kCols; ++n) {
+                    if constexpr (kPacked) {
+                        *reinterpret_cast<float2*>(so + n * 8) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
+                    } else {
+                        *reinterpret_cast<float2*>(so + n * 8) = make_float2(o[n][0], o[n][1]);
+                        *reinterpret_cast<float2*>(so + 8 * S::kOutPitch + n * 8) = make_float2(o[n][2], o[n][3]);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
+                    sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 2);
+                    if (t4 == 0) {
+                        s_ref[warp][g + 8 * x] = ref[x];
+                        s_sum[warp][g + 8 * x] = sum[x];
+                    }
+                }
+                __syncthreads();
+                const int hk = cu.hm / a.row_blocks, q0 = (cu.hm % a.row_blocks) * kRows;
+                const int rows = min(kRows, a.group - q0), head0 = hk * a.group + q0;
+                const bool starts_here = group_u0 >= u0, whole = group_end && starts_here;
+                float* part = a.parts + (2 * static_cast<int64_t>(blockIdx.x) + starts_here) * kPart;
+                for (int e = tid; e < rows * (DP / 4); e += kThreads) {
+                    const int row = e / (DP / 4), c = e % (DP / 4) * 4;
+                    float m = s_ref[0][row], l = 0.f;
+#pragma unroll
+                    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_ref[w][row]);
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) {
+                        const float rw = s_ref[w][row], f = rw == -INFINITY ? 0.f : exp2_approx(rw - m);
+                        const float4 x = *reinterpret_cast<const float4*>(
+                            smem + w * S::kStages * S::kStageBytes + slot_at + (row * S::kOutPitch + c) * 4);
+                        l = fmaf(f, s_sum[w][row], l);
+                        v.x = fmaf(f, x.x, v.x);
+                        v.y = fmaf(f, x.y, v.y);
+                        v.z = fmaf(f, x.z, v.z);
+                        v.w = fmaf(f, x.w, v.w);
+                    }
+                    if (whole) {
+                        write_out<To>(a, cu.r, head0 + row, c, v, l);
+                        if (c == 0) write_lse(a, cu.r, head0 + row, m, l);
+                    } else {
+                        __stcg(reinterpret_cast<float4*>(part + row * DP + c), v);
+                        if (c == 0) {
+                            __stcg(part + kRows * DP + row, m);
+                            __stcg(part + kRows * DP + kRows + row, l);
+                        }
+                    }
+                }
+                if (!whole && tid == 0) s_partial[starts_here] = Partial{1, cu.r, head0, rows, cu.s.nt, group_u0};
+                __syncthreads();   // the slots, refs and sums are free again
+                if (a.d < DP) {    // ... and the slot's padding columns zero again
+                    const int from = a.d / 8;
+                    for (int e = lane; e < 32 * (S::kChunks - from); e += 32)
+                        *reinterpret_cast<uint4*>(smem + ring_at + slot_at + e / (S::kChunks - from) * S::kPitch +
+                                                  (from + e % (S::kChunks - from)) * 16) = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                }
+                fresh = true;
+            }
+            if (group_end) group_u0 += cu.s.nt;
+            next_unit(a, cu, per_row);
+            if (++stage == S::kStages) stage = 0;
+        }
+
+        // ---- report the partial groups; the last to report one joins it ----
+        // (the parts are all threads' stores: the group's barrier orders them before
+        // this thread's release, its acquire before what the next barrier lets run)
+        if (lane == 0 && warp < 2) {
+            Partial& pt = s_partial[warp];
+            int parts = 0;
+            if (pt.live) {
+                pt.c0 = sh.owner(pt.u0);
+                const int n = sh.owner(pt.u0 + pt.nt - 1) - pt.c0 + 1;
+                if (add_acq_rel(a.counters + pt.c0, 1u) + 1 == static_cast<uint32_t>(n)) {
+                    a.counters[pt.c0] = 0;   // for the next launch: all parts have arrived
+                    parts = n;
+                }
+            }
+            s_last[warp] = parts;
+        }
+        __syncthreads();
+        for (int x = 0; x < 2; ++x) {
+            const int n_parts = s_last[x];
+            if (!n_parts) continue;
+            const Partial pt = s_partial[x];
+            const auto part_of = [&](int p) {
+                return a.parts + (2 * static_cast<int64_t>(pt.c0 + p) + (p == 0 ? 1 : 0)) * kPart;
+            };
+            // refs and sums of all parts (the ring is free now: kRows x kMaxCtas x 2 floats fit it)
+            float* wt = reinterpret_cast<float*>(smem);           // [parts][rows] refs, then weights
+            float* sm = wt + n_parts * pt.rows;                   // [parts][rows] sums
+            __syncthreads();
+            for (int i = tid; i < n_parts * pt.rows; i += kThreads) {
+                const float* q = part_of(i / pt.rows) + kRows * DP + i % pt.rows;
+                wt[i] = __ldcg(q);
+                sm[i] = __ldcg(q + kRows);
+            }
+            __syncthreads();
+            for (int row = warp; row < pt.rows; row += kWarps) {
+                float m = -INFINITY, l = 0.f;
+                for (int p = lane; p < n_parts; p += 32) m = fmaxf(m, wt[p * pt.rows + row]);
+                for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+                for (int p = lane; p < n_parts; p += 32) {
+                    float& w = wt[p * pt.rows + row];
+                    w = w == -INFINITY ? 0.f : exp2_approx(w - m);
+                    l = fmaf(w, sm[p * pt.rows + row], l);
+                }
+                for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+                if (lane == 0) {
+                    s_sum[0][row] = l;
+                    write_lse(a, pt.r, pt.head0 + row, m, l);
+                }
+            }
+            __syncthreads();
+            // The outputs.  Few outputs: the parts too are dealt to threads, and added up
+            // in a second step; the loads of all outputs and four parts are in flight.
+            constexpr int kEach = (kRows * DP / 4 + kThreads - 1) / kThreads;
+            const int n_out = pt.rows * (DP / 4), subs = n_out < kThreads ? min(kThreads / n_out, n_parts) : 1;
+            const int sub = subs > 1 ? tid / n_out : 0, e0 = subs > 1 ? tid % n_out : tid;
+            float4 acc[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (sub < subs) {
+#pragma unroll 4
+                for (int p = sub; p < n_parts; p += subs) {
+                    const float4* q = reinterpret_cast<const float4*>(part_of(p));
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {
+                        const int e = e0 + i * kThreads;
+                        if (e < n_out) {
+                            const float f = wt[p * pt.rows + e / (DP / 4)];
+                            const float4 v = __ldcg(q + e);
+                            acc[i].x = fmaf(f, v.x, acc[i].x);
+                            acc[i].y = fmaf(f, v.y, acc[i].y);
+                            acc[i].z = fmaf(f, v.z, acc[i].z);
+                            acc[i].w = fmaf(f, v.w, acc[i].w);
+                        }
+                    }
+                }
+            }
+            if (subs > 1) {
+                float4* red = reinterpret_cast<float4*>(smem + 2 * kRows * kMaxCtas * 4);
+                if (sub < subs) red[tid] = acc[0];
+                __syncthreads();
+                if (tid < n_out)
+                    for (int k = 1; k < subs; ++k) {
+                        const float4 v = red[k * n_out + tid];
+                        acc[0].x += v.x;
+                        acc[0].y += v.y;
+                        acc[0].z += v.z;
+                        acc[0].w += v.w;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int e = e0 + i * kThreads;
+                if (sub == 0 && e < n_out)
+                    write_out<To>(a, pt.r, pt.head0 + e / (DP / 4), e % (DP / 4) * 4, acc[i], s_sum[0][e / (DP / 4)]);
+            }
+        }
+    }
 
     // rows with nothing to read
     for (int r = blockIdx.x * kWarps + warp; r < a.n_rows; r += gridDim.x * kWarps) {
         if (span_of(a, r).nt) continue;
         To* o = static_cast<To*>(a.out) + r * a.ldo;
-        for (int i = lane; i < a.n_head * a.d; i += 32) store_out(o + i, 0.f);
+        for (int i = lane; i < a.n_head * a.d; i += 32) o[i] = from_f32<To>(0.f);
         if (a.lse)
             for (int i = lane; i < a.n_head; i += 32) a.lse[static_cast<int64_t>(r) * a.n_head + i] = -INFINITY;
-    }
-    if (cta >= ctas) return;
-
-    const long long u0 = total * cta / ctas, u1 = total * (cta + 1) / ctas;
-    if (u0 >= base && u0 < base + mine) {   // exactly one thread
-        long long b = base;
-        for (int r = r0; r < r1; ++r) {
-            const long long n = static_cast<long long>(span_of(a, r).nt) * per_row;
-            if (u0 < b + n) {
-                s_row = r;
-                s_u0 = b;
-                break;
-            }
-            b += n;
-        }
-    }
-    __syncthreads();
-    Cursor ld;
-    ld.r = s_row;
-    ld.s = span_of(a, ld.r);
-    ld.hm = static_cast<int>((u0 - s_u0) / ld.s.nt);
-    ld.t = static_cast<int>((u0 - s_u0) % ld.s.nt);
-    Cursor cu = ld;
-    const int n_units = static_cast<int>(min(u1 - u0, 0x7FFFFFFFll));
-    long long group_u0 = u0 - cu.t;           // first unit of the current group
-
-    // ---- loading: lane l < 16 looks up key l's page one tile ahead of its copies ----
-    int pg = -1, key = 0;
-    bool live = false;
-    auto look_up = [&](int i) {
-        live = false;
-        if (i < n_units && lane < 16) {
-            key = (ld.s.t0 + ld.t) * kTile + warp * 16 + lane;
-            live = key >= ld.s.first && key < ld.s.len;
-            if (live) pg = a.table[ld.s.seq * a.bt_stride + (key >> a.c.page_shift)];
-        }
-    };
-    auto issue = [&](int i) {
-        if (i < n_units) {
-            bool ok = live && pg >= 0 && pg < a.c.n_pages;
-            if (live && !ok) report(a.err, kDevBadPage);
-            int64_t off = 0;
-            if (ok)
-                off = pg * a.c.page_stride + (ld.hm / a.row_blocks) * a.c.head_stride +
-                      (key & a.c.page_mask) * a.c.token_stride;
-            const uint32_t valid = __ballot_sync(0xffffffffu, ok);
-            const int stage = i % S::kStages;
-            if (lane == 0) s_valid[warp][stage] = valid;
-            if (valid) {
-                const int chunk = lane % S::kLanes;
-                const uint32_t dst = ring + stage * S::kStageBytes + chunk * 16;
-#pragma unroll
-                for (int row0 = 0; row0 < 16; row0 += 32 / S::kLanes) {
-                    const int row = row0 + lane / S::kLanes;
-                    const int64_t o = __shfl_sync(0xffffffffu, off, row);
-                    const bool in = (valid >> row) & 1;
-                    if (chunk * 8 < a.d) {
-                        cp_async_16(dst + row * S::kPitch, a.c.k + o + chunk * 8, in);
-                        cp_async_16(dst + (16 + row) * S::kPitch, a.c.v + o + chunk * 8, in);
-                    }
-                }
-            }
-            next_unit(a, ld, per_row);
-        }
-        cp_commit();
-    };
-    if (a.d < DP) __syncthreads();            // the zeros are in place
-#pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
-        look_up(i);
-        issue(i);
-    }
-    look_up(S::kStages - 1);
-
-    uint32_t qf[kSteps][4];
-    float o[kCols][4];
-    float ref[2], sum[2];
-    bool fresh = true;
-
-    for (int i = 0; i < n_units; ++i) {
-        issue(i + S::kStages - 1);
-        look_up(i + S::kStages);
-        if (fresh) {   // a new group: its queries, empty sums
-            fresh = false;
-            const int hk = cu.hm / a.row_blocks, q0 = (cu.hm % a.row_blocks) * kRows;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int row = q0 + g + 8 * x;
-                const bool in = row < a.group && (x == 0 || !kPacked);
-                const T* q = a.q + cu.r * a.ldq + static_cast<int64_t>(hk * a.group + (in ? row : 0)) * a.d;
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const int col = k * 16 + y * 8 + 2 * t4;
-                        qf[k][x + 2 * y] = in && col < a.d ? *reinterpret_cast<const uint32_t*>(q + col) : 0u;
-                    }
-                ref[x] = -INFINITY;
-                sum[x] = 0.f;
-            }
-#pragma unroll
-            for (int n = 0; n < kCols; ++n)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[n][x] = 0.f;
-        }
-        cp_wait<S::kStages - 1>();
-        __syncwarp();
-        const int stage = i % S::kStages;
-        const uint32_t valid = s_valid[warp][stage];
-        if (valid) {
-            const uint32_t sk = ring + stage * S::kStageBytes, sv = sk + 16 * S::kPitch;
-            float s[2][4] = {};
-            const uint32_t ka = sk + ((lane & 7) + (lane >> 4) * 8) * S::kPitch + ((lane >> 3) & 1) * 16;
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                uint32_t b[4];
-                ldsm_x4(b, ka + k * 32);
-                mma_16816<T>(s[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
-                mma_16816<T>(s[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
-            }
-            constexpr int kHalves = kPacked ? 1 : 2;
-            bool moved = false;
-            float factor[2] = {1.f, 1.f};
-#pragma unroll
-            for (int x = 0; x < kHalves; ++x) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& v = s[n][2 * x + e];
-                        v = (valid >> (n * 8 + 2 * t4 + e)) & 1 ? v * a.scale_log2 : -INFINITY;
-                        mx = fmaxf(mx, v);
-                    }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float nr = fmaxf(ref[x], mx - kLift);
-                if (nr > ref[x]) {
-                    factor[x] = exp2_approx(ref[x] - nr);
-                    ref[x] = nr;
-                    moved = true;
-                }
-            }
-            if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                for (int n = 0; n < kCols; ++n) {
-                    o[n][0] *= factor[0];
-                    o[n][1] *= factor[0];
-                    o[n][2] *= factor[kPacked ? 0 : 1];
-                    o[n][3] *= factor[kPacked ? 0 : 1];
-                }
-                sum[0] *= factor[0];
-                sum[1] *= factor[1];
-            }
-            // p = 2^(s - ref), split into 16-bit pieces in operand order
-            uint32_t hi[4], lo[4], th[4];
-#pragma unroll
-            for (int x = 0; x < kHalves; ++x) {
-                const float rf = ref[x] == -INFINITY ? 0.f : ref[x];
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float p0 = exp2_approx(s[n][2 * x] - rf), p1 = exp2_approx(s[n][2 * x + 1] - rf);
-                    sum[x] += p0 + p1;
-                    const uint32_t h = pack2<T>(p0, p1);
-                    const float2 hf = unpack2<T>(h);
-                    const float d0 = p0 - hf.x, d1 = p1 - hf.y;
-                    const uint32_t l = pack2<T>(d0, d1);
-                    hi[x + 2 * n] = h;
-                    lo[x + 2 * n] = l;
-                    if constexpr (kThird) {
-                        const float2 lf = unpack2<T>(l);
-                        th[x + 2 * n] = pack2<T>(d0 - lf.x, d1 - lf.y);
-                    }
-                }
-            }
-            const uint32_t va = sv + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::kPitch + (lane >> 4) * 16;
-#pragma unroll
-            for (int n = 0; n < kCols; n += 2) {
-                uint32_t b[4];
-                ldsm_x4_trans(b, va + n * 16);
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const uint32_t b0 = b[2 * y], b1 = b[2 * y + 1];
-                    if constexpr (kPacked) {
-                        mma_16816<T>(o[n + y], hi[0], lo[0], hi[2], lo[2], b0, b1);
-                        if constexpr (kThird) mma_16816<T>(o[n + y], th[0], 0u, th[2], 0u, b0, b1);
-                    } else {
-                        mma_16816<T>(o[n + y], hi[0], hi[1], hi[2], hi[3], b0, b1);
-                        mma_16816<T>(o[n + y], lo[0], lo[1], lo[2], lo[3], b0, b1);
-                        if constexpr (kThird) mma_16816<T>(o[n + y], th[0], th[1], th[2], th[3], b0, b1);
-                    }
-                }
-            }
-        }
-        __syncwarp();
-
-        // ---- the end of a group, or of the share: join the warps ----
-        const bool group_end = cu.t + 1 == cu.s.nt;
-        if (group_end || i + 1 == n_units) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
-                sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 2);
-                if (t4 == 0) {
-                    s_ref[warp][g + 8 * x] = ref[x];
-                    s_sum[warp][g + 8 * x] = sum[x];
-                }
-            }
-            __syncthreads();
-            float fac[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float m = -INFINITY;
-                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ref[w][g + 8 * x]);
-                fac[x] = ref[x] == -INFINITY ? 0.f : exp2_approx(ref[x] - m);
-            }
-            if (tid < kRows) {
-                float m = -INFINITY, l = 0.f;
-                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ref[w][tid]);
-                for (int w = 0; w < kWarps; ++w)
-                    l += s_ref[w][tid] == -INFINITY ? 0.f : s_sum[w][tid] * exp2_approx(s_ref[w][tid] - m);
-                s_row_ref[tid] = m;
-                s_row_sum[tid] = l;
-            }
-            for (int w = 0; w < kWarps; ++w) {   // in turn: a fixed order of the additions
-                if (warp == w) {
-#pragma unroll
-                    for (int n = 0; n < kCols; ++n) {
-                        float2* p = reinterpret_cast<float2*>(s_out + g * S::kOutPitch + n * 8 + 2 * t4);
-                        if constexpr (kPacked) {
-                            float2 v = make_float2((o[n][0] + o[n][2]) * fac[0], (o[n][1] + o[n][3]) * fac[0]);
-                            if (w) v = make_float2(p->x + v.x, p->y + v.y);
-                            *p = v;
-                        } else {
-                            float2* p8 = p + 4 * S::kOutPitch;
-                            float2 v = make_float2(o[n][0] * fac[0], o[n][1] * fac[0]);
-                            float2 v8 = make_float2(o[n][2] * fac[1], o[n][3] * fac[1]);
-                            if (w) {
-                                v = make_float2(p->x + v.x, p->y + v.y);
-                                v8 = make_float2(p8->x + v8.x, p8->y + v8.y);
-                            }
-                            *p = v;
-                            *p8 = v8;
-                        }
-                    }
-                }
-                __syncthreads();
-            }
-            const int hk = cu.hm / a.row_blocks, q0 = (cu.hm % a.row_blocks) * kRows;
-            const int rows = min(kRows, a.group - q0), head0 = hk * a.group + q0;
-            const bool whole = group_end && group_u0 >= u0;
-            bool write = whole;
-            const long long last_u = group_u0 + cu.s.nt - 1;
-            const int c0 = static_cast<int>(((group_u0 + 1) * ctas - 1) / total);
-            const int c1 = static_cast<int>(((last_u + 1) * ctas - 1) / total);
-            const int n_parts = c1 - c0 + 1;
-            constexpr int kPart = part_floats<DP, kRows>();
-            if (!whole) {
-                float* part = a.parts + (2 * cta + (group_u0 >= u0 ? 1 : 0)) * kPart;
-                for (int e = tid; e < rows * (DP / 4); e += kThreads) {
-                    const int row = e / (DP / 4), c = e % (DP / 4) * 4;
-                    __stcg(reinterpret_cast<float4*>(part + row * DP + c),
-                           *reinterpret_cast<const float4*>(s_out + row * S::kOutPitch + c));
-                }
-                if (tid < rows) {
-                    __stcg(part + kRows * DP + tid, s_row_ref[tid]);
-                    __stcg(part + kRows * DP + kRows + tid, s_row_sum[tid]);
-                }
-                __threadfence();
-                __syncthreads();
-                if (tid == 0) {
-                    const uint32_t before = atomicAdd(a.counters + c0, 1u);
-                    s_last = before + 1 == static_cast<uint32_t>(n_parts);
-                    if (s_last) a.counters[c0] = 0;   // for the next launch: all parts have arrived
-                }
-                __syncthreads();
-                if (s_last) {
-                    __threadfence();
-                    const auto part_of = [&](int p) {
-                        return a.parts + (2 * static_cast<int64_t>(c0 + p) + (p == 0 ? 1 : 0)) * kPart;
-                    };
-                    for (int row = warp; row < rows; row += kWarps) {
-                        float m = -INFINITY, l = 0.f;
-                        for (int p = lane; p < n_parts; p += 32) m = fmaxf(m, __ldcg(part_of(p) + kRows * DP + row));
-                        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-                        for (int p = lane; p < n_parts; p += 32) {
-                            const float* q = part_of(p) + kRows * DP + row;
-                            const float rf = __ldcg(q);
-                            l += rf == -INFINITY ? 0.f : __ldcg(q + kRows) * exp2_approx(rf - m);
-                        }
-                        for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-                        if (lane == 0) {
-                            s_row_ref[row] = m;
-                            s_row_sum[row] = l;
-                        }
-                    }
-                    __syncthreads();
-                    for (int e = tid; e < rows * (DP / 4); e += kThreads) {
-                        const int row = e / (DP / 4), c = e % (DP / 4) * 4;
-                        const float m = s_row_ref[row];
-                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                        for (int p = 0; p < n_parts; ++p) {
-                            const float* q = part_of(p);
-                            const float rf = __ldcg(q + kRows * DP + row);
-                            const float f = rf == -INFINITY ? 0.f : exp2_approx(rf - m);
-                            const float4 v = __ldcg(reinterpret_cast<const float4*>(q + row * DP + c));
-                            acc.x = fmaf(f, v.x, acc.x);
-                            acc.y = fmaf(f, v.y, acc.y);
-                            acc.z = fmaf(f, v.z, acc.z);
-                            acc.w = fmaf(f, v.w, acc.w);
-                        }
-                        *reinterpret_cast<float4*>(s_out + row * S::kOutPitch + c) = acc;
-                    }
-                    __syncthreads();
-                    write = true;
-                }
-            }
-            if (write) {
-                To* out = static_cast<To*>(a.out) + cu.r * a.ldo + static_cast<int64_t>(head0) * a.d;
-                for (int e = tid; e < rows * DP; e += kThreads) {
-                    const int row = e / DP, c = e % DP;
-                    const float l = s_row_sum[row], v = s_out[row * S::kOutPitch + c];
-                    if (c < a.d) store_out(out + static_cast<int64_t>(row) * a.d + c, l == 0.f ? 0.f : v / l);
-                }
-                if (a.lse && tid < rows) {
-                    const float l = s_row_sum[tid];
-                    a.lse[static_cast<int64_t>(cu.r) * a.n_head + head0 + tid] =
-                        l == 0.f ? -INFINITY : (s_row_ref[tid] + log2f(l)) * 0.69314718055994531f;
-                }
-            }
-            __syncthreads();   // s_out and the sums are free again
-            fresh = true;
-        }
-        if (group_end) group_u0 += cu.s.nt;
-        next_unit(a, cu, per_row);
     }
 }
 
@@ -600,7 +724,7 @@ b2q_status b2q_attention_paged(const void* q, int64_t ldq, int64_t n_rows, int32
         using To = decltype(to);
         return with_shape(c.d_head, group, [&](auto dp, auto rows) {
             constexpr int DP = decltype(dp)::value, kRows = decltype(rows)::value;
-            constexpr size_t smem = smem_bytes<DP, kRows>();
+            constexpr int smem = smem_bytes<DP, kRows>();
             PagedArgs<T> a{static_cast<const T*>(q), ldq, static_cast<int>(n_rows), n_head, group,
                            (group + kRows - 1) / kRows, c.d_head, max_blocks, n_table_rows, window, view_of<T>(c),
                            block_table, bt_stride, seq_of, kv_len, scale * 1.44269504088896340736f, out, ldo, lse,
@@ -608,7 +732,7 @@ b2q_status b2q_attention_paged(const void* q, int64_t ldq, int64_t n_rows, int32
                            reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + kCounterBytes), ds->err};
             auto* kernel = paged_kernel<T, To, DP, kRows>;
             static std::atomic<uint64_t> allowed{0};
-            const b2q_status s = allow_smem(kernel, static_cast<int>(smem), allowed, ds->device);
+            const b2q_status s = allow_smem(kernel, smem, allowed, ds->device);
             if (s) return s;
             kernel<<<grid_of(ds->num_sms, Shape<DP>::kCtas), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
             count_launch();
