@@ -139,6 +139,34 @@ inline b2q_status allow_smem(Kernel* kernel, int bytes, std::atomic<uint64_t>& d
     return st;
 }
 
+// ---- back-to-back launches ---------------------------------------------------
+// The decode kernels are launched so that one may start while the one before it
+// in the stream still runs (programmatic dependent launch): it lets its successor
+// start (`let_next_start`) and waits for its predecessors' results
+// (`wait_for_previous`) before it touches anything that they may read or write.
+// What comes before that wait reads only its arguments and registered weights,
+// which are complete when their registration returns.  A kernel launched any other
+// way keeps its full order.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... Params, class... Args>
+inline cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                                const Args&... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 // B2Q_OK and the strides filled in, or the error of a bad description.
 inline b2q_status check_cache(const b2q_kv_cache* in, b2q_kv_cache* c) {
     if (!in || !in->k || !in->v) return set_error(B2Q_ERR_INVALID, "null cache");

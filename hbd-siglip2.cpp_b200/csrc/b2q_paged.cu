@@ -222,6 +222,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
             *reinterpret_cast<uint4*>(smem + i / n * S::kPitch + (from + i % n) * 16) = make_uint4(0, 0, 0, 0);
     }
     if (tid < 2) s_partial[tid].live = 0;
+    let_next_start();
+    wait_for_previous();
 
     // ---- the units of all rows, and this CTA's share ----
     const int per = (a.n_rows + kThreads - 1) / kThreads;
@@ -734,9 +736,9 @@ b2q_status b2q_attention_paged(const void* q, int64_t ldq, int64_t n_rows, int32
             static std::atomic<uint64_t> allowed{0};
             const b2q_status s = allow_smem(kernel, smem, allowed, ds->device);
             if (s) return s;
-            kernel<<<grid_of(ds->num_sms, Shape<DP>::kCtas), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
-            count_launch();
-            return cuda_check(cudaGetLastError(), "paged attention launch");
+            return cuda_check(launch_after(kernel, dim3(grid_of(ds->num_sms, Shape<DP>::kCtas)), dim3(kThreads), smem,
+                                           static_cast<cudaStream_t>(stream), a),
+                              "paged attention launch");
         });
     };
     auto with_out = [&](auto t) { return out_dtype == B2Q_TYPE_F32 ? go(t, float{}) : go(t, t); };

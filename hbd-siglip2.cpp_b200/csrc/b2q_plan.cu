@@ -66,6 +66,8 @@ __device__ __forceinline__ int find_seq(const int* base, int n, int i) {
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     extern __shared__ int sums[];             // row_s [n_seq + 1], first_s [n_seq + 1]
     __shared__ int warp_rows[kPlanThreads / 32], warp_pages[kPlanThreads / 32];
+    let_next_start();
+    wait_for_previous();
     int* rows = sums;
     int* pages = sums + a.n_seq + 1;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -186,7 +188,7 @@ extern "C" b2q_status b2q_kv_plan(const int32_t* ctx_len, const int32_t* new_len
     const int64_t work = max_tokens > n_seq ? max_tokens : n_seq;
     int64_t grid = (work + 2 * kPlanThreads - 1) / (2 * kPlanThreads);
     grid = grid < 1 ? 1 : (grid > ds->num_sms ? ds->num_sms : grid);
-    kv_plan_kernel<<<static_cast<unsigned>(grid), kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
-    count_launch();
-    return cuda_check(cudaGetLastError(), "plan launch");
+    return cuda_check(launch_after(kv_plan_kernel, dim3(static_cast<unsigned>(grid)), dim3(kPlanThreads), smem,
+                                   static_cast<cudaStream_t>(stream), a),
+                      "plan launch");
 }

@@ -374,6 +374,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
     };
 #pragma unroll
     for (int i = 0; i < kStages; ++i) issue(ring + i * kUnit);
+    // the weights are on their way; the activations may be another kernel's results
+    let_next_start();
+    wait_for_previous();
     stage_rows<kMin, kWarps>(a, smem, st);
 
     // This lane's operand columns.  A column that no row has computes on the
@@ -584,11 +587,10 @@ b2q_status b2q_weight_q4_register(const void* blocks, int32_t ggml_type, int64_t
         count_launch();
         st = cuda_check(cudaGetLastError(), "4-bit weight layout");
     }
-    if (src_is_host) {
-        const b2q_status sync = cuda_check(cudaStreamSynchronize(s), "4-bit weight layout");
-        if (!st) st = sync;
-        cudaFree(staged);
-    }
+    // complete when this returns: the product reads weights before it waits for other kernels
+    const b2q_status sync = cuda_check(cudaStreamSynchronize(s), "4-bit weight layout");
+    if (!st) st = sync;
+    if (staged) cudaFree(staged);
     if (st) {
         cudaFree(w->packed);
         delete w;
@@ -655,9 +657,8 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
             static std::atomic<uint64_t> allowed{0};
             const b2q_status st = allow_smem(kernel, kSmemMax, allowed, ds->device);
             if (st) return st;
-            kernel<<<grid, warps * 32, p.bytes, s>>>(a);
-            count_launch();
-            return cuda_check(cudaGetLastError(), "4-bit product launch");
+            return cuda_check(launch_after(kernel, dim3(grid), dim3(warps * 32), p.bytes, s, a),
+                              "4-bit product launch");
         };
         auto with_stages = [&](auto mn, auto nt, auto wp) {
             return p.stages == 4   ? go(mn, nt, std::integral_constant<int, 4>{}, wp)

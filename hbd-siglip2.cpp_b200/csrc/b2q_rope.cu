@@ -128,6 +128,8 @@ __global__ void __launch_bounds__(256, kHeads == 2 ? 4 : 1) rope_kernel(RopeArgs
     const bool has_a = pa < pieces, has_b = pb < pieces;   // a lane without a piece reads the first and stores none
     if (!has_a) pa = 0;
     if (!has_b) pb = 0;
+    let_next_start();
+    wait_for_previous();
     Piece<Tin, kVec> ra[kHeads], rb[kHeads];
     const Tin* src = a.x + (live ? t : a.n_rows - 1) * a.ld;
 #pragma unroll
@@ -241,6 +243,8 @@ __global__ void __launch_bounds__(256, kHeads == 2 ? 4 : 1) rope_kernel(RopeArgs
 template <class Tin, class Tc>
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(RopeArgs<Tin, Tc> a) {
     __shared__ float sx[kRopeWarps][256];
+    let_next_start();
+    wait_for_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int heads = a.n_head + 2 * a.n_kv;
     const int64_t item = static_cast<int64_t>(blockIdx.x) * kRopeWarps + warp;
@@ -315,27 +319,23 @@ cudaError_t launch(const RopeArgs<Tin, Tc>& a, cudaStream_t s) {
             const int groups = (heads + runs * kHeads - 1) / (runs * kHeads);
             const dim3 block(group, groups, 32 / group);
             const dim3 grid(static_cast<unsigned>((a.n_rows + block.z - 1) / block.z), runs);
-            rope_kernel<Tin, Tc, kVec, kHeads, decltype(norm)::value, decltype(inter)::value><<<grid, block, 0, s>>>(a);
+            return launch_after(rope_kernel<Tin, Tc, kVec, kHeads, decltype(norm)::value, decltype(inter)::value>, grid,
+                                block, 0, s, a);
         };
         auto with_heads = [&](auto norm, auto inter) {
             // one head a group until the lanes fill the GPU (half a million), for the shorter wait
-            if (items * group < (1 << 19)) with(std::integral_constant<int, 1>{}, norm, inter);
-            else with(std::integral_constant<int, 2>{}, norm, inter);
+            return items * group < (1 << 19) ? with(std::integral_constant<int, 1>{}, norm, inter)
+                                             : with(std::integral_constant<int, 2>{}, norm, inter);
         };
         auto with_norm = [&](auto inter) {
-            if (a.qw || a.kw) with_heads(std::true_type{}, inter);
-            else with_heads(std::false_type{}, inter);
+            return a.qw || a.kw ? with_heads(std::true_type{}, inter) : with_heads(std::false_type{}, inter);
         };
-        if (a.interleaved) with_norm(std::true_type{});
-        else with_norm(std::false_type{});
+        return a.interleaved ? with_norm(std::true_type{}) : with_norm(std::false_type{});
     };
-    if (fits(8)) go(std::integral_constant<int, 8>{});
-    else if (fits(4)) go(std::integral_constant<int, 4>{});
-    else
-        rope_any_kernel<Tin, Tc>
-            <<<static_cast<unsigned>((items + kRopeWarps - 1) / kRopeWarps), kRopeWarps * 32, 0, s>>>(a);
-    count_launch();
-    return cudaGetLastError();
+    if (fits(8)) return go(std::integral_constant<int, 8>{});
+    if (fits(4)) return go(std::integral_constant<int, 4>{});
+    return launch_after(rope_any_kernel<Tin, Tc>, dim3(static_cast<unsigned>((items + kRopeWarps - 1) / kRopeWarps)),
+                        dim3(kRopeWarps * 32), 0, s, a);
 }
 
 }  // namespace

@@ -390,7 +390,7 @@ b2q_status b2q_attention_paged(const void *q, int64_t ldq, int64_t n_rows, int32
  * A registered ggml Q4_0 tensor (18-byte blocks of 32: fp16 d, 16 bytes of
  * nibbles, low nibbles first; w = d (q - 8)) or Q4_1 (20 bytes: fp16 d, fp16
  * m; w = d q + m): N rows of K (a multiple of 32), row stride row_bytes.
- * Repacked once; the source is not retained. */
+ * Repacked once; synchronises `stream`; the source is not retained. */
 typedef struct b2q_weight_q4 b2q_weight_q4;
 b2q_status b2q_weight_q4_register(const void *blocks, int32_t ggml_type, int64_t N, int64_t K, int64_t row_bytes,
                                   int src_is_host, void *stream, b2q_weight_q4 **out);
