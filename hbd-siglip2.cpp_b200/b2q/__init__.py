@@ -471,16 +471,20 @@ def score(img, txt, logit_scale: float, logit_bias: float, logits=True, probs=Tr
 # A decode step calls these once per layer on small tensors, so the common case
 # (contiguous tensors on the current device) is checked in few steps.
 _TYPE_IDS: dict = {}
-_INT32 = None
-_raw = None          # (current device, raw stream of a device): torch's cheap forms
+_INT32 = _F32 = None
+_device = _raw_stream = None     # torch's cheap forms: current device, stream of a device
+_plan = _rope = _paged = _vec = None
 
 
 def _setup():
-    global _INT32, _raw
+    """What the calls below look up once."""
+    global _INT32, _F32, _device, _raw_stream, _plan, _rope, _paged, _vec
     import torch
-    _INT32 = torch.int32
+    _INT32, _F32 = torch.int32, torch.float32
     _TYPE_IDS.update({torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16})
-    _raw = (torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+    _device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    L = lib()
+    _plan, _rope, _paged, _vec = L.b2q_kv_plan, L.b2q_qk_norm_rope, L.b2q_attention_paged, L.b2q_mul_vec_q4
 
 
 def _type_of(t) -> int:
@@ -511,23 +515,16 @@ def _rows(t, width: int, name: str) -> int:
     return ld if shape[0] > 1 else width
 
 
-def _on(stream, *tensors):
-    """The stream to launch on; every tensor (None skipped) is on the current device."""
-    if _raw is None:
-        _setup()
-    dev = _raw[0]()
+def _refuse_device(dev, *tensors):
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise B2QError(ERR_INVALID, f"a tensor on {t.device}, the current device is cuda:{dev}")
-    return stream.cuda_stream if stream is not None else _raw[1](dev)
 
 
 def _i32(t, n, name: str) -> int:
     """Address of a contiguous int32 tensor of n entries (None = any number)."""
     if t.dtype is not _INT32:
-        _setup()
-        if t.dtype is not _INT32:
-            raise B2QError(ERR_INVALID, f"{name} must be int32")
+        raise B2QError(ERR_INVALID, f"{name} must be int32")
     if not t.is_contiguous() or (n is not None and t.numel() != n):
         raise B2QError(ERR_SHAPE, f"{name} must be contiguous with {n} entries")
     return t.data_ptr()
@@ -545,9 +542,7 @@ def _f32(t, n: int, name: str):
 def _table(t):
     """(address, row stride, entries of a row, rows) of a block table."""
     if t.dtype is not _INT32:
-        _setup()
-        if t.dtype is not _INT32:
-            raise B2QError(ERR_INVALID, "block_table must be int32")
+        raise B2QError(ERR_INVALID, "block_table must be int32")
     shape = t.shape
     if len(shape) != 2:
         raise B2QError(ERR_SHAPE, "block_table must be [requests][max_blocks]")
@@ -566,7 +561,7 @@ class KVCache:
         _require(k.stride(3) == 1, "the elements of a head must be contiguous")
         self.k, self.v = k, v
         self.n_pages, self.n_kv_head, self.page_size, self.d_head = k.shape
-        self.dtype = k.dtype
+        self.dtype, self.device = k.dtype, k.get_device()
         self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _type_of(k), self.n_pages, self.page_size, self.n_kv_head,
                                 self.d_head, k.stride(0), k.stride(1), k.stride(2))
         self.ref = C.addressof(self.desc)
@@ -578,15 +573,30 @@ def kv_plan(ctx_len, new_len, page_size: int, free_pages, block_table, seq_of, p
     ctx_len, new_len: int32 [n_seq]; block_table: int32 [n_seq][max_blocks],
     entered in place; seq_of, pos, slot, kv_len: int32 [max_tokens] and counts
     int32 [2], written."""
-    n, rows = ctx_len.numel(), seq_of.numel()
+    if _plan is None:
+        _setup()
+    n, rows, i32, dev = ctx_len.numel(), seq_of.numel(), _INT32, _device()
     table, stride, width, requests = _table(block_table)
-    _require(requests == n, "block_table must be [n_seq][max_blocks]")
-    check(lib().b2q_kv_plan(_i32(ctx_len, n, "ctx_len"), _i32(new_len, n, "new_len"), n, page_size,
-                            _i32(free_pages, None, "free_pages"), free_pages.numel(), table, stride, width,
-                            rows, _i32(seq_of, rows, "seq_of"), _i32(pos, rows, "pos"),
-                            _i32(slot, rows, "slot"), _i32(kv_len, rows, "kv_len"),
-                            _i32(counts, 2, "counts"),
-                            _on(stream, ctx_len, new_len, free_pages, block_table, seq_of, pos, slot, kv_len, counts)))
+    if not (requests == n == new_len.numel() and rows == pos.numel() == slot.numel() == kv_len.numel()
+            and counts.numel() == 2 and ctx_len.is_contiguous() and new_len.is_contiguous()
+            and free_pages.is_contiguous() and seq_of.is_contiguous() and pos.is_contiguous()
+            and slot.is_contiguous() and kv_len.is_contiguous() and counts.is_contiguous()
+            and ctx_len.dtype is i32 and new_len.dtype is i32 and free_pages.dtype is i32 and seq_of.dtype is i32
+            and pos.dtype is i32 and slot.dtype is i32 and kv_len.dtype is i32 and counts.dtype is i32):
+        _require(requests == n, "block_table must be [n_seq][max_blocks]")
+        for name, t, k in (("ctx_len", ctx_len, n), ("new_len", new_len, n), ("free_pages", free_pages, None),
+                           ("seq_of", seq_of, rows), ("pos", pos, rows), ("slot", slot, rows),
+                           ("kv_len", kv_len, rows), ("counts", counts, 2)):
+            _i32(t, k, name)
+    if not (dev == ctx_len.get_device() == new_len.get_device() == free_pages.get_device() == block_table.get_device()
+            == seq_of.get_device() == pos.get_device() == slot.get_device() == kv_len.get_device()
+            == counts.get_device()):
+        _refuse_device(dev, ctx_len, new_len, free_pages, block_table, seq_of, pos, slot, kv_len, counts)
+    status = _plan(ctx_len.data_ptr(), new_len.data_ptr(), n, page_size, free_pages.data_ptr(), free_pages.numel(),
+                   table, stride, width, rows, seq_of.data_ptr(), pos.data_ptr(), slot.data_ptr(), kv_len.data_ptr(),
+                   counts.data_ptr(), _raw_stream(dev) if stream is None else stream.cuda_stream)
+    if status:
+        check(status)
 
 
 def rope_table(n_pos: int, rot_dim: int, theta: float = 10000.0, device="cuda"):
@@ -604,22 +614,31 @@ def qk_norm_rope(qkv, n_head: int, cache: KVCache, q_out, pos, slot, q_weight=No
     their cache slots (b2q_qk_norm_rope).  qkv: [rows][(n_head + 2 n_kv_head)
     d_head]; q_out: [rows][n_head d_head] of the cache's type; pos, slot: int32
     [rows]; rope: fp32 [n_pos][rot_dim] (see rope_table)."""
-    d = cache.d_head
+    if _rope is None:
+        _setup()
+    d, dev = cache.d_head, _device()
     ld = _rows(qkv, (n_head + 2 * cache.n_kv_head) * d, "qkv")
     ldq = _rows(q_out, n_head * d, "q_out")
     rows = qkv.shape[0]
     if q_out.shape[0] != rows or q_out.dtype is not cache.dtype:
         raise B2QError(ERR_SHAPE, "q_out must have qkv's rows and the cache's type")
-    n_pos = rot = 0
+    n_pos, rot, table = 0, 0, None
     if rope is not None:
-        if rope.dim() != 2 or not rope.is_contiguous() or _type_of(rope) != GGML_F32:
+        if rope.dim() != 2 or not rope.is_contiguous() or rope.dtype is not _F32:
             raise B2QError(ERR_SHAPE, "rope must be fp32 [n_pos][rot_dim]")
         n_pos, rot = rope.shape
-    check(lib().b2q_qk_norm_rope(qkv.data_ptr(), _type_of(qkv), ld, rows, n_head, _f32(q_weight, d, "q_weight"),
-                                 _f32(k_weight, d, "k_weight"), eps, rope.data_ptr() if rot else None, n_pos, rot,
-                                 interleaved, _i32(pos, rows, "pos"), _i32(slot, rows, "slot"),
-                                 q_out.data_ptr(), ldq, cache.ref,
-                                 _on(stream, qkv, q_out, pos, slot, q_weight, k_weight, rope, cache.k)))
+        if rot:
+            table = rope.data_ptr()
+    if not (dev == qkv.get_device() == q_out.get_device() == pos.get_device() == slot.get_device() == cache.device
+            and (rope is None or rope.get_device() == dev) and (q_weight is None or q_weight.get_device() == dev)
+            and (k_weight is None or k_weight.get_device() == dev)):
+        _refuse_device(dev, qkv, q_out, pos, slot, cache.k, rope, q_weight, k_weight)
+    status = _rope(qkv.data_ptr(), _type_of(qkv), ld, rows, n_head, _f32(q_weight, d, "q_weight"),
+                   _f32(k_weight, d, "k_weight"), eps, table, n_pos, rot, interleaved, _i32(pos, rows, "pos"),
+                   _i32(slot, rows, "slot"), q_out.data_ptr(), ldq, cache.ref,
+                   _raw_stream(dev) if stream is None else stream.cuda_stream)
+    if status:
+        check(status)
 
 
 def _paged_scratch_bytes(n_head: int, cache: KVCache) -> int:
@@ -643,8 +662,9 @@ def attention_paged(q, cache: KVCache, block_table, kv_len, out, scratch, seq_of
     (b2q_attention_paged).  q: [rows][n_head d_head] of the cache's type; out
     the same shape, fp32 or the cache's type; block_table: int32 [requests]
     [max_blocks]; kv_len (and seq_of): int32 [rows]; lse: fp32 [rows][n_head]."""
-    d = cache.d_head
-    shape = q.shape
+    if _paged is None:
+        _setup()
+    d, dev, shape = cache.d_head, _device(), q.shape
     if len(shape) != 2 or out.shape != shape or q.dtype is not cache.dtype:
         raise B2QError(ERR_SHAPE, "q and out must be [rows][n_head d_head], q of the cache's type")
     rows, width = shape
@@ -653,12 +673,17 @@ def attention_paged(q, cache: KVCache, block_table, kv_len, out, scratch, seq_of
     if scratch.numel() < _paged_scratch_bytes(n_head, cache):
         raise B2QError(ERR_SHAPE, "scratch smaller than attention_paged_scratch")
     table, stride, blocks, requests = _table(block_table)
-    check(lib().b2q_attention_paged(q.data_ptr(), ldq, rows, n_head, cache.ref, table, stride, blocks, requests,
-                                    None if seq_of is None else _i32(seq_of, rows, "seq_of"),
-                                    _i32(kv_len, rows, "kv_len"), d ** -0.5 if scale is None else scale, window,
-                                    out.data_ptr(), _type_of(out), ldo, _f32(lse, rows * n_head, "lse"),
-                                    scratch.data_ptr(),
-                                    _on(stream, q, cache.k, block_table, kv_len, out, scratch, seq_of, lse)))
+    if not (dev == q.get_device() == cache.device == block_table.get_device() == kv_len.get_device()
+            == out.get_device() == scratch.get_device() and (seq_of is None or seq_of.get_device() == dev)
+            and (lse is None or lse.get_device() == dev)):
+        _refuse_device(dev, q, cache.k, block_table, kv_len, out, scratch, seq_of, lse)
+    status = _paged(q.data_ptr(), ldq, rows, n_head, cache.ref, table, stride, blocks, requests,
+                    None if seq_of is None else _i32(seq_of, rows, "seq_of"), _i32(kv_len, rows, "kv_len"),
+                    d ** -0.5 if scale is None else scale, window, out.data_ptr(), _type_of(out), ldo,
+                    _f32(lse, rows * n_head, "lse"), scratch.data_ptr(),
+                    _raw_stream(dev) if stream is None else stream.cuda_stream)
+    if status:
+        check(status)
 
 
 class WeightQ4:
@@ -693,19 +718,27 @@ def mul_vec_q4(w: WeightQ4, x, m: int, y, bias=None, residual=None, stream=None)
     """y[m][n] = x @ w^T (+ bias) (+ residual) for few rows (b2q_mul_vec_q4).
     x: [m][x_cols] fp32, fp16 or bf16 (x_cols rounds up to the weight's K); y:
     [m][n] fp32 or x's type; bias fp32 [n]; residual fp32 like y."""
-    n = w.n
-    if x.dim() != 2:
+    if _vec is None:
+        _setup()
+    n, dev, shape = w.n, _device(), x.shape
+    if len(shape) != 2:
         raise B2QError(ERR_SHAPE, "x must be [m][x_cols]")
-    x_rows, x_cols = x.shape
+    x_rows, x_cols = shape
     ldx, ldy = _rows(x, x_cols, "x"), _rows(y, n, "y")
     if x_rows < m or y.shape[0] < m:
         raise B2QError(ERR_SHAPE, "x and y need m rows")
-    if residual is not None and (_type_of(residual) != GGML_F32 or residual.shape != y.shape
-                                 or _rows(residual, n, "residual") != ldy):
-        raise B2QError(ERR_SHAPE, "residual must be fp32 with y's rows and stride")
-    check(lib().b2q_mul_vec_q4(w.handle, x.data_ptr(), _type_of(x), m, x_cols, ldx, y.data_ptr(), _type_of(y), ldy,
-                               _f32(bias, n, "bias"), None if residual is None else residual.data_ptr(),
-                               _on(stream, x, y, bias, residual)))
+    res = None
+    if residual is not None:
+        if residual.dtype is not _F32 or residual.shape != y.shape or _rows(residual, n, "residual") != ldy:
+            raise B2QError(ERR_SHAPE, "residual must be fp32 with y's rows and stride")
+        res = residual.data_ptr()
+    if not (dev == x.get_device() == y.get_device() and (bias is None or bias.get_device() == dev)
+            and (residual is None or residual.get_device() == dev)):
+        _refuse_device(dev, x, y, bias, residual)
+    status = _vec(w.handle, x.data_ptr(), _type_of(x), m, x_cols, ldx, y.data_ptr(), _type_of(y), ldy,
+                  _f32(bias, n, "bias"), res, _raw_stream(dev) if stream is None else stream.cuda_stream)
+    if status:
+        check(status)
 
 
 class Gguf:
