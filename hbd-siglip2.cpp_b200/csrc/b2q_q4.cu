@@ -14,17 +14,17 @@
 //  * A nibble masked out of its word is an fp16 number as it stands, the
 //    subnormal q 2^-24 (in bits 0-3 of a half) or q 2^-20 (bits 4-7); the factor
 //    between the two is put into the activations.  Five instructions unpack eight
-//    weights: four masks and one shift.  The 8 of Q4_0 goes into the sums' start
-//    value, -8 X.
-//  * An activation row is scaled by a power of two to a largest value in
-//    [2^14, 2^15) and becomes fp16 operands: fp16 and bf16 values one, an fp32 value
-//    three (11 bits of its mantissa each), in as many of the eight activation
-//    columns; with one or two rows they are free.  What this loses lies 2^-36
-//    below the row's largest value.  (As bf16 the three pieces would need no scale,
-//    but bf16 holds one nibble in its mantissa, which takes 11 instructions for
-//    eight weights: 65 against 35 us for 256000 x 1152.)
-//  * S - 8 X leaves the tensor core once per block, is scaled by the fp32 value of d
-//    and summed in fp32.
+//    weights: four masks and one shift.  The 8 of Q4_0 is taken off the sums, as 8 X.
+//  * An activation row is scaled by a power of two and becomes fp16 operands: an fp32
+//    value three of 8 bits each, which sum to it, in as many of the eight activation
+//    columns (with one or two rows they are free); a bf16 value one; an fp16 value
+//    one, or two where the result keeps 32 bits.  8 bits and not the 11 that fp16
+//    holds: the tensor core aligns a sum's products to the largest and drops what
+//    falls below some 24 bits, which 12-bit products mostly stay clear of (relative
+//    error of 1 x 1152 x 4320: 2.1e-7; with pieces of 11 bits 5e-7, and 1.1e-6 where
+//    the sums start from -8 X).  The scale loses what lies 2^-30 below the row's
+//    largest value.
+//  * S leaves the tensor core once per block and is summed in fp32, d (S - 8 X).
 //
 // The weights are laid out at registration in the order the lanes want them:
 // per 16 rows a run of units of 128 columns, each 1024 bytes of nibbles (lane l of
@@ -36,6 +36,7 @@
 // tile, each taking every split-th unit, and add up in a fixed order.
 #include "b2q_decode.cuh"
 
+#include <cstddef>
 #include <new>
 #include <type_traits>
 
@@ -104,6 +105,7 @@ struct Q4Args {
     int64_t N;
     int tiles, units, split;
     int part_log2;          // 2^part_log2 lanes add up the warps of an output
+    bool pair;              // two CTAs stage the activations for one another
     const void* x;
     int x_type, pieces;
     int rows;               // activation rows of this launch
@@ -180,16 +182,20 @@ struct Eight {
 // from its first 32 values, the largest of them taken to [2^9, 2^10): that leaves
 // the row's largest value a factor of 32, and loses no more than 2^-30 of it.  The
 // same pass takes the peaks; a row that needs more room is staged again with the
-// power that its peak gives (`again`).
-template <class Tx, bool kMin, int kWarps>
+// power that its peak gives (`again`).  Two CTAs of a cluster (`pair`) stage half of
+// the work each and store it in both shared memories.
+template <class Tx, int kPieces, bool kMin, int kWarps>
 __device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState& st, bool again) {
-    constexpr int kPieces = std::is_same<Tx, float>::value ? 3 : 1;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int chunks = a.units * 16, segs = (chunks + 31) / 32;   // of 8 columns; of 32 chunks
     const Tx* px = static_cast<const Tx*>(a.x);
     const bool vec = (a.ldx * sizeof(Tx)) % 16 == 0 && (reinterpret_cast<uintptr_t>(px) & 15) == 0;
-    const int pairs = (a.rows + 1) / 2, row_step = kWarps / segs, seg_step = kWarps % segs;
-    int m = warp / segs, seg = warp % segs;
+    const int pairs = (a.rows + 1) / 2;
+    const uint32_t rank = a.pair ? cluster_rank() : 0, here = smem_u32(smem), state = smem_u32(&st);
+    const uint32_t there = a.pair ? in_cta(here, rank ^ 1) : 0, state_there = a.pair ? in_cta(state, rank ^ 1) : 0;
+    const int workers = a.pair ? 2 * kWarps : kWarps, worker = warp + (rank ? kWarps : 0);
+    const int row_step = workers / segs, seg_step = workers % segs;
+    int m = worker / segs, seg = worker % segs;
     Eight<Tx> next;
     Tx next_sample = from_f32<Tx>(0.f);
     auto load = [&]() {
@@ -232,6 +238,11 @@ __device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState
                 atomicMax(&st.peak[row], peak);
                 if (odd) atomicOr(&st.odd, 1u << row);
                 st.shift[row] = shift;   // every warp of the row finds the same
+                if (a.pair) {
+                    max_cluster_32(state_there + offsetof(RowState, peak) + 4 * row, peak);
+                    if (odd) or_cluster_32(state_there + offsetof(RowState, odd), 1u << row);
+                    st_cluster_32(state_there + offsetof(RowState, shift) + 4 * row, static_cast<uint32_t>(shift));
+                }
             }
         }
         const float s = pow2(shift), s16 = s * 0.0625f;
@@ -248,22 +259,24 @@ __device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState
             x.x *= j & 1 ? s16 : s;   // where the nibble stands four bits higher
             x.y *= j & 1 ? s16 : s;
 #pragma unroll
-            for (int z = 0; z < kPieces; ++z) {
-                p[z][j] = pack2<__half>(x.x, x.y);
-                if (z + 1 < kPieces) {
-                    const float2 h = unpack2<__half>(p[z][j]);
-                    x.x -= h.x;
-                    x.y -= h.y;
-                }
+            for (int z = 0; z + 1 < kPieces; ++z) {   // 8 bits, as fp16
+                const float2 h = unpack2<__nv_bfloat16>(pack2<__nv_bfloat16>(x.x, x.y));
+                p[z][j] = pack2<__half>(h.x, h.y);
+                x.x -= h.x;
+                x.y -= h.y;
             }
+            p[kPieces - 1][j] = pack2<__half>(x.x, x.y);
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         if (c < chunks) {
-            uint8_t* dst = smem + row * a.pitch + c * 16;
+            const int dst = row * a.pitch + c * 16;
 #pragma unroll
-            for (int z = 0; z < kPieces; ++z)
-                *reinterpret_cast<uint4*>(dst + z * a.rows * a.pitch) = make_uint4(p[z][0], p[z][1], p[z][2], p[z][3]);
+            for (int z = 0; z < kPieces; ++z) {
+                const uint4 v = make_uint4(p[z][0], p[z][1], p[z][2], p[z][3]);
+                *reinterpret_cast<uint4*>(smem + dst + z * a.rows * a.pitch) = v;
+                if (a.pair) st_cluster_128(there + dst + z * a.rows * a.pitch, v);
+            }
             if ((c & 3) == 0) {
                 const int unit = c >> 4, block = (c >> 2) & 3;
                 if constexpr (kMin) {
@@ -275,13 +288,19 @@ __device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState
                         sum -= __half2float(h[z]);
                     }
                     h[3] = __float2half_rn(0.f);
-                    *reinterpret_cast<uint2*>(smem + a.sum_at + ((unit * a.rows + row) * 4 + block) * 8) =
-                        *reinterpret_cast<const uint2*>(h);
+                    const int at = a.sum_at + ((unit * a.rows + row) * 4 + block) * 8;
+                    *reinterpret_cast<uint2*>(smem + at) = *reinterpret_cast<const uint2*>(h);
+                    if (a.pair) st_cluster_64(there + at, *reinterpret_cast<const uint2*>(h));
                 } else {
-                    float* out = reinterpret_cast<float*>(smem + a.sum_at) +
-                                 ((unit * pairs + (row >> 1)) * 4 + block) * 2 + (row & 1);
-                    out[0] = sum * -4.76837158203125e-7f;
-                    if (row + 1 == a.rows && !(row & 1)) out[1] = 0.f;
+                    const int at = a.sum_at + (((unit * pairs + (row >> 1)) * 4 + block) * 2 + (row & 1)) * 4;
+                    const float v = sum * -4.76837158203125e-7f;
+                    const bool last = row + 1 == a.rows && !(row & 1);   // the pair's other row is none
+                    *reinterpret_cast<float*>(smem + at) = v;
+                    if (last) *reinterpret_cast<float*>(smem + at + 4) = 0.f;
+                    if (a.pair) {
+                        st_cluster_32(there + at, __float_as_uint(v));
+                        if (last) st_cluster_32(there + at + 4, 0u);
+                    }
                 }
             }
         }
@@ -294,15 +313,20 @@ __device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState
 template <bool kMin, int kWarps>
 __device__ __forceinline__ void stage_rows(const Q4Args& a, uint8_t* smem, RowState& st) {
     const int tid = threadIdx.x;
+    auto meet = [&]() {
+        if (a.pair) cluster_sync();
+        else __syncthreads();
+    };
     if (tid < kMaxRows) st.peak[tid] = 0;
     if (tid == 0) st.odd = 0;
-    __syncthreads();
+    meet();
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
-        if (a.x_type == B2Q_TYPE_F32) stage_x<float, kMin, kWarps>(a, smem, st, pass);
-        else if (a.x_type == B2Q_TYPE_F16) stage_x<__half, kMin, kWarps>(a, smem, st, pass);
-        else stage_x<__nv_bfloat16, kMin, kWarps>(a, smem, st, pass);
-        __syncthreads();
+        if (a.x_type == B2Q_TYPE_F32) stage_x<float, 3, kMin, kWarps>(a, smem, st, pass);
+        else if (a.x_type == B2Q_TYPE_BF16) stage_x<__nv_bfloat16, 1, kMin, kWarps>(a, smem, st, pass);
+        else if (a.pieces == 1) stage_x<__half, 1, kMin, kWarps>(a, smem, st, pass);
+        else stage_x<__half, 2, kMin, kWarps>(a, smem, st, pass);
+        meet();   // (peaks and shifts are the same in both CTAs of a pair, and so is what follows)
         const bool mine = pass == 0 && tid < a.rows;
         const bool over = mine && st.shift[tid] > top_shift(st.peak[tid]);
         if (over) st.shift[tid] = top_shift(st.peak[tid]);
@@ -398,7 +422,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
     }
     int slot = ring, buf = 0;
     for (int tile = first; tile < a.tiles; tile += step, buf ^= 1) {
-        float acc[kN][4] = {}, accm[kN][4] = {};   // sums with d, sums with m
+        float acc[kN][4] = {};
         int xo = 0, so[kN];
 #pragma unroll
         for (int n = 0; n < kN; ++n) so[n] = sum0[n];
@@ -422,7 +446,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
                     const uint2 xp = *reinterpret_cast<const uint2*>(smem + so[n]);
-                    mma_16816<__half>(accm[n], m0, m8, m0, m8, xp.x, xp.y);
+                    float v[4];
+                    mma_16816_from0(v, m0, m8, m0, m8, xp.x, xp.y);
+                    // X was scaled by 2^-5, the nibbles by 2^-24
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(v[e], 1.9073486328125e-6f, acc[n][e]);
                 }
             }
 #pragma unroll
@@ -437,8 +465,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
                     float2 x = make_float2(0.f, 0.f);
                     if constexpr (!kMin) x = *reinterpret_cast<const float2*>(smem + so[n] + b * 8);
                     float s[4];
-                    mma_16816_start(s, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y, x.x, x.y);
+                    mma_16816_from0(s, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
                     mma_16816<__half>(s, lo[2], hi[2], lo[3], hi[3], xv.z, xv.w);
+                    if constexpr (!kMin) {
+                        s[0] += x.x;
+                        s[1] += x.y;
+                        s[2] += x.x;
+                        s[3] += x.y;
+                    }
                     acc[n][0] = fmaf(d.x, s[0], acc[n][0]);
                     acc[n][1] = fmaf(d.x, s[1], acc[n][1]);
                     acc[n][2] = fmaf(d.y, s[2], acc[n][2]);
@@ -457,9 +491,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
         for (int n = 0; n < kN; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                // Q4_1: the operands of m were scaled by 2^-5, those of d by 2^-24
-                const float v = kMin ? fmaf(accm[n][e], 1.9073486328125e-6f, acc[n][e]) : acc[n][e];
-                if (n * 8 + 2 * t + (e & 1) < cols) red[8 * (e >> 1) * pitch + n * 8 + (e & 1)] = v;
+                if (n * 8 + 2 * t + (e & 1) < cols) red[8 * (e >> 1) * pitch + n * 8 + (e & 1)] = acc[n][e];
             }
         if (split == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(group), "r"(split * 32) : "memory");
@@ -472,7 +504,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
             if (in) {
                 const float* p = all + part * part_floats + row * pitch + m;
                 for (int w = part; w < split; w += 1 << a.part_log2, p += part_floats << a.part_log2)
-                    v += a.pieces == 3 ? p[0] + (p[a.rows] + p[2 * a.rows]) : p[0];
+                    v += a.pieces == 1 ? p[0] : a.pieces == 2 ? p[0] + p[a.rows] : p[0] + (p[a.rows] + p[2 * a.rows]);
             }
             for (int x = 1 << a.part_log2 >> 1; x; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
             if (!in || part || n >= a.N) continue;
@@ -628,8 +660,8 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool min = w->type == B2Q_TYPE_Q4_1;
     const int units = static_cast<int>(w->units);
-    const int pieces = x_dtype == B2Q_TYPE_F32 ? 3 : 1;
-    const size_t es = pieces == 3 ? 4 : 2, ys = y_dtype == B2Q_TYPE_F32 ? 4 : 2;
+    const int pieces = x_dtype == B2Q_TYPE_F32 ? 3 : x_dtype == B2Q_TYPE_F16 && y_dtype == B2Q_TYPE_F32 ? 2 : 1;
+    const size_t es = x_dtype == B2Q_TYPE_F32 ? 4 : 2, ys = y_dtype == B2Q_TYPE_F32 ? 4 : 2;
     const int64_t per_sm = (w->tiles + ds->num_sms - 1) / ds->num_sms * units;
     auto plan_rows = [&](int rows) {
         const int n = n_tiles_of(rows, pieces);
@@ -645,9 +677,13 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
         const Q4Plan p = plan_rows(rows);
         if (!p.stages) return set_error(B2Q_ERR_SHAPE, "an activation row does not fit shared memory");
         const int split = split_of(w->tiles, units, ds->num_sms, warps);
-        const unsigned grid = static_cast<unsigned>(w->tiles < ds->num_sms ? w->tiles : ds->num_sms);
+        // Pairs where each warp would stage more than two pieces of 256 columns by itself
+        // (7 rows of 8,192: 33.7 -> PAIRED us); an SM may stay idle where their number is odd.
+        const bool pair = rows * ((units + 1) / 2) > 2 * warps && w->tiles > 1 && ds->num_sms >= 2;
+        unsigned grid = static_cast<unsigned>(w->tiles < ds->num_sms ? w->tiles : ds->num_sms);
+        if (pair) grid = grid / 2 * 2;
         const Q4Args a{w->packed, w->N, static_cast<int>(w->tiles), units, split,
-                       part_log2_of(split, rows),
+                       part_log2_of(split, rows), pair,
                        static_cast<const uint8_t*>(x) + m0 * ldx * es, x_dtype, pieces, rows, x_cols, ldx,
                        static_cast<uint8_t*>(y) + m0 * ldy * ys, ldy, y_dtype == B2Q_TYPE_F32, bias,
                        residual ? residual + m0 * ldy : nullptr, p.pitch, p.ring_at, p.red_at, p.sum_at};
@@ -657,7 +693,7 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
             static std::atomic<uint64_t> allowed{0};
             const b2q_status st = allow_smem(kernel, kSmemMax, allowed, ds->device);
             if (st) return st;
-            return cuda_check(launch_after(kernel, dim3(grid), dim3(warps * 32), p.bytes, s, a),
+            return cuda_check(launch_after(pair ? 2 : 1, kernel, dim3(grid), dim3(warps * 32), p.bytes, s, a),
                               "4-bit product launch");
         };
         auto with_stages = [&](auto mn, auto nt, auto wp) {
