@@ -69,7 +69,7 @@ struct Shape {
 template <int DP, int kRows>
 constexpr int smem_bytes() {
     constexpr int ring = kWarps * Shape<DP>::kStages * Shape<DP>::kStageBytes;
-    constexpr int join = 2 * kRows * kMaxCtas * 4 + kThreads * 16;
+    constexpr int join = 2 * kRows * (kMaxCtas + 2) * 4 + kThreads * 16;
     return ring > join ? ring : join;
 }
 // floats of one partial result: output rows, then refs and sums
@@ -346,45 +346,49 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
             }
             cp_commit();
         };
-        Pending first[S::kStages];
-#pragma unroll
-        for (int i = 0; i < S::kStages; ++i) first[i] = look_up();
-#pragma unroll
-        for (int i = 0; i < S::kStages - 1; ++i) issue(first[i], i);
-        Pending next = first[S::kStages - 1];
-
         uint32_t qf[kSteps][4];
         constexpr int kHalves = kPacked ? 1 : 2;   // sets of 8 query rows
         float o[kCols][2 * kHalves];
         float ref[2], sum[2];
-        bool fresh = true;
+        auto new_group = [&]() {   // its queries, empty sums
+            const int hk = cu.hm / a.row_blocks, q0 = (cu.hm % a.row_blocks) * kRows;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int row = q0 + g + 8 * x;
+                const bool in = row < a.group && (x == 0 || !kPacked);
+                const T* q = a.q + cu.r * a.ldq + static_cast<int64_t>(hk * a.group + (in ? row : 0)) * a.d;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int col = k * 16 + y * 8 + 2 * t4;
+                        qf[k][x + 2 * y] = in && col < a.d ? *reinterpret_cast<const uint32_t*>(q + col) : 0u;
+                    }
+                ref[x] = -INFINITY;
+                sum[x] = 0.f;
+            }
+#pragma unroll
+            for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                for (int x = 0; x < 2 * kHalves; ++x) o[n][x] = 0.f;
+        };
+        Pending first[S::kStages];
+#pragma unroll
+        for (int i = 0; i < S::kStages; ++i) first[i] = look_up();
+        new_group();   // (queries asked for before the keys fill the queues)
+#pragma unroll
+        for (int i = 0; i < S::kStages - 1; ++i) issue(first[i], i);
+        Pending next = first[S::kStages - 1];
+
+        bool fresh = false;
         int stage = 0;
 
         for (int i = 0; i < n_units; ++i) {
             issue(next, stage == 0 ? S::kStages - 1 : stage - 1);
             next = look_up();
-            if (fresh) {   // a new group: its queries, empty sums
+            if (fresh) {
                 fresh = false;
-                const int hk = cu.hm / a.row_blocks, q0 = (cu.hm % a.row_blocks) * kRows;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int row = q0 + g + 8 * x;
-                    const bool in = row < a.group && (x == 0 || !kPacked);
-                    const T* q = a.q + cu.r * a.ldq + static_cast<int64_t>(hk * a.group + (in ? row : 0)) * a.d;
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const int col = k * 16 + y * 8 + 2 * t4;
-                            qf[k][x + 2 * y] = in && col < a.d ? *reinterpret_cast<const uint32_t*>(q + col) : 0u;
-                        }
-                    ref[x] = -INFINITY;
-                    sum[x] = 0.f;
-                }
-#pragma unroll
-                for (int n = 0; n < kCols; ++n)
-#pragma unroll
-                    for (int x = 0; x < 2 * kHalves; ++x) o[n][x] = 0.f;
+                new_group();
             }
             cp_wait<S::kStages - 1>();
             __syncwarp();
@@ -564,24 +568,42 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
             s_last[warp] = parts;
         }
         __syncthreads();
-        for (int x = 0; x < 2; ++x) {
-            const int n_parts = s_last[x];
-            if (!n_parts) continue;
+        // One group: all threads join it.  Two: half of the threads each.
+        const int n0 = s_last[0], n1 = s_last[1], teams = (n0 != 0) + (n1 != 0);
+        if (teams) {
+            const int team_threads = kThreads / teams, team = tid / team_threads, me = tid % team_threads;
+            const int x = teams == 2 ? team : n0 ? 0 : 1;
             const Partial pt = s_partial[x];
+            const int n_parts = x ? n1 : n0, n_out = pt.rows * (DP / 4);
             const auto part_of = [&](int p) {
                 return a.parts + (2 * static_cast<int64_t>(pt.c0 + p) + (p == 0 ? 1 : 0)) * kPart;
             };
-            // refs and sums of all parts (the ring is free now: kRows x kMaxCtas x 2 floats fit it)
-            float* wt = reinterpret_cast<float*>(smem);           // [parts][rows] refs, then weights
-            float* sm = wt + n_parts * pt.rows;                   // [parts][rows] sums
-            __syncthreads();
-            for (int i = tid; i < n_parts * pt.rows; i += kThreads) {
+            // shared: per team refs (then weights) and sums of all parts, and half-way outputs (the ring is free now)
+            constexpr int kTeamFloats = 2 * kRows * (kMaxCtas + 2);
+            float* wt = reinterpret_cast<float*>(smem) + (x ? 2 * kRows * (n0 ? n0 : 0) : 0);
+            float* sm = wt + n_parts * pt.rows;
+            float4* red = reinterpret_cast<float4*>(smem + kTeamFloats * 4);
+            // Few outputs: the parts too are dealt to threads, and added up in a second step.
+            const int subs = n_out < team_threads ? min(team_threads / n_out, n_parts) : 1;
+            const int sub = subs > 1 ? me / n_out : 0, e0 = subs > 1 ? me % n_out : me;
+            constexpr int kEach = (kRows * DP / 4 + kThreads / 2 - 1) / (kThreads / 2);   // outputs of a thread, at most
+            constexpr int kFirst = kEach <= 8 ? 2 : 1;   // its parts that are asked for at once, with the refs
+            float4 early[kFirst][kEach];
+#pragma unroll
+            for (int k = 0; k < kFirst; ++k)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int p = sub + k * subs, e = e0 + i * team_threads;
+                    if (sub < subs && p < n_parts && e < n_out)
+                        early[k][i] = __ldcg(reinterpret_cast<const float4*>(part_of(p)) + e);
+                }
+            for (int i = me; i < n_parts * pt.rows; i += team_threads) {
                 const float* q = part_of(i / pt.rows) + kRows * DP + i % pt.rows;
                 wt[i] = __ldcg(q);
                 sm[i] = __ldcg(q + kRows);
             }
             __syncthreads();
-            for (int row = warp; row < pt.rows; row += kWarps) {
+            for (int row = me / 32; row < pt.rows; row += team_threads / 32) {
                 float m = -INFINITY, l = 0.f;
                 for (int p = lane; p < n_parts; p += 32) m = fmaxf(m, wt[p * pt.rows + row]);
                 for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
@@ -592,55 +614,54 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
                 }
                 for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
                 if (lane == 0) {
-                    s_sum[0][row] = l;
+                    s_sum[x][row] = l;
                     write_lse(a, pt.r, pt.head0 + row, m, l);
                 }
             }
             __syncthreads();
-            // The outputs.  Few outputs: the parts too are dealt to threads, and added up
-            // in a second step; the loads of all outputs and four parts are in flight.
-            constexpr int kEach = (kRows * DP / 4 + kThreads - 1) / kThreads;
-            const int n_out = pt.rows * (DP / 4), subs = n_out < kThreads ? min(kThreads / n_out, n_parts) : 1;
-            const int sub = subs > 1 ? tid / n_out : 0, e0 = subs > 1 ? tid % n_out : tid;
             float4 acc[kEach];
 #pragma unroll
             for (int i = 0; i < kEach; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto add = [&](int i, int p, int e, float4 v) {
+                const float f = wt[p * pt.rows + e / (DP / 4)];
+                acc[i].x = fmaf(f, v.x, acc[i].x);
+                acc[i].y = fmaf(f, v.y, acc[i].y);
+                acc[i].z = fmaf(f, v.z, acc[i].z);
+                acc[i].w = fmaf(f, v.w, acc[i].w);
+            };
             if (sub < subs) {
+#pragma unroll
+                for (int k = 0; k < kFirst; ++k)
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {
+                        const int p = sub + k * subs, e = e0 + i * team_threads;
+                        if (p < n_parts && e < n_out) add(i, p, e, early[k][i]);
+                    }
 #pragma unroll 4
-                for (int p = sub; p < n_parts; p += subs) {
+                for (int p = sub + kFirst * subs; p < n_parts; p += subs) {
                     const float4* q = reinterpret_cast<const float4*>(part_of(p));
 #pragma unroll
                     for (int i = 0; i < kEach; ++i) {
-                        const int e = e0 + i * kThreads;
-                        if (e < n_out) {
-                            const float f = wt[p * pt.rows + e / (DP / 4)];
-                            const float4 v = __ldcg(q + e);
-                            acc[i].x = fmaf(f, v.x, acc[i].x);
-                            acc[i].y = fmaf(f, v.y, acc[i].y);
-                            acc[i].z = fmaf(f, v.z, acc[i].z);
-                            acc[i].w = fmaf(f, v.w, acc[i].w);
-                        }
+                        const int e = e0 + i * team_threads;
+                        if (e < n_out) add(i, p, e, __ldcg(q + e));
                     }
                 }
             }
-            if (subs > 1) {
-                float4* red = reinterpret_cast<float4*>(smem + 2 * kRows * kMaxCtas * 4);
-                if (sub < subs) red[tid] = acc[0];
-                __syncthreads();
-                if (tid < n_out)
-                    for (int k = 1; k < subs; ++k) {
-                        const float4 v = red[k * n_out + tid];
-                        acc[0].x += v.x;
-                        acc[0].y += v.y;
-                        acc[0].z += v.z;
-                        acc[0].w += v.w;
-                    }
-            }
+            if (subs > 1 && sub < subs) red[tid] = acc[0];
+            __syncthreads();
+            if (subs > 1 && sub == 0)
+                for (int k = 1; k < subs; ++k) {
+                    const float4 v = red[tid + k * n_out];
+                    acc[0].x += v.x;
+                    acc[0].y += v.y;
+                    acc[0].z += v.z;
+                    acc[0].w += v.w;
+                }
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
-                const int e = e0 + i * kThreads;
+                const int e = e0 + i * team_threads;
                 if (sub == 0 && e < n_out)
-                    write_out<To>(a, pt.r, pt.head0 + e / (DP / 4), e % (DP / 4) * 4, acc[i], s_sum[0][e / (DP / 4)]);
+                    write_out<To>(a, pt.r, pt.head0 + e / (DP / 4), e % (DP / 4) * 4, acc[i], s_sum[x][e / (DP / 4)]);
             }
         }
     }
