@@ -57,6 +57,34 @@ def quantize_q8_0(w: np.ndarray, k_pad: int | None = None) -> np.ndarray:
     return out.reshape(n, (kp // QK) * Q8_0_BLOCK_BYTES)
 
 
+def quantize_q4_0(w: np.ndarray) -> np.ndarray:
+    """Quantize rows of ``w`` ([N][K] fp32, K a multiple of 32) to ggml Q4_0
+    bytes ([N][K/32*18]): d = m / -8 for the value m of largest size, q =
+    trunc(x / d + 8.5) up to 15; low nibbles hold the first 16 values."""
+    w = np.ascontiguousarray(w, dtype=np.float32)
+    n, k = w.shape
+    if k % QK:
+        raise ValueError(f"K={k} is not a multiple of {QK}")
+    blocks = w.reshape(-1, QK)
+    m = np.take_along_axis(blocks, np.abs(blocks).argmax(axis=1)[:, None], 1)
+    d = m / np.float32(-8)
+    with np.errstate(divide="ignore"):
+        inv = np.where(d == 0, np.float32(0), np.float32(1) / d).astype(np.float32)
+    q = np.minimum(np.trunc(blocks * inv + np.float32(8.5)), 15).astype(np.uint8)
+    out = np.empty((blocks.shape[0], 18), np.uint8)
+    out[:, :2] = d.astype(np.float16).view(np.uint8)
+    out[:, 2:] = q[:, :16] | (q[:, 16:] << 4)
+    return out.reshape(n, k // QK * 18)
+
+
+def dequantize_q4_0(q: np.ndarray, k: int) -> np.ndarray:
+    """Q4_0 bytes ([N][K/32*18]) as [N][K] fp32."""
+    blocks = np.ascontiguousarray(q).reshape(-1, 18)
+    d = blocks[:, :2].copy().view(np.float16).astype(np.float32)
+    v = np.concatenate([blocks[:, 2:] & 15, blocks[:, 2:] >> 4], 1).astype(np.float32) - 8
+    return (v * d).reshape(-1, k)
+
+
 def dequantize_q8_0(q: np.ndarray, kp: int) -> np.ndarray:
     n = q.shape[0]
     b = q.reshape(-1, Q8_0_BLOCK_BYTES)

@@ -127,7 +127,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
         int ctx, add;
         lengths_of(a, s, ctx, add, bad);
         const int b = blocks_of(a, ctx) + (i - pages[s]);
-        a.table[s * a.bt_stride + b] = i < a.n_free ? a.free_pages[i] : -1;
+        const int page = i < a.n_free ? a.free_pages[i] : -1;
+        if (page < 0) report(a.err, kDevPlanFull);   // a negative entry ends the list
+        a.table[s * a.bt_stride + b] = page < 0 ? -1 : page;
     }
     for (int t = at; t < a.max_tokens; t += step) {
         int seq = -1, pos = -1, slot = -1, len = 0;
