@@ -213,7 +213,7 @@ inline b2q_status check_cache(const b2q_kv_cache* in, b2q_kv_cache* c) {
     *c = *in;
     if (c->dtype != B2Q_TYPE_F16 && c->dtype != B2Q_TYPE_BF16)
         return set_error(B2Q_ERR_INVALID, "the cache must be F16 or BF16");
-    if (c->n_pages <= 0 || c->n_kv_head <= 0) return set_error(B2Q_ERR_SHAPE, "bad n_pages / n_kv_head");
+    if (c->n_pages <= 0 || c->n_kv_head <= 0 || c->n_kv_head > 65535) return set_error(B2Q_ERR_SHAPE, "bad n_pages / n_kv_head");
     if (c->page_size <= 0 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
         return set_error(B2Q_ERR_SHAPE, "page_size must be a power of two up to 1024");
     if (static_cast<int64_t>(c->n_pages) * c->page_size > INT32_MAX)

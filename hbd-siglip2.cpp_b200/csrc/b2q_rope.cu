@@ -12,10 +12,11 @@
 // first is used; the row's position, slot and rotation values are fetched once for
 // both.  Norm and pairing are compiled in and lanes without a piece read the first
 // one's: instructions, not bytes, were the limit before (19 an element).
-// Measured on one B200, 20,011 rows of 24 + 2 x 4 heads of 128, fp16, half rotated,
-// 333 MB: 61 us, 5.46 TB/s (one head a group 67, four 69); 20,000 rows of 32 + 2 x 8
-// heads, bf16, normed and rotated, 502 MB: 102 us, 4.92 TB/s (141, 153).  Heads of 72
-// (36 pairs: pieces of 4, 9 of 16 lanes at work) reach 2.9 TB/s.
+// Measured on one B200 (copy bandwidth 6.53 TB/s): 20,011 rows of 24 + 2 x 4 heads of
+// 128, fp16, half rotated, 333 MB: 60 us, 5.54 TB/s (one head a group 67, four 69);
+// 20,000 rows of 32 + 2 x 8 heads, bf16, normed and rotated, 502 MB: 100 us, 5.0 TB/s
+// (141, 153); 20,000 rows of 48 heads of 72, fp32 in, normed and rotated, 421 MB: 119
+// us, 3.5 TB/s (pieces of 4 instead of 12: 146); 256 rows: 2.8 us, the launch.
 #include "b2q_decode.cuh"
 
 #include <type_traits>
@@ -65,21 +66,24 @@ __device__ __forceinline__ RowPlace place_of(const RopeArgs<Tin, Tc>& a, int64_t
     return o;
 }
 
-// kVec elements in 16-byte (or 8-byte) accesses
+// kVec elements in 16-byte accesses, or 8-byte ones where they are not a multiple
 template <class T, int kVec>
 struct Piece {
     static constexpr int kWords = kVec * sizeof(T) / 4;
     uint32_t w[kWords];
     __device__ __forceinline__ void load(const T* p) {
-        if constexpr (kWords >= 4) {
+        if constexpr (kWords % 4 == 0) {
 #pragma unroll
             for (int i = 0; i < kWords / 4; ++i) {
                 const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + i);
                 w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
             }
         } else {
-            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
-            w[0] = v.x, w[1] = v.y;
+#pragma unroll
+            for (int i = 0; i < kWords / 2; ++i) {
+                const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p) + i);
+                w[2 * i] = v.x, w[2 * i + 1] = v.y;
+            }
         }
     }
     __device__ __forceinline__ void get(float (&x)[kVec]) const {
@@ -97,14 +101,21 @@ __device__ __forceinline__ void store_piece(T* p, const float (&x)[kVec]) {
     uint32_t w[kVec / 2];
 #pragma unroll
     for (int i = 0; i < kVec / 2; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-    if constexpr (kVec == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    if constexpr (kVec == 8) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec / 4; ++i) reinterpret_cast<uint2*>(p)[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+    }
 }
 template <int kN>
 __device__ __forceinline__ void load_f32(const float* p, float (&x)[kN]) {
-    if constexpr (kN == 2) {
-        const float2 v = __ldg(reinterpret_cast<const float2*>(p));
-        x[0] = v.x, x[1] = v.y;
+    if constexpr (kN % 4) {
+#pragma unroll
+        for (int i = 0; i < kN / 2; ++i) {
+            const float2 v = __ldg(reinterpret_cast<const float2*>(p) + i);
+            x[2 * i] = v.x, x[2 * i + 1] = v.y;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < kN / 4; ++i) {
@@ -293,15 +304,16 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(RopeArgs<Tin,
 }
 
 // Pieces of 8 elements where every row, cache row and rotation half is made of
-// whole aligned ones, of 4 where that holds for 4 (halves such as 36 of 72), else the
+// whole aligned ones, else of 12 or of 4 where that holds for them (halves of 36, in
+// heads of 72: three of four lanes at work instead of nine of sixteen), else the
 // element-wise kernel.
 template <class Tin, class Tc>
 cudaError_t launch(const RopeArgs<Tin, Tc>& a, cudaStream_t s) {
     const int64_t items = a.n_rows * (a.n_head + 2 * a.n_kv);
     auto fits = [&](int vec) {
-        const size_t in = vec * sizeof(Tin) < 16 ? vec * sizeof(Tin) : 16, out = vec * 2;
+        const size_t in = vec * sizeof(Tin) % 16 ? 8 : 16, out = vec * 2 % 16 ? 8 : 16;
         const int unit = a.interleaved ? vec : 2 * vec;
-        return a.rot % unit == 0 && a.d / vec <= 64 && ptr_aligned(a.x, in) && a.ld * sizeof(Tin) % in == 0 &&
+        return a.d % vec == 0 && a.rot % unit == 0 && a.d / vec <= 64 && ptr_aligned(a.x, in) && a.ld * sizeof(Tin) % in == 0 &&
                ptr_aligned(a.q, out) && a.ldq * 2 % out == 0 && ptr_aligned(a.qw, 16) && ptr_aligned(a.kw, 16) &&
                ptr_aligned(a.rope, 16);
     };
@@ -323,9 +335,10 @@ cudaError_t launch(const RopeArgs<Tin, Tc>& a, cudaStream_t s) {
                                 block, 0, s, a);
         };
         auto with_heads = [&](auto norm, auto inter) {
-            // one head a group until the lanes fill the GPU (half a million), for the shorter wait
-            return items * group < (1 << 19) ? with(std::integral_constant<int, 1>{}, norm, inter)
-                                             : with(std::integral_constant<int, 2>{}, norm, inter);
+            // two heads a group once the lanes fill the GPU (half a million); one waits less
+            if constexpr (kVec <= 8)   // (pieces of 12 fill the registers with one)
+                if (items * group >= (1 << 19)) return with(std::integral_constant<int, 2>{}, norm, inter);
+            return with(std::integral_constant<int, 1>{}, norm, inter);
         };
         auto with_norm = [&](auto inter) {
             return a.qw || a.kw ? with_heads(std::true_type{}, inter) : with_heads(std::false_type{}, inter);
@@ -333,6 +346,7 @@ cudaError_t launch(const RopeArgs<Tin, Tc>& a, cudaStream_t s) {
         return a.interleaved ? with_norm(std::true_type{}) : with_norm(std::false_type{});
     };
     if (fits(8)) return go(std::integral_constant<int, 8>{});
+    if (fits(12)) return go(std::integral_constant<int, 12>{});
     if (fits(4)) return go(std::integral_constant<int, 4>{});
     return launch_after(rope_any_kernel<Tin, Tc>, dim3(static_cast<unsigned>((items + kRopeWarps - 1) / kRopeWarps)),
                         dim3(kRopeWarps * 32), 0, s, a);

@@ -389,7 +389,8 @@ b2q_status b2q_attention_paged(const void *q, int64_t ldq, int64_t n_rows, int32
 /* ---- matrix-vector products with 4-bit weights -------------------------------
  * A registered ggml Q4_0 tensor (18-byte blocks of 32: fp16 d, 16 bytes of
  * nibbles, low nibbles first; w = d (q - 8)) or Q4_1 (20 bytes: fp16 d, fp16
- * m; w = d q + m): N rows of K (a multiple of 32), row stride row_bytes.
+ * m; w = d q + m): N rows of K (a multiple of 32 up to 28672), row stride
+ * row_bytes.
  * Repacked once; synchronises `stream`; the source is not retained. */
 typedef struct b2q_weight_q4 b2q_weight_q4;
 b2q_status b2q_weight_q4_register(const void *blocks, int32_t ggml_type, int64_t N, int64_t K, int64_t row_bytes,
@@ -399,8 +400,10 @@ b2q_status b2q_weight_q4_release(b2q_weight_q4 *w);
  * x[M][ldx] (x_dtype F32, F16 or BF16) of x_cols columns, x_cols rounded up to
  * 32 = K (columns x_cols..K-1 read as zero).  y (y_dtype F32 or x_dtype) and
  * residual (fp32, may be y) have row stride ldy; bias and residual may be
- * NULL.  The activations are not quantized: products and sums are in fp32,
- * rounded once.  Meant for few rows (one weight pass per eight or so). */
+ * NULL; y overlaps neither x nor bias.  The activations are not quantized:
+ * products and sums are in fp32, rounded once.  Meant for few rows: a launch
+ * takes up to 32 fp16 or bf16 rows or ten fp32 ones, fewer where their columns
+ * do not fit shared memory, and reads the weights once. */
 b2q_status b2q_mul_vec_q4(const b2q_weight_q4 *w, const void *x, int32_t x_dtype, int64_t M, int64_t x_cols,
                           int64_t ldx, void *y, int32_t y_dtype, int64_t ldy, const float *bias,
                           const float *residual, void *stream);

@@ -130,6 +130,36 @@ def test_activation_ranges(scale):
     check(2, 100, 512, Q4_1, F32, scale=scale)
 
 
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("head, tail", [(0.0, 1.0), (1e-3, 50.0), (1.0, 3e4), (100.0, 1e-2)])
+def test_rows_whose_first_columns_say_nothing_of_the_rest(dt, head, tail):
+    # the operands' scale is guessed from a row's first 32 values: zeros, far smaller or far larger ones
+    rng = np.random.default_rng(11)
+    b, w, mag = blocks(rng, 100, 1024, Q4_0)
+    x = rng.standard_normal((3, 1024)).astype(np.float32)
+    x[:, :32] *= head
+    x[:, 32:] *= 1e-2
+    x[:, 700] *= tail / 1e-2
+    x[1] = rng.standard_normal(1024)      # a row of the same launch whose guess is right
+    xd = torch.from_numpy(x).to(dt).cuda()
+    y = torch.zeros((3, 100), device="cuda")
+    W = b2q.WeightQ4(b, 100, 1024)
+    b2q.mul_vec_q4(W, xd, 3, y)
+    x64 = xd.double().cpu().numpy()
+    within(y.double().cpu().numpy(), x64 @ w.T, (32 + 32 + 8) * 2.0 ** -23 * (np.abs(x64) @ mag.T)
+           + 2.0 ** -29 * np.abs(x64).max(1, keepdims=True) * mag.sum(1)[None])
+
+
+def test_zero_rows():
+    rng = np.random.default_rng(12)
+    b, _, _ = blocks(rng, 50, 320, Q4_1)
+    W = b2q.WeightQ4(b, 50, 320, Q4_1)
+    for dt in (F32, F16, BF16):
+        y = torch.ones((2, 50), dtype=dt, device="cuda")
+        b2q.mul_vec_q4(W, torch.zeros((2, 320), dtype=dt, device="cuda"), 2, y)
+        assert (y == 0).all()
+
+
 def test_infinite_and_nan_activations_reach_the_result():
     rng = np.random.default_rng(0)
     b, w, _ = blocks(rng, 40, 64, Q4_0)
