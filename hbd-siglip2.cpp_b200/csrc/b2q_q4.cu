@@ -1,7 +1,7 @@
 // b2q_q4.cu — products of few activation rows with ggml Q4_0 / Q4_1 weights
 // (b2q_weight_q4_*, b2q_mul_vec_q4).
 //
-// y[n] = sum_kb d[n,kb] (S[n,kb] - 8 X[kb])   (Q4_1: d S + m X), S the sum of q x
+// y[n] = sum_kb d[n,kb] S[n,kb] (+ m[n,kb] X[kb]), S the sum of (q - 8) x (Q4_1: q x)
 // over the 32 columns of block kb, X that of x.
 //
 // Bound: bytes, 18 (20) per 32 weights and at most once.  At the measured copy
@@ -11,20 +11,20 @@
 // tensor cores: one mma.sync (16 weight rows x 16 columns x 8 activation columns)
 // does 8 of a lane's products and sums in fp32, and almost nothing is unpacked:
 //
-//  * A nibble masked out of its word is an fp16 number as it stands, the
-//    subnormal q 2^-24 (in bits 0-3 of a half) or q 2^-20 (bits 4-7); the factor
-//    between the two is put into the activations.  Five instructions unpack eight
-//    weights: four masks and one shift.  The 8 of Q4_0 is taken off the sums, as 8 X.
-//  * An activation row is scaled by a power of two and becomes fp16 operands: an fp32
-//    value three of 8 bits each, which sum to it, in as many of the eight activation
-//    columns (with one or two rows they are free); a bf16 value one; an fp16 value
-//    one, or two where the result keeps 32 bits.  8 bits and not the 11 that fp16
-//    holds: the tensor core aligns a sum's products to the largest and drops what
-//    falls below some 24 bits, which 12-bit products mostly stay clear of (relative
-//    error of 1 x 1152 x 4320: 2.1e-7; with pieces of 11 bits 5e-7, and 1.1e-6 where
-//    the sums start from -8 X).  The scale loses what lies 2^-30 below the row's
-//    largest value.
-//  * S leaves the tensor core once per block and is summed in fp32, d (S - 8 X).
+//  * A nibble OR-ed into the mantissa of 2^10 is the fp16 number 1024 + q (in bits 0-3
+//    of a half) or 1024 + 16 q (bits 4-7), and one exact addition or multiply-add
+//    makes it q - 8 (Q4_1: q): nine instructions for eight weights.  (Left in place as
+//    fp16 subnormals q 2^-24 and q 2^-20 they take five, and 256000 x 1152 35 us; but the
+//    tensor core aligns a sum's products by the operands' exponents, of which a
+//    subnormal has the largest, and cuts off seven bits: relative errors of 1e-6, and
+//    of 1e-5 beside a large activation.)
+//  * An activation row is scaled by a power of two and becomes fp16 operands: fp16 and
+//    bf16 values one, an fp32 value two, x rounded to 11 bits and the rest rounded to
+//    11 bits, which leaves at most 2^-24 |x|, what a rounding to fp32 may leave; they
+//    take as many of the eight activation columns.  The scale loses what lies 2^-35
+//    below the row's largest value.
+//  * S leaves the tensor core once per block and is summed in fp32, d S.
+// Relative error of 1 x 1152 x 4320 against 64 bits: 9e-8 (plain fp32 products 2e-7).
 //
 // The weights are laid out at registration in the order the lanes want them:
 // per 16 rows a run of units of 128 columns, each 1024 bytes of nibbles (lane l of
@@ -55,7 +55,7 @@ namespace {
 // 0.7 us less (1 x 1152 x 4320: 5.8 against 7.0 us).
 int warps_of(int n_tiles, int64_t units_per_sm) { return n_tiles == 1 && units_per_sm > 64 ? 32 : 16; }
 constexpr int kMaxRows = 32;        // of one launch
-constexpr int kMaxK = 28672;        // three pieces of a row still fit shared memory next to the rings
+constexpr int kMaxK = 28672;        // two pieces of a row still fit shared memory next to the rings
 constexpr int kSmemMax = 227 * 1024 - 1024;   // next to the static part
 
 constexpr int unit_bytes(bool min) { return min ? 1280 : 1152; }
@@ -115,15 +115,25 @@ struct Q4Args {
     bool y_f32;
     const float *bias, *residual;
     int pitch, ring_at, red_at, sum_at;   // shared memory: bytes of an operand column, parts' offsets
+    uint32_t magic = 0x64006400u;         // 2^10 twice.  An argument, so that it stays in a register: with two
+                                          // constants in sight the compiler makes two instructions of (w & a) | b
 };
 
-// The word's four pairs of a lane as fp16 operands: q 2^-24, q 2^-20, q 2^-24, q 2^-20.
-__device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t (&r)[4]) {
-    const uint32_t s = w >> 8;
-    r[0] = w & 0x000F000Fu;
-    r[1] = w & 0x00F000F0u;
-    r[2] = s & 0x000F000Fu;
-    r[3] = s & 0x00F000F0u;
+// The word's four pairs of a lane as fp16 integers q - 8 (Q4_1: q): OR-ed into the
+// mantissa of 2^10 a nibble gives 1024 + q (bits 0-3) or 1024 + 16 q (bits 4-7), and
+// one exact addition or multiply-add takes the rest off.
+template <bool kMin>
+__device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t magic, uint32_t (&r)[4]) {
+    const __half2 off = __float2half2_rn(kMin ? -1024.f : -1032.f);
+    const __half2 off16 = __float2half2_rn(kMin ? -64.f : -72.f), s16 = __float2half2_rn(0.0625f);
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+        const uint32_t s = w >> (4 * j), u = (s & 0x000F000Fu) | magic, v = (s & 0x00F000F0u) | magic;
+        const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&u), off);
+        const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&v), s16, off16);
+        r[j] = *reinterpret_cast<const uint32_t*>(&x);
+        r[j + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    }
 }
 
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
@@ -132,7 +142,7 @@ __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823
 struct RowState {
     uint32_t peak[kMaxRows];   // bits of the largest finite |x|
     int shift[kMaxRows];       // the operands are x 2^shift
-    float back[kMaxRows][2];   // factors that take a row's sums back: 2^(24 - shift), in two
+    float back[kMaxRows][2];   // factors that take a row's sums back: 2^-shift, in two
     uint32_t odd;              // rows that hold an infinity or a NaN (left out of the operands)
 };
 // x 2^top_shift(peak) has its largest value in [2^14, 2^15); peaks below 2^-113 stay smaller.
@@ -174,13 +184,13 @@ struct Eight {
 };
 
 // Activation rows into shared memory: operand column p * rows + m holds piece p
-// of row m.  `sum_at` gets the sums X of each block's scaled values.  Q4_0: what
-// its products start from, -8 X 2^-24 in fp32, four blocks x two rows per unit and
-// pair of rows.  Q4_1: X 2^-5 as operands of the product with m, in three fp16
-// pieces side by side in k, four blocks x 8 bytes per unit and row.
+// of row m, x 2^shift.  Q4_1: `sum_at` gets the sums X of each block's scaled values,
+// times 2^-5, as operands of the product with m: three fp16 pieces side by side in
+// k, four blocks x 8 bytes per unit and row.
+//
 // A warp takes 256 columns of a row at a time.  A row's power of two is a guess
 // from its first 32 values, the largest of them taken to [2^9, 2^10): that leaves
-// the row's largest value a factor of 32, and loses no more than 2^-30 of it.  The
+// the row's largest value a factor of 32, and loses no more than 2^-35 of it.  The
 // same pass takes the peaks; a row that needs more room is staged again with the
 // power that its peak gives (`again`).  Two CTAs of a cluster (`pair`) stage half of
 // the work each and store it in both shared memories.
@@ -190,7 +200,6 @@ __device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState
     const int chunks = a.units * 16, segs = (chunks + 31) / 32;   // of 8 columns; of 32 chunks
     const Tx* px = static_cast<const Tx*>(a.x);
     const bool vec = (a.ldx * sizeof(Tx)) % 16 == 0 && (reinterpret_cast<uintptr_t>(px) & 15) == 0;
-    const int pairs = (a.rows + 1) / 2;
     const uint32_t rank = a.pair ? cluster_rank() : 0, here = smem_u32(smem), state = smem_u32(&st);
     const uint32_t there = a.pair ? in_cta(here, rank ^ 1) : 0, state_there = a.pair ? in_cta(state, rank ^ 1) : 0;
     const int workers = a.pair ? 2 * kWarps : kWarps, worker = warp + (rank ? kWarps : 0);
@@ -245,7 +254,7 @@ __device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState
                 }
             }
         }
-        const float s = pow2(shift), s16 = s * 0.0625f;
+        const float s = pow2(shift);
         float sum = 0.f;
         uint32_t p[kPieces][4];
 #pragma unroll
@@ -255,20 +264,22 @@ __device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState
                 if (!is_finite(x.x)) x.x = 0.f;
                 if (!is_finite(x.y)) x.y = 0.f;
             }
-            sum = fmaf(x.x, s, fmaf(x.y, s, sum));
-            x.x *= j & 1 ? s16 : s;   // where the nibble stands four bits higher
-            x.y *= j & 1 ? s16 : s;
+            x.x *= s;
+            x.y *= s;
+            if constexpr (kMin) sum += x.x + x.y;
 #pragma unroll
-            for (int z = 0; z + 1 < kPieces; ++z) {   // 8 bits, as fp16
-                const float2 h = unpack2<__nv_bfloat16>(pack2<__nv_bfloat16>(x.x, x.y));
-                p[z][j] = pack2<__half>(h.x, h.y);
+            for (int z = 0; z + 1 < kPieces; ++z) {
+                p[z][j] = pack2<__half>(x.x, x.y);
+                const float2 h = unpack2<__half>(p[z][j]);
                 x.x -= h.x;
                 x.y -= h.y;
             }
             p[kPieces - 1][j] = pack2<__half>(x.x, x.y);
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if constexpr (kMin) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        }
         if (c < chunks) {
             const int dst = row * a.pitch + c * 16;
 #pragma unroll
@@ -277,37 +288,23 @@ __device__ __forceinline__ void stage_x(const Q4Args& a, uint8_t* smem, RowState
                 *reinterpret_cast<uint4*>(smem + dst + z * a.rows * a.pitch) = v;
                 if (a.pair) st_cluster_128(there + dst + z * a.rows * a.pitch, v);
             }
-            if ((c & 3) == 0) {
-                const int unit = c >> 4, block = (c >> 2) & 3;
-                if constexpr (kMin) {
-                    __half h[4];
-                    sum *= 0.03125f;
+            if (kMin && (c & 3) == 0) {
+                __half h[4];
+                sum *= 0.03125f;
 #pragma unroll
-                    for (int z = 0; z < 3; ++z) {
-                        h[z] = __float2half_rn(sum);
-                        sum -= __half2float(h[z]);
-                    }
-                    h[3] = __float2half_rn(0.f);
-                    const int at = a.sum_at + ((unit * a.rows + row) * 4 + block) * 8;
-                    *reinterpret_cast<uint2*>(smem + at) = *reinterpret_cast<const uint2*>(h);
-                    if (a.pair) st_cluster_64(there + at, *reinterpret_cast<const uint2*>(h));
-                } else {
-                    const int at = a.sum_at + (((unit * pairs + (row >> 1)) * 4 + block) * 2 + (row & 1)) * 4;
-                    const float v = sum * -4.76837158203125e-7f;
-                    const bool last = row + 1 == a.rows && !(row & 1);   // the pair's other row is none
-                    *reinterpret_cast<float*>(smem + at) = v;
-                    if (last) *reinterpret_cast<float*>(smem + at + 4) = 0.f;
-                    if (a.pair) {
-                        st_cluster_32(there + at, __float_as_uint(v));
-                        if (last) st_cluster_32(there + at + 4, 0u);
-                    }
+                for (int z = 0; z < 3; ++z) {
+                    h[z] = __float2half_rn(sum);
+                    sum -= __half2float(h[z]);
                 }
+                h[3] = __float2half_rn(0.f);
+                const int at = a.sum_at + (((c >> 4) * a.rows + row) * 4 + ((c >> 2) & 3)) * 8;
+                *reinterpret_cast<uint2*>(smem + at) = *reinterpret_cast<const uint2*>(h);
+                if (a.pair) st_cluster_64(there + at, *reinterpret_cast<const uint2*>(h));
             }
         }
     }
     // what columns of other pieces take
-    if (threadIdx.x < 8)
-        reinterpret_cast<float*>(smem + a.sum_at)[a.units * (kMin ? a.rows : pairs) * 8 + threadIdx.x] = 0.f;
+    if (kMin && threadIdx.x < 8) reinterpret_cast<float*>(smem + a.sum_at)[a.units * a.rows * 8 + threadIdx.x] = 0.f;
 }
 
 template <bool kMin, int kWarps>
@@ -322,16 +319,15 @@ __device__ __forceinline__ void stage_rows(const Q4Args& a, uint8_t* smem, RowSt
     meet();
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
-        if (a.x_type == B2Q_TYPE_F32) stage_x<float, 3, kMin, kWarps>(a, smem, st, pass);
+        if (a.x_type == B2Q_TYPE_F32) stage_x<float, 2, kMin, kWarps>(a, smem, st, pass);
         else if (a.x_type == B2Q_TYPE_BF16) stage_x<__nv_bfloat16, 1, kMin, kWarps>(a, smem, st, pass);
-        else if (a.pieces == 1) stage_x<__half, 1, kMin, kWarps>(a, smem, st, pass);
-        else stage_x<__half, 2, kMin, kWarps>(a, smem, st, pass);
+        else stage_x<__half, 1, kMin, kWarps>(a, smem, st, pass);
         meet();   // (peaks and shifts are the same in both CTAs of a pair, and so is what follows)
         const bool mine = pass == 0 && tid < a.rows;
         const bool over = mine && st.shift[tid] > top_shift(st.peak[tid]);
         if (over) st.shift[tid] = top_shift(st.peak[tid]);
         if (mine) {
-            const int e = 24 - st.shift[tid];
+            const int e = -st.shift[tid];
             st.back[tid][0] = pow2(e >> 1);
             st.back[tid][1] = pow2(e - (e >> 1));
         }
@@ -364,7 +360,8 @@ __device__ __noinline__ float odd_terms(const Q4Args& a, int64_t n, int m) {
     return v;
 }
 
-template <bool kMin, int kN, int kStages, int kWarps>
+// kGroup units of a tile are waited for together, where kStages rings of them fit.
+template <bool kMin, int kN, int kGroup, int kStages, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid_constant__ Q4Args a) {
     constexpr int kUnit = unit_bytes(kMin);
     extern __shared__ __align__(128) uint8_t smem[];
@@ -375,29 +372,37 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
     const int per_tile = (a.units - sub + split - 1) / split;   // units of this warp in each of its tiles
 
     // ---- the weights' stream: a unit is asked for as soon as its slot is free ----
-    const int ring = a.ring_at + warp * kStages * kUnit;
-    const uint8_t* src = a.w + (static_cast<int64_t>(first) * a.units + sub) * kUnit + lane * 16;
+    constexpr int kSlot = kGroup * kUnit;
+    const int ring = a.ring_at + warp * kStages * kSlot;
+    const uint8_t* tile_src = a.w + (static_cast<int64_t>(first) * a.units + sub) * kUnit + lane * 16;
+    const uint8_t* src = tile_src;
     const int64_t unit_step = static_cast<int64_t>(split) * kUnit;
-    const int64_t tile_step = (static_cast<int64_t>(step) * a.units - static_cast<int64_t>(per_tile) * split) * kUnit;
-    int left = first < a.tiles ? (a.tiles - first + step - 1) / step * per_tile : 0;   // units still to ask for
-    int left_tile = per_tile;
+    const int64_t tile_step = static_cast<int64_t>(step) * a.units * kUnit;
+    int tiles_left = first < a.tiles ? (a.tiles - first + step - 1) / step : 0;   // tiles still to ask for
+    int left = per_tile;                                                          // units of this one
     auto issue = [&](int slot) {
-        if (left > 0) {
+        if (tiles_left > 0) {
             const uint32_t dst = smem_u32(smem) + slot + lane * 16;
-            cp_async_16(dst, src, true);
-            cp_async_16(dst + 512, src + 512, true);
-            if (lane < (kUnit - 1024) / 16) cp_async_16(dst + 1024, src + 1024, true);
-            --left;
-            src += unit_step;
-            if (--left_tile == 0) {
-                left_tile = per_tile;
-                src += tile_step;
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u)
+                if (u == 0 || left > u) {
+                    cp_async_16(dst + u * kUnit, src, true);
+                    cp_async_16(dst + u * kUnit + 512, src + 512, true);
+                    if (lane < (kUnit - 1024) / 16) cp_async_16(dst + u * kUnit + 1024, src + 1024, true);
+                    src += unit_step;
+                }
+            left -= kGroup;
+            if (left <= 0) {
+                left = per_tile;
+                --tiles_left;
+                tile_src += tile_step;
+                src = tile_src;
             }
         }
         cp_commit();
     };
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) issue(ring + i * kUnit);
+    for (int i = 0; i < kStages; ++i) issue(ring + i * kSlot);
     // the weights are on their way; the activations may be another kernel's results
     let_next_start();
     wait_for_previous();
@@ -405,20 +410,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
 
     // This lane's operand columns.  A column that no row has computes on the
     // first one's values; its results are not read.
-    const int cols = a.rows * a.pieces, pairs = (a.rows + 1) / 2;
-    int x0[kN], sum0[kN], sum_step[kN];   // sums: Q4_0 of columns 2 t, 2 t + 1, Q4_1 of this lane's column, block t
+    const int cols = a.rows * a.pieces;
+    int x0[kN], sum0[kN], sum_step[kN];   // sums (Q4_1): of this lane's column, block t
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-        const int col = n * 8 + g < cols ? n * 8 + g : 0, pair = n * 4 + t;
+        const int col = n * 8 + g < cols ? n * 8 + g : 0;
+        const bool own = n * 8 + g < a.rows;   // X goes with a row's first piece
         x0[n] = col * a.pitch + t * 16 + sub * 256;
-        if constexpr (kMin) {
-            const bool own = n * 8 + g < a.rows;
-            sum_step[n] = own ? a.rows * 32 : 0;
-            sum0[n] = a.sum_at + (own ? (sub * a.rows + col) * 32 : a.units * a.rows * 32) + t * 8;
-        } else {
-            sum_step[n] = pair < pairs ? pairs * 32 : 0;
-            sum0[n] = a.sum_at + (pair < pairs ? (sub * pairs + pair) * 32 : a.units * pairs * 32);
-        }
+        sum_step[n] = own ? a.rows * 32 : 0;
+        sum0[n] = a.sum_at + (own ? (sub * a.rows + col) * 32 : a.units * a.rows * 32) + t * 8;
     }
     int slot = ring, buf = 0;
     for (int tile = first; tile < a.tiles; tile += step, buf ^= 1) {
@@ -426,61 +426,55 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
         int xo = 0, so[kN];
 #pragma unroll
         for (int n = 0; n < kN; ++n) so[n] = sum0[n];
-        for (int j = 0; j < per_tile; ++j, xo += split * 256) {
+        for (int j = 0; j < per_tile; j += kGroup) {
             cp_wait<kStages - 1>();
-            __syncwarp();   // every lane's part of the unit has come
-            const uint8_t* use = smem + slot;
-            const uint4 wa = *reinterpret_cast<const uint4*>(use + lane * 16);
-            const uint4 wb = *reinterpret_cast<const uint4*>(use + 512 + lane * 16);
-            const uint4 dd = *reinterpret_cast<const uint4*>(use + 1024 + g * 16);
-            uint32_t mm = 0;
-            if constexpr (kMin) mm = *reinterpret_cast<const uint32_t*>(use + 1152 + g * 16 + t * 4);
-            __syncwarp();   // all lanes have their words: the slot may be filled again
-            issue(slot);
-            slot += kUnit;
-            if (slot == ring + kStages * kUnit) slot = ring;
-            const uint32_t w8[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
-            const uint32_t d4[4] = {dd.x, dd.y, dd.z, dd.w};
-            if constexpr (kMin) {   // block t's m three times in k, against the pieces of its X
-                const uint32_t m0 = __byte_perm(mm, 0, 0x1010), m8 = __byte_perm(mm, 0, 0x3232);
+            __syncwarp();   // every lane's part of the units has come
 #pragma unroll
-                for (int n = 0; n < kN; ++n) {
-                    const uint2 xp = *reinterpret_cast<const uint2*>(smem + so[n]);
-                    float v[4];
-                    mma_16816_from0(v, m0, m8, m0, m8, xp.x, xp.y);
-                    // X was scaled by 2^-5, the nibbles by 2^-24
+            for (int u = 0; u < kGroup; ++u) {
+                if (u && j + u >= per_tile) break;
+                const uint8_t* use = smem + slot + u * kUnit;
+                const uint4 wa = *reinterpret_cast<const uint4*>(use + lane * 16);
+                const uint4 wb = *reinterpret_cast<const uint4*>(use + 512 + lane * 16);
+                const uint4 dd = *reinterpret_cast<const uint4*>(use + 1024 + g * 16);
+                const uint32_t w8[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+                const uint32_t d4[4] = {dd.x, dd.y, dd.z, dd.w};
+                if constexpr (kMin) {   // block t's m three times in k, against the pieces of its X
+                    const uint32_t mm = *reinterpret_cast<const uint32_t*>(use + 1152 + g * 16 + t * 4);
+                    const uint32_t m0 = __byte_perm(mm, 0, 0x1010), m8 = __byte_perm(mm, 0, 0x3232);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(v[e], 1.9073486328125e-6f, acc[n][e]);
-                }
-            }
+                    for (int n = 0; n < kN; ++n) {
+                        const uint2 xp = *reinterpret_cast<const uint2*>(smem + so[n]);
+                        float v[4];
+                        mma_16816_from0(v, m0, m8, m0, m8, xp.x, xp.y);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                uint32_t lo[4], hi[4];
-                unpack_q4(w8[2 * b], lo);
-                unpack_q4(w8[2 * b + 1], hi);
-                const float2 d = unpack2<__half>(d4[b]);
-#pragma unroll
-                for (int n = 0; n < kN; ++n) {
-                    const uint4 xv = *reinterpret_cast<const uint4*>(smem + x0[n] + xo + b * 64);
-                    float2 x = make_float2(0.f, 0.f);
-                    if constexpr (!kMin) x = *reinterpret_cast<const float2*>(smem + so[n] + b * 8);
-                    float s[4];
-                    mma_16816_from0(s, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
-                    mma_16816<__half>(s, lo[2], hi[2], lo[3], hi[3], xv.z, xv.w);
-                    if constexpr (!kMin) {
-                        s[0] += x.x;
-                        s[1] += x.y;
-                        s[2] += x.x;
-                        s[3] += x.y;
+                        for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(v[e], 32.f, acc[n][e]);   // (X was scaled by 2^-5)
+                        so[n] += split * sum_step[n];
                     }
-                    acc[n][0] = fmaf(d.x, s[0], acc[n][0]);
-                    acc[n][1] = fmaf(d.x, s[1], acc[n][1]);
-                    acc[n][2] = fmaf(d.y, s[2], acc[n][2]);
-                    acc[n][3] = fmaf(d.y, s[3], acc[n][3]);
                 }
-            }
 #pragma unroll
-            for (int n = 0; n < kN; ++n) so[n] += split * sum_step[n];
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t lo[4], hi[4];
+                    unpack_q4<kMin>(w8[2 * b], a.magic, lo);
+                    unpack_q4<kMin>(w8[2 * b + 1], a.magic, hi);
+                    const float2 d = unpack2<__half>(d4[b]);
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) {
+                        const uint4 xv = *reinterpret_cast<const uint4*>(smem + x0[n] + xo + b * 64);
+                        float s[4];
+                        mma_16816_from0(s, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
+                        mma_16816<__half>(s, lo[2], hi[2], lo[3], hi[3], xv.z, xv.w);
+                        acc[n][0] = fmaf(d.x, s[0], acc[n][0]);
+                        acc[n][1] = fmaf(d.x, s[1], acc[n][1]);
+                        acc[n][2] = fmaf(d.y, s[2], acc[n][2]);
+                        acc[n][3] = fmaf(d.y, s[3], acc[n][3]);
+                    }
+                }
+                xo += split * 256;
+            }
+            __syncwarp();   // the slot may be filled again
+            issue(slot);
+            slot += kSlot;
+            if (slot == ring + kStages * kSlot) slot = ring;
         }
         // ---- add up the tile's warps and the pieces, in order; two buffers, so that
         // one meeting a tile suffices ----
@@ -504,7 +498,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
             if (in) {
                 const float* p = all + part * part_floats + row * pitch + m;
                 for (int w = part; w < split; w += 1 << a.part_log2, p += part_floats << a.part_log2)
-                    v += a.pieces == 1 ? p[0] : a.pieces == 2 ? p[0] + p[a.rows] : p[0] + (p[a.rows] + p[2 * a.rows]);
+                    v += a.pieces == 1 ? p[0] : p[0] + p[a.rows];
             }
             for (int x = 1 << a.part_log2 >> 1; x; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
             if (!in || part || n >= a.N) continue;
@@ -547,7 +541,7 @@ int part_log2_of(int split, int rows) {
 }
 
 struct Q4Plan {
-    int stages, pitch, ring_at, red_at, sum_at, bytes;
+    int group, stages, pitch, ring_at, red_at, sum_at, bytes;
 };
 // Shared memory of a launch over `rows` activation rows, with as deep a ring as
 // it holds; stages 0 where it does not fit.
@@ -556,12 +550,14 @@ Q4Plan plan_of(int rows, int pieces, int warps, int units, bool min) {
     p.pitch = units * 256 + 64;   // 64 bytes off a multiple of 128: eight columns' chunks miss one another's banks
     p.red_at = static_cast<int>(round_up(rows * pieces * p.pitch, 128));
     p.sum_at = p.red_at + static_cast<int>(round_up(2 * warps * 16 * red_pitch(rows * pieces) * 4, 128));
-    const int sums = (units * (min ? rows : (rows + 1) / 2) + 1) * 32;
-    p.ring_at = p.sum_at + static_cast<int>(round_up(sums, 128));
-    for (int stages : {4, 2, 1}) {
-        p.bytes = p.ring_at + warps * unit_bytes(min) * stages;
+    p.ring_at = p.sum_at + (min ? static_cast<int>(round_up((units * rows + 1) * 32, 128)) : 0);
+    constexpr int kRings[][2] = {{2, 3}, {2, 2}, {1, 2}, {1, 1}};   // units of a group, stages; the last for long rows only
+    for (const auto& r : kRings) {
+        if (warps == 32 && r[1] == 3) continue;   // (32 warps fill shared memory with two)
+        p.bytes = p.ring_at + warps * unit_bytes(min) * r[0] * r[1];
         if (p.bytes <= kSmemMax) {
-            p.stages = stages;
+            p.group = r[0];
+            p.stages = r[1];
             break;
         }
     }
@@ -660,7 +656,7 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool min = w->type == B2Q_TYPE_Q4_1;
     const int units = static_cast<int>(w->units);
-    const int pieces = x_dtype == B2Q_TYPE_F32 ? 3 : x_dtype == B2Q_TYPE_F16 && y_dtype == B2Q_TYPE_F32 ? 2 : 1;
+    const int pieces = x_dtype == B2Q_TYPE_F32 ? 2 : 1;
     const size_t es = x_dtype == B2Q_TYPE_F32 ? 4 : 2, ys = y_dtype == B2Q_TYPE_F32 ? 4 : 2;
     const int64_t per_sm = (w->tiles + ds->num_sms - 1) / ds->num_sms * units;
     auto plan_rows = [&](int rows) {
@@ -687,19 +683,24 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
                        static_cast<const uint8_t*>(x) + m0 * ldx * es, x_dtype, pieces, rows, x_cols, ldx,
                        static_cast<uint8_t*>(y) + m0 * ldy * ys, ldy, y_dtype == B2Q_TYPE_F32, bias,
                        residual ? residual + m0 * ldy : nullptr, p.pitch, p.ring_at, p.red_at, p.sum_at};
-        auto go = [&](auto mn, auto nt, auto stages, auto wp) {
-            auto* kernel = mul_vec_q4_kernel<decltype(mn)::value, decltype(nt)::value, decltype(stages)::value,
-                                             decltype(wp)::value>;
+        auto go = [&](auto mn, auto nt, auto group, auto stages, auto wp) {
+            auto* kernel = mul_vec_q4_kernel<decltype(mn)::value, decltype(nt)::value, decltype(group)::value,
+                                             decltype(stages)::value, decltype(wp)::value>;
             static std::atomic<uint64_t> allowed{0};
             const b2q_status st = allow_smem(kernel, kSmemMax, allowed, ds->device);
             if (st) return st;
             return cuda_check(launch_after(pair ? 2 : 1, kernel, dim3(grid), dim3(warps * 32), p.bytes, s, a),
                               "4-bit product launch");
         };
+        constexpr std::integral_constant<int, 1> one{};
+        constexpr std::integral_constant<int, 2> two{};
         auto with_stages = [&](auto mn, auto nt, auto wp) {
-            return p.stages == 4   ? go(mn, nt, std::integral_constant<int, 4>{}, wp)
-                   : p.stages == 2 ? go(mn, nt, std::integral_constant<int, 2>{}, wp)
-                                   : go(mn, nt, std::integral_constant<int, 1>{}, wp);
+            if (p.group == 2 && p.stages == 3) {
+                if constexpr (decltype(wp)::value == 16) return go(mn, nt, two, std::integral_constant<int, 3>{}, wp);
+            }
+            return p.group == 2    ? go(mn, nt, two, two, wp)
+                   : p.stages == 2 ? go(mn, nt, one, two, wp)
+                                   : go(mn, nt, one, one, wp);
         };
         constexpr std::integral_constant<int, 16> w16{};
         constexpr std::integral_constant<int, 32> w32{};

@@ -402,7 +402,7 @@ b2q_status b2q_weight_q4_release(b2q_weight_q4 *w);
  * residual (fp32, may be y) have row stride ldy; bias and residual may be
  * NULL; y overlaps neither x nor bias.  The activations are not quantized:
  * products and sums are in fp32, rounded once.  Meant for few rows: a launch
- * takes up to 32 fp16 or bf16 rows or ten fp32 ones, fewer where their columns
+ * takes up to 32 fp16 or bf16 rows or 16 fp32 ones, fewer where their columns
  * do not fit shared memory, and reads the weights once. */
 b2q_status b2q_mul_vec_q4(const b2q_weight_q4 *w, const void *x, int32_t x_dtype, int64_t M, int64_t x_cols,
                           int64_t ldx, void *y, int32_t y_dtype, int64_t ldy, const float *bias,
