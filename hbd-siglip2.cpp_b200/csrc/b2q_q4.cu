@@ -476,32 +476,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
             slot += kSlot;
             if (slot == ring + kStages * kSlot) slot = ring;
         }
-        // ---- add up the tile's warps and the pieces, in order; two buffers, so that
-        // one meeting a tile suffices ----
-        const int pitch = red_pitch(cols), part_floats = 16 * pitch;
-        float* all = reinterpret_cast<float*>(smem + a.red_at) + (buf * kWarps + group * split) * part_floats;
-        float* red = all + sub * part_floats + g * pitch + 2 * t;
-#pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (n * 8 + 2 * t + (e & 1) < cols) red[8 * (e >> 1) * pitch + n * 8 + (e & 1)] = acc[n][e];
-            }
-        if (split == 1) __syncwarp();
-        else asm volatile("bar.sync %0, %1;" ::"r"(group), "r"(split * 32) : "memory");
-        // 2^part_log2 neighbouring lanes take an output, each some of its warps' parts
-        const int me = tid - group * split * 32, part = me & ((1 << a.part_log2) - 1);
-        for (int base = 0; base < 16 * a.rows; base += split * 32 >> a.part_log2) {
-            const int o = base + (me >> a.part_log2), row = o & 15, m = o >> 4, n = tile * 16 + row;
-            const bool in = m < a.rows;
-            float v = 0.f;
-            if (in) {
-                const float* p = all + part * part_floats + row * pitch + m;
-                for (int w = part; w < split; w += 1 << a.part_log2, p += part_floats << a.part_log2)
-                    v += a.pieces == 1 ? p[0] : p[0] + p[a.rows];
-            }
-            for (int x = 1 << a.part_log2 >> 1; x; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
-            if (!in || part || n >= a.N) continue;
+        auto put = [&](int m, int n, float v) {
+            if (n >= a.N) return;
             v = v * st.back[m][0] * st.back[m][1];
             if ((st.odd >> m) & 1) v += odd_terms<kMin>(a, n, m);
             const int64_t at = m * a.ldy + n;
@@ -510,6 +486,39 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
             if (a.y_f32) static_cast<float*>(a.y)[at] = v;
             else if (a.x_type == B2Q_TYPE_F16) static_cast<__half*>(a.y)[at] = from_f32<__half>(v);
             else static_cast<__nv_bfloat16*>(a.y)[at] = from_f32<__nv_bfloat16>(v);
+        };
+        if (split == 1 && a.rows == 1) {   // a lane has all of an output: its row's pieces, columns 0 and 1
+            if (t == 0) {
+                put(0, tile * 16 + g, a.pieces == 1 ? acc[0][0] : acc[0][0] + acc[0][1]);
+                put(0, tile * 16 + g + 8, a.pieces == 1 ? acc[0][2] : acc[0][2] + acc[0][3]);
+            }
+            continue;
+        }
+        // ---- add up the tile's warps and the pieces, in order; two buffers, so that
+        // one meeting a tile suffices ----
+        const int pitch = red_pitch(cols), part_floats = 16 * pitch;
+        float* all = reinterpret_cast<float*>(smem + a.red_at) + (buf * kWarps + group * split) * part_floats;
+        float* red = all + sub * part_floats + g * pitch + 2 * t;
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n * 8 + 2 * t + (e & 1) < cols) red[8 * (e >> 1) * pitch + n * 8 + (e & 1)] = acc[n][e];
+        if (split == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(group), "r"(split * 32) : "memory");
+        // 2^part_log2 neighbouring lanes take an output, each some of its warps' parts
+        const int me = tid - group * split * 32, part = me & ((1 << a.part_log2) - 1);
+        for (int base = 0; base < 16 * a.rows; base += split * 32 >> a.part_log2) {
+            const int o = base + (me >> a.part_log2), row = o & 15, m = o >> 4;
+            const bool in = m < a.rows;
+            float v = 0.f;
+            if (in) {
+                const float* p = all + part * part_floats + row * pitch + m;
+                for (int w = part; w < split; w += 1 << a.part_log2, p += part_floats << a.part_log2)
+                    v += a.pieces == 1 ? p[0] : p[0] + p[a.rows];
+            }
+            for (int x = 1 << a.part_log2 >> 1; x; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+            if (in && !part) put(m, tile * 16 + row, v);
         }
     }
 }
