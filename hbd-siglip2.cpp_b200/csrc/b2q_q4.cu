@@ -50,10 +50,6 @@ struct b2q_weight_q4 {
 namespace b2q {
 namespace {
 
-// Warps of a CTA (one per SM): 32 where 64 registers suffice (one operand tile) and
-// an SM has more than four units for each of 16 warps; else 16, whose start takes
-// 0.7 us less (1 x 1152 x 4320: 5.8 against 7.0 us).
-int warps_of(int n_tiles, int64_t units_per_sm) { return n_tiles == 1 && units_per_sm > 64 ? 32 : 16; }
 constexpr int kMaxRows = 32;        // of one launch
 constexpr int kMaxK = 28672;        // two pieces of a row still fit shared memory next to the rings
 constexpr int kSmemMax = 227 * 1024 - 1024;   // next to the static part
@@ -524,22 +520,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mul_vec_q4_kernel(const __grid
 }
 
 // ------------------------------------------------------------------ launch
-// Warps per row tile: the split whose warps on the fullest SM have the least to
-// do, in half units: two a unit that they stream, and per tile three for its end,
-// four where warps meet there.
-int split_of(int64_t tiles, int units, int sms, int warps) {
-    int best = 1;
-    int64_t best_cost = INT64_MAX;
-    const int64_t per_sm = (tiles + sms - 1) / sms;
-    for (int s = 1; s <= warps && s <= units; s *= 2) {
-        const int64_t rounds = (per_sm * s + warps - 1) / warps;
-        const int64_t cost = rounds * (2 * ((units + s - 1) / s) + (s > 1 ? 4 : 3));
-        if (cost < best_cost) {
-            best = s;
-            best_cost = cost;
-        }
-    }
-    return best;
+// What the fullest SM has to do, in half units of all its warps: two a unit that a
+// warp streams, and per tile three for its end, four where `split` warps meet there.
+int64_t cost_of(int64_t tiles, int units, int sms, int warps, int split) {
+    const int64_t rounds = ((tiles + sms - 1) / sms * split + warps - 1) / warps;
+    return rounds * (2 * ((units + split - 1) / split) + (split > 1 ? 4 : 3)) * warps;
 }
 // log2 of the lanes that share an output at a tile's end: all warps' parts side by
 // side where the outputs leave that many lanes.
@@ -562,7 +547,7 @@ Q4Plan plan_of(int rows, int pieces, int warps, int units, bool min) {
     p.ring_at = p.sum_at + (min ? static_cast<int>(round_up((units * rows + 1) * 32, 128)) : 0);
     constexpr int kRings[][2] = {{2, 3}, {2, 2}, {1, 2}, {1, 1}};   // units of a group, stages; the last for long rows only
     for (const auto& r : kRings) {
-        if (warps == 32 && r[1] == 3) continue;   // (32 warps fill shared memory with two)
+        if (warps > 16 && r[1] == 3) continue;   // (as many warps fill shared memory with two)
         p.bytes = p.ring_at + warps * unit_bytes(min) * r[0] * r[1];
         if (p.bytes <= kSmemMax) {
             p.group = r[0];
@@ -576,6 +561,35 @@ Q4Plan plan_of(int rows, int pieces, int warps, int units, bool min) {
 int n_tiles_of(int rows, int pieces) {
     const int n = rows <= kMaxRows ? (rows * pieces + 7) / 8 : 5;
     return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 0;
+}
+// The warps of a CTA (one per SM), the split and the shared memory of a launch.  One
+// operand tile leaves the registers for 24 or 32 warps, and what suits the number
+// of tiles costs least: 256000 x 1152 takes 37.8 us with 32 warps and 35.8 with 24,
+// 7 x 28672 x 8192 33.9 and 35.2.  16 warps start 0.7 us sooner: where an SM has no
+// more than four units for each (1 x 1152 x 4320: 4.4 against 5.1 us), and where two
+// or four operand tiles need the registers.
+struct Choice {
+    int n_tiles, warps, split;
+    Q4Plan plan;
+};
+Choice choose(int rows, int pieces, int64_t tiles, int units, int sms, bool min) {
+    Choice best{};
+    const int n = n_tiles_of(rows, pieces);
+    if (!n) return best;
+    const bool few = n > 1 || (tiles + sms - 1) / sms * units <= 64;
+    int64_t best_cost = INT64_MAX;
+    for (int warps : {16, 24, 32}) {
+        if ((warps == 16) != few) continue;
+        const Q4Plan p = plan_of(rows, pieces, warps, units, min);
+        if (!p.stages || p.stages < best.plan.stages) continue;
+        for (int split = 1; warps % split == 0 && split <= units; split *= 2) {
+            const int64_t cost = cost_of(tiles, units, sms, warps, split);
+            if (cost >= best_cost && p.stages == best.plan.stages) continue;
+            best = Choice{n, warps, split, p};
+            best_cost = cost;
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -667,23 +681,19 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
     const int units = static_cast<int>(w->units);
     const int pieces = x_dtype == B2Q_TYPE_F32 ? 2 : 1;
     const size_t es = x_dtype == B2Q_TYPE_F32 ? 4 : 2, ys = y_dtype == B2Q_TYPE_F32 ? 4 : 2;
-    const int64_t per_sm = (w->tiles + ds->num_sms - 1) / ds->num_sms * units;
-    auto plan_rows = [&](int rows) {
-        const int n = n_tiles_of(rows, pieces);
-        return n ? plan_of(rows, pieces, warps_of(n, per_sm), units, min) : Q4Plan{};
-    };
+    auto choice = [&](int rows) { return choose(rows, pieces, w->tiles, units, ds->num_sms, min); };
     // the most rows that a launch takes (operand tiles and shared memory), then as even launches as that allows
     int most = 1;
-    while (most < M && plan_rows(most + 1).stages >= 2) ++most;
+    while (most < M && choice(most + 1).plan.stages >= 2) ++most;
     const int64_t launches = (M + most - 1) / most;
     for (int64_t i = 0, m0 = 0; i < launches; ++i) {
         const int rows = static_cast<int>((M - m0 + launches - i - 1) / (launches - i));
-        const int n_tiles = n_tiles_of(rows, pieces), warps = warps_of(n_tiles, per_sm);
-        const Q4Plan p = plan_rows(rows);
+        const Choice c = choice(rows);
+        const Q4Plan& p = c.plan;
+        const int n_tiles = c.n_tiles, warps = c.warps, split = c.split;
         if (!p.stages) return set_error(B2Q_ERR_SHAPE, "an activation row does not fit shared memory");
-        const int split = split_of(w->tiles, units, ds->num_sms, warps);
         // Pairs where each warp would stage more than two pieces of 256 columns by itself
-        // (7 rows of 8,192: 33.7 -> PAIRED us); an SM may stay idle where their number is odd.
+        // (7 x 32 x 8192: 11.1 -> 8.4 us); an SM may stay idle where their number is odd.
         const bool pair = rows * ((units + 1) / 2) > 2 * warps && w->tiles > 1 && ds->num_sms >= 2;
         unsigned grid = static_cast<unsigned>(w->tiles < ds->num_sms ? w->tiles : ds->num_sms);
         if (pair) grid = grid / 2 * 2;
@@ -712,10 +722,12 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
                                    : go(mn, nt, one, one, wp);
         };
         constexpr std::integral_constant<int, 16> w16{};
+        constexpr std::integral_constant<int, 24> w24{};
         constexpr std::integral_constant<int, 32> w32{};
         auto with_tiles = [&](auto mn) {
-            return n_tiles == 1   ? (warps == 32 ? with_stages(mn, std::integral_constant<int, 1>{}, w32)
-                                                 : with_stages(mn, std::integral_constant<int, 1>{}, w16))
+            return n_tiles == 1   ? (warps == 32   ? with_stages(mn, one, w32)
+                                     : warps == 24 ? with_stages(mn, one, w24)
+                                                   : with_stages(mn, one, w16))
                    : n_tiles == 2 ? with_stages(mn, std::integral_constant<int, 2>{}, w16)
                                   : with_stages(mn, std::integral_constant<int, 4>{}, w16);
         };
