@@ -38,6 +38,13 @@
 // one would.  The tensor core cuts its sums off rather than rounding them, so a tile's
 // products are summed from zero there and added to the output in fp32: a chain over
 // thousands of keys would shrink it (131,071 keys: relative error 4.0e-6 against 1.1e-6).
+//
+// Measured on one B200 (copy bandwidth 6.53 TB/s), device time: 3 requests of 131,071
+// keys, 40/8 heads of 128, fp16, 1.61 GB: 267 to 277 us, 5.8 to 6.0 TB/s; 61 ragged ones
+// of 17 to 8,191, 32/8 heads of 128, bf16, 0.99 GB: 170 us, 5.8 TB/s; 256 rows with a
+// window of 1,024, 8/1 heads of 256, 264 MB: 66 to 70 us, 3.9 TB/s, the start and the
+// joins being exposed with one CTA an SM; one request of 997 keys, 16 heads of 72: 9.5 us,
+// round trips one after the other.
 #include "b2q_decode.cuh"
 
 #include <cmath>

@@ -32,8 +32,13 @@
 // m).  A warp streams units through its own ring of asynchronous copies, which runs
 // on across row tiles (with one bulk copy and a barrier per unit the stream took 64
 // of 176 instructions a unit); the activations sit in shared memory for the whole
-// launch (a fixed grid of one CTA of 16 or 32 warps per SM).  `split` warps share a row
+// launch (a fixed grid of one CTA of 16, 24 or 32 warps per SM).  `split` warps share a row
 // tile, each taking every split-th unit, and add up in a fixed order.
+//
+// Measured on one B200 (copy bandwidth 6.53 TB/s), device time: 1 x 256000 x 1152, Q4_1,
+// fp32, 185 MB: 36.4 us, 5.1 TB/s, issue slots 69% busy; 7 x 28672 x 8192, bf16, 133 MB:
+// 34.3 us, 3.9 TB/s, of which 7 until the rows are staged; 1 x 28672 x 8192: 29.6 us; 1 x
+// 4096 x 4096: 4.6 us; 1 x 1152 x 4320, fp32: 4.4 us, the launch and one trip to memory.
 #include "b2q_decode.cuh"
 
 #include <cstddef>
