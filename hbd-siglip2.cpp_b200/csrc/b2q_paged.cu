@@ -10,7 +10,7 @@
 // Bound: bytes.  Every key costs 4 d bytes of cache and 4 d operations per query
 // head of its group, so even 16 heads on one key are 16 operations a byte.
 //
-// Work split.  A unit is 64 keys (a tile) of one (row, key head, block of query
+// Work split.  A unit is a tile of 64 to 128 keys (16 a warp) of one (row, key head, block of query
 // rows).  The units of all rows in order are dealt to a fixed grid of CTAs in
 // equal contiguous shares, whatever the lengths: one request of 100,000 keys
 // and hundreds of ragged ones load every SM alike, lengths are read on the
@@ -20,7 +20,7 @@
 // two partial groups, and the last to report a group joins the parts in their order
 // (so the bits repeat).  Nobody waits.
 //
-// Inside a CTA each of four warps takes 16 keys of every tile and keeps its own
+// Inside a CTA each of four to eight warps takes 16 keys of every tile and keeps its own
 // ref, sum and output; they meet only where a group ends, each leaving its output
 // in the ring slot that it has just read.  Keys and values come by 16-byte
 // asynchronous copies, each warp filling its own ring of stages, so loads run on
@@ -40,11 +40,11 @@
 // thousands of keys would shrink it (131,071 keys: relative error 4.0e-6 against 1.1e-6).
 //
 // Measured on one B200 (copy bandwidth 6.53 TB/s), device time: 3 requests of 131,071
-// keys, 40/8 heads of 128, fp16, 1.61 GB: 267 to 277 us, 5.8 to 6.0 TB/s; 61 ragged ones
-// of 17 to 8,191, 32/8 heads of 128, bf16, 0.99 GB: 170 us, 5.8 TB/s; 256 rows with a
-// window of 1,024, 8/1 heads of 256, 264 MB: 66 to 70 us, 3.9 TB/s, the start and the
-// joins being exposed with one CTA an SM; one request of 997 keys, 16 heads of 72: 9.5 us,
-// round trips one after the other.
+// keys, 40/8 heads of 128, fp16, 1.61 GB: 268 us, 6.0 TB/s; 61 ragged ones of 17 to 8,191,
+// 32/8 heads of 128, bf16, 0.99 GB: 166 us, 6.0 TB/s; 256 rows with a window of 1,024, 8/1
+// heads of 256, 264 MB: 62 us, 4.3 TB/s (with four warps and three stages 70, as one warp a
+// scheduler waits for its own products); one request of 997 keys, 16 heads of 72: 9.5 us,
+// round trips one after the other.  Two stages or three a warp: 268 and 275, 166 and 169 us.
 #include "b2q_decode.cuh"
 
 #include <cmath>
@@ -53,20 +53,21 @@
 namespace b2q {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kTile = 16 * kWarps;     // keys of a unit
 constexpr int kMaxCtas = 444;          // three per SM of a full GPU (148)
 constexpr size_t kCounterBytes = 2048;   // a join counter per CTA, at the start of the scratch
 
-// Per head width (padded to DP): stages of the ring and CTAs per SM, as many as
-// the 227 KB of shared memory hold.
+// Per head width (padded to DP): warps of a CTA and CTAs per SM.  Two stages a warp are
+// enough bytes in flight; what the 227 KB of shared memory and the registers hold beyond
+// that goes to more warps.
 template <int DP>
 struct Shape {
     static constexpr int kChunks = (DP / 8) | 1;            // 16-byte chunks of a shared row
     static constexpr int kPitch = kChunks * 16;
     static constexpr int kStageBytes = 2 * 16 * kPitch;     // one warp's keys and values
-    static constexpr int kStages = 3;
+    static constexpr int kStages = 2;
+    static constexpr int kWarps = DP > 192 ? 6 : (DP > 128 ? 8 : 4);
+    static constexpr int kThreads = kWarps * 32;
+    static constexpr int kTile = 16 * kWarps;               // keys of a unit
     static constexpr int kCtas = DP > 128 ? 1 : (DP > 64 ? 2 : 3);
     static constexpr int kLanes = DP <= 64 ? 8 : (DP <= 128 ? 16 : 32);   // lanes that copy one row
     static constexpr int kOutPitch = DP + 8;
@@ -75,8 +76,8 @@ struct Shape {
 // The ring, which at the end also holds a join's weights, sums and half-way outputs.
 template <int DP, int kRows>
 constexpr int smem_bytes() {
-    constexpr int ring = kWarps * Shape<DP>::kStages * Shape<DP>::kStageBytes;
-    constexpr int join = 2 * kRows * (kMaxCtas + 2) * 4 + kThreads * 16;
+    constexpr int ring = Shape<DP>::kWarps * Shape<DP>::kStages * Shape<DP>::kStageBytes;
+    constexpr int join = 2 * kRows * (kMaxCtas + 2) * 4 + Shape<DP>::kThreads * 16;
     return ring > join ? ring : join;
 }
 // floats of one partial result: output rows, then refs and sums
@@ -105,7 +106,7 @@ struct PagedArgs {
 struct Span {
     int seq, first, len, t0, nt;
 };
-template <class T>
+template <int kTile, class T>
 __device__ __forceinline__ Span span_of(const PagedArgs<T>& a, int r) {
     Span s;
     s.len = a.kv_len[r];
@@ -131,14 +132,14 @@ struct Cursor {
     int r, hm, t;
     Span s;
 };
-template <class T>
+template <int kTile, class T>
 __device__ __forceinline__ void next_unit(const PagedArgs<T>& a, Cursor& c, int per_row) {
     if (++c.t < c.s.nt) return;
     c.t = 0;
     if (++c.hm < per_row) return;
     c.hm = 0;
     c.s.nt = 0;
-    while (c.s.nt == 0 && ++c.r < a.n_rows) c.s = span_of(a, c.r);
+    while (c.s.nt == 0 && ++c.r < a.n_rows) c.s = span_of<kTile>(a, c.r);
 }
 
 // x / y for y that fits an int: 32-bit wherever x does too (64-bit division is some
@@ -180,10 +181,10 @@ __device__ __forceinline__ uint32_t add_acq_rel(uint32_t* p, uint32_t v) {
     return old;
 }
 
+// v f, f = 1 / l, for a sum of l; no key: zeros
 template <class To, class T>
-__device__ __forceinline__ void write_out(const PagedArgs<T>& a, int r, int head, int c, float4 v, float l) {
+__device__ __forceinline__ void write_out(const PagedArgs<T>& a, int r, int head, int c, float4 v, float l, float f) {
     if (c >= a.d) return;   // d is a multiple of 8
-    const float f = l == 0.f ? 0.f : 1.0f / l;
     To* o = static_cast<To*>(a.out) + r * a.ldo + static_cast<int64_t>(head) * a.d + c;
     v = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
     o[0] = from_f32<To>(v.x);
@@ -199,8 +200,9 @@ __device__ __forceinline__ void write_lse(const PagedArgs<T>& a, int r, int head
 }
 
 template <class T, class To, int DP, int kRows>
-__global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(PagedArgs<T> a) {
+__global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_kernel(PagedArgs<T> a) {
     using S = Shape<DP>;
+    constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kTile = S::kTile;
     constexpr int kSteps = DP / 16;           // of 16 elements in q.k
     constexpr int kCols = DP / 8;             // 8-wide column tiles of the output
     constexpr bool kPacked = kRows == 8;      // head and remainder share one operand
@@ -240,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
     Span mine_span{};
     long long mine = 0;
     for (int r = r0; r < r1; ++r) {
-        mine_span = span_of(a, r);
+        mine_span = span_of<kTile>(a, r);
         mine += mine_span.nt;
     }
     long long incl = mine;
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
     base *= per_row;
     if (works && u0 >= base && u0 < base + mine * per_row) {   // exactly one thread
         for (int r = r0; r < r1; ++r) {
-            if (per > 1) mine_span = span_of(a, r);
+            if (per > 1) mine_span = span_of<kTile>(a, r);
             const long long n = static_cast<long long>(mine_span.nt) * per_row;
             if (u0 < base + n) {
                 s_start = Start{r, u0 - base, mine_span};
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
                 if (mine) p.page = a.table[ld.s.seq * a.bt_stride + (key >> a.c.page_shift)];
                 const int head = a.row_blocks == 1 ? ld.hm : ld.hm / a.row_blocks;
                 p.rest = head * a.c.head_stride + (key & a.c.page_mask) * a.c.token_stride;
-                next_unit(a, ld, per_row);
+                next_unit<kTile>(a, ld, per_row);
             }
             return p;
         };
@@ -379,38 +381,43 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
 #pragma unroll
                 for (int x = 0; x < 2 * kHalves; ++x) o[n][x] = 0.f;
         };
-        Pending first[S::kStages];
-#pragma unroll
-        for (int i = 0; i < S::kStages; ++i) first[i] = look_up();
-        new_group();   // (queries asked for before the keys fill the queues)
-#pragma unroll
-        for (int i = 0; i < S::kStages - 1; ++i) issue(first[i], i);
-        Pending next = first[S::kStages - 1];
+        Pending next = look_up();
+        bool fresh = true;
+        int stage = 1;   // of tile i; tile i + kStages - 1 goes to the one before it
 
-        bool fresh = false;
-        int stage = 0;
-
-        for (int i = 0; i < n_units; ++i) {
+        // (The ring is filled by the same instructions: code that runs once is fetched at
+        // memory latency, and a few warps have nothing to hide that behind.)
+#pragma unroll 1
+        for (int i = 1 - S::kStages; i < n_units; ++i) {
             issue(next, stage == 0 ? S::kStages - 1 : stage - 1);
             next = look_up();
-            if (fresh) {
+            if (fresh) {   // (at the start: before the rest of the ring's keys fill the queues)
                 fresh = false;
                 new_group();
+            }
+            if (i < 0) {
+                if (++stage == S::kStages) stage = 0;
+                continue;
             }
             cp_wait<S::kStages - 1>();
             __syncwarp();
             const uint32_t valid = s_valid[warp][stage];
             if (valid) {
                 const uint32_t sk = ring + stage * S::kStageBytes, sv = sk + 16 * S::kPitch;
-                float s[2][4] = {};
+                float sc[2][2][4] = {};   // two chains of dependent products a result
                 const uint32_t ka = sk + ((lane & 7) + (lane >> 4) * 8) * S::kPitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     uint32_t b[4];
                     ldsm_x4(b, ka + k * 32);
-                    mma_16816<T>(s[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
-                    mma_16816<T>(s[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+                    mma_16816<T>(sc[k % 2][0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
+                    mma_16816<T>(sc[k % 2][1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
                 }
+                float (&s)[2][4] = sc[0];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[n][x] += sc[1][n][x];
                 bool moved = false;
                 float factor[2] = {1.f, 1.f};
 #pragma unroll
@@ -532,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
                         v.w = fmaf(f, x.w, v.w);
                     }
                     if (whole) {
-                        write_out<To>(a, cu.r, head0 + row, c, v, l);
+                        write_out<To>(a, cu.r, head0 + row, c, v, l, 1.0f / l);
                         if (c == 0) write_lse(a, cu.r, head0 + row, m, l);
                     } else {
                         __stcg(reinterpret_cast<float4*>(part + row * DP + c), v);
@@ -554,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
                 fresh = true;
             }
             if (group_end) group_u0 += cu.s.nt;
-            next_unit(a, cu, per_row);
+            next_unit<kTile>(a, cu, per_row);
             if (++stage == S::kStages) stage = 0;
         }
 
@@ -610,18 +617,21 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
                 sm[i] = __ldcg(q + kRows);
             }
             __syncthreads();
-            for (int row = me / 32; row < pt.rows; row += team_threads / 32) {
+            // eight lanes a row: all rows of a group at once
+            for (int row = me / 8; row < pt.rows; row += team_threads / 8) {
+                const uint32_t eight = 0xFFu << (lane & 24);
                 float m = -INFINITY, l = 0.f;
-                for (int p = lane; p < n_parts; p += 32) m = fmaxf(m, wt[p * pt.rows + row]);
-                for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-                for (int p = lane; p < n_parts; p += 32) {
+                for (int p = lane & 7; p < n_parts; p += 8) m = fmaxf(m, wt[p * pt.rows + row]);
+                for (int k = 4; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(eight, m, k));
+                for (int p = lane & 7; p < n_parts; p += 8) {
                     float& w = wt[p * pt.rows + row];
                     w = w == -INFINITY ? 0.f : exp2_approx(w - m);
                     l = fmaf(w, sm[p * pt.rows + row], l);
                 }
-                for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
-                if (lane == 0) {
+                for (int k = 4; k; k >>= 1) l += __shfl_xor_sync(eight, l, k);
+                if ((lane & 7) == 0) {
                     s_sum[x][row] = l;
+                    s_ref[x][row] = 1.0f / l;
                     write_lse(a, pt.r, pt.head0 + row, m, l);
                 }
             }
@@ -668,14 +678,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) paged_kernel(Paged
             for (int i = 0; i < kEach; ++i) {
                 const int e = e0 + i * team_threads;
                 if (sub == 0 && e < n_out)
-                    write_out<To>(a, pt.r, pt.head0 + e / (DP / 4), e % (DP / 4) * 4, acc[i], s_sum[x][e / (DP / 4)]);
+                    write_out<To>(a, pt.r, pt.head0 + e / (DP / 4), e % (DP / 4) * 4, acc[i], s_sum[x][e / (DP / 4)],
+                                  s_ref[x][e / (DP / 4)]);
             }
         }
     }
 
     // rows with nothing to read
     for (int r = blockIdx.x * kWarps + warp; r < a.n_rows; r += gridDim.x * kWarps) {
-        if (span_of(a, r).nt) continue;
+        if (span_of<kTile>(a, r).nt) continue;
         To* o = static_cast<To*>(a.out) + r * a.ldo;
         for (int i = lane; i < a.n_head * a.d; i += 32) o[i] = from_f32<To>(0.f);
         if (a.lse)
@@ -765,7 +776,7 @@ b2q_status b2q_attention_paged(const void* q, int64_t ldq, int64_t n_rows, int32
             static std::atomic<uint64_t> allowed{0};
             const b2q_status s = allow_smem(kernel, smem, allowed, ds->device);
             if (s) return s;
-            return cuda_check(launch_after(kernel, dim3(grid_of(ds->num_sms, Shape<DP>::kCtas)), dim3(kThreads), smem,
+            return cuda_check(launch_after(kernel, dim3(grid_of(ds->num_sms, Shape<DP>::kCtas)), dim3(Shape<DP>::kThreads), smem,
                                            static_cast<cudaStream_t>(stream), a),
                               "paged attention launch");
         });
