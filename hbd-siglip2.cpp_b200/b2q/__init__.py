@@ -468,30 +468,52 @@ def score(img, txt, logit_scale: float, logit_bias: float, logits=True, probs=Tr
 
 
 # ---- decoding over a paged key-value cache ---------------------------------
-# A decode step calls these once per layer on small tensors, so the common case
-# (contiguous tensors on the current device) is checked in few steps.
+# A decode step calls these once per layer on small tensors, so the host's time
+# counts.  Valid calls take one native step (csrc/b2q_host.cpp); what it does not
+# accept, or every call where it was not built, goes through the checks here, which
+# say what is wrong.
 _TYPE_IDS: dict = {}
 _INT32 = _F32 = None
 _device = _raw_stream = None     # torch's cheap forms: current device, stream of a device
 _plan = _rope = _paged = _vec = None
+HOST_PATH = PKG / "lib" / "b2q_host.so"
+
+
+def _not_native(*args):
+    return None
+
+
+_native_plan = _native_rope = _native_paged = _native_vec = _not_native
 
 
 def _setup():
     """What the calls below look up once."""
     global _INT32, _F32, _device, _raw_stream, _plan, _rope, _paged, _vec
+    global _native_plan, _native_rope, _native_paged, _native_vec
     import torch
     _INT32, _F32 = torch.int32, torch.float32
     _TYPE_IDS.update({torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16})
     _device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
     L = lib()
     _plan, _rope, _paged, _vec = L.b2q_kv_plan, L.b2q_qk_norm_rope, L.b2q_attention_paged, L.b2q_mul_vec_q4
+    if HOST_PATH.exists():
+        from importlib import machinery, util
+        spec = util.spec_from_file_location("b2q_host", HOST_PATH, loader=machinery.ExtensionFileLoader(
+            "b2q_host", str(HOST_PATH)))
+        native = util.module_from_spec(spec)
+        spec.loader.exec_module(native)
+        native.setup(*(C.cast(f, C.c_void_p).value for f in (_plan, _rope, _paged, L.b2q_attention_paged_scratch_bytes,
+                                                             _vec)))
+        _native_plan, _native_rope = native.kv_plan, native.qk_norm_rope
+        _native_paged, _native_vec = native.attention_paged, native.mul_vec_q4
 
 
 def _type_of(t) -> int:
     try:
         return _TYPE_IDS[t.dtype]
     except KeyError:
-        _setup()
+        if _vec is None:
+            _setup()
         if t.dtype not in _TYPE_IDS:
             raise B2QError(ERR_INVALID, f"element type {t.dtype} is not one of float32, float16, bfloat16") from None
         return _TYPE_IDS[t.dtype]
@@ -573,6 +595,10 @@ def kv_plan(ctx_len, new_len, page_size: int, free_pages, block_table, seq_of, p
     ctx_len, new_len: int32 [n_seq]; block_table: int32 [n_seq][max_blocks],
     entered in place; seq_of, pos, slot, kv_len: int32 [max_tokens] and counts
     int32 [2], written."""
+    status = _native_plan(ctx_len, new_len, page_size, free_pages, block_table, seq_of, pos, slot, kv_len, counts,
+                          stream)
+    if status is not None:
+        return check(status) if status else None
     if _plan is None:
         _setup()
     n, rows, i32, dev = ctx_len.numel(), seq_of.numel(), _INT32, _device()
@@ -614,6 +640,10 @@ def qk_norm_rope(qkv, n_head: int, cache: KVCache, q_out, pos, slot, q_weight=No
     their cache slots (b2q_qk_norm_rope).  qkv: [rows][(n_head + 2 n_kv_head)
     d_head]; q_out: [rows][n_head d_head] of the cache's type; pos, slot: int32
     [rows]; rope: fp32 [n_pos][rot_dim] (see rope_table)."""
+    status = _native_rope(qkv, n_head, cache.ref, cache.device, q_out, pos, slot, q_weight, k_weight, eps, rope,
+                          interleaved, stream)
+    if status is not None:
+        return check(status) if status else None
     if _rope is None:
         _setup()
     d, dev = cache.d_head, _device()
@@ -662,6 +692,10 @@ def attention_paged(q, cache: KVCache, block_table, kv_len, out, scratch, seq_of
     (b2q_attention_paged).  q: [rows][n_head d_head] of the cache's type; out
     the same shape, fp32 or the cache's type; block_table: int32 [requests]
     [max_blocks]; kv_len (and seq_of): int32 [rows]; lse: fp32 [rows][n_head]."""
+    status = _native_paged(q, cache.ref, cache.device, block_table, kv_len, out, scratch, seq_of, scale, window, lse,
+                           stream)
+    if status is not None:
+        return check(status) if status else None
     if _paged is None:
         _setup()
     d, dev, shape = cache.d_head, _device(), q.shape
@@ -718,6 +752,9 @@ def mul_vec_q4(w: WeightQ4, x, m: int, y, bias=None, residual=None, stream=None)
     """y[m][n] = x @ w^T (+ bias) (+ residual) for few rows (b2q_mul_vec_q4).
     x: [m][x_cols] fp32, fp16 or bf16 (x_cols rounds up to the weight's K); y:
     [m][n] fp32 or x's type; bias fp32 [n]; residual fp32 like y."""
+    status = _native_vec(w.handle.value, w.n, x, m, y, bias, residual, stream)
+    if status is not None:
+        return check(status) if status else None
     if _vec is None:
         _setup()
     n, dev, shape = w.n, _device(), x.shape
