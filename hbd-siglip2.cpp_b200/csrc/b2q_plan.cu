@@ -12,8 +12,9 @@
 // found by bisection in the scanned sums.  A row's page comes from the free
 // list itself where it is one that this step enters, so no row waits for a
 // table entry that another CTA writes.
-// Measured on one B200, device time: 33 requests of one token 3.1 us, 509 requests of
-// 260,000 rows (4.2 MB) 6.6 us.
+// Measured on one B200, device time: 33 requests of one token 3.2 us, 509 requests of
+// 260,000 rows (4.2 MB) 4.8 us (one row of a thread at a time 6.6; more than one CTA an
+// SM 7.5 to 9).
 #include "b2q_decode.cuh"
 
 namespace b2q {
@@ -55,23 +56,29 @@ __device__ __forceinline__ int blocks_of(const PlanArgs& a, int64_t tokens) {
     return static_cast<int>(b < a.max_blocks ? b : a.max_blocks);
 }
 
-// last s with base[s] <= i (base ascending, base[0] = 0 <= i)
-__device__ __forceinline__ int find_seq(const int* base, int n, int i) {
-    int lo = 0, hi = n;   // base[lo] <= i < base[hi], base[n] > i
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (base[mid] <= i) lo = mid; else hi = mid;
+// last s < n with base[s] <= i of each i (base ascending, base[0] = 0 <= i); searched
+// side by side, as every step is one read from shared memory
+template <int kN>
+__device__ __forceinline__ void find_seqs(const int* base, int n, const int (&i)[kN], int (&s)[kN]) {
+#pragma unroll
+    for (int k = 0; k < kN; ++k) s[k] = 0;
+    for (int left = n; left > 1;) {
+        const int half = left >> 1;
+#pragma unroll
+        for (int k = 0; k < kN; ++k)
+            if (base[s[k] + half] <= i[k]) s[k] += half;
+        left -= half;
     }
-    return lo;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
-    extern __shared__ int sums[];             // row_s [n_seq + 1], first_s [n_seq + 1]
+    extern __shared__ int sums[];             // row_s [n_seq + 1], first_s [n_seq + 1], ctx_s [n_seq]
     __shared__ int warp_rows[kPlanThreads / 32], warp_pages[kPlanThreads / 32];
     let_next_start();
     wait_for_previous();
     int* rows = sums;
-    int* pages = sums + a.n_seq + 1;
+    int* pages = rows + a.n_seq + 1;
+    int* ctxs = pages + a.n_seq + 1;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (a.n_seq + kPlanThreads - 1) / kPlanThreads;
     const int s0 = min(tid * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
@@ -108,6 +115,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
         lengths_of(a, s, ctx, add, again);
         rows[s] = br;
         pages[s] = bp;
+        ctxs[s] = ctx;
         br = sat_add(br, min(add, kPlanCap));
         bp = sat_add(bp, blocks_of(a, static_cast<int64_t>(ctx) + add) - blocks_of(a, ctx));
     }
@@ -125,38 +133,46 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     if (bad || n_rows > a.max_tokens || n_pages > a.n_free) report(a.err, kDevPlanFull);
 
     for (int i = at; i < n_pages; i += step) {
-        const int s = find_seq(pages, a.n_seq, i);
-        int ctx, add;
-        lengths_of(a, s, ctx, add, bad);
-        const int b = blocks_of(a, ctx) + (i - pages[s]);
+        const int one[1] = {i};
+        int s[1];
+        find_seqs(pages, a.n_seq, one, s);
+        const int b = blocks_of(a, ctxs[s[0]]) + (i - pages[s[0]]);
         const int page = i < a.n_free ? a.free_pages[i] : -1;
         if (page < 0) report(a.err, kDevPlanFull);   // a negative entry ends the list
-        a.table[s * a.bt_stride + b] = page < 0 ? -1 : page;
+        a.table[s[0] * a.bt_stride + b] = page < 0 ? -1 : page;
     }
-    for (int t = at; t < a.max_tokens; t += step) {
-        int seq = -1, pos = -1, slot = -1, len = 0;
-        if (t < n_rows) {
-            seq = find_seq(rows, a.n_seq, t);
-            int ctx, add;
-            lengths_of(a, seq, ctx, add, bad);
+    // Four rows of a thread at a time, so that their searches and page reads overlap.
+    constexpr int kEach = 4;
+    for (int t0 = at; t0 < a.max_tokens; t0 += kEach * step) {
+        int t[kEach], seq[kEach], pos[kEach], page[kEach];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) t[k] = t0 + min(k, (a.max_tokens - 1 - t0) / step) * step;
+        find_seqs(rows, a.n_seq, t, seq);   // (0 for a row behind the last; not used)
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            page[k] = -1;
+            if (t[k] >= n_rows) continue;
+            const int ctx = ctxs[seq[k]];
             // a row behind the table's room has no page; its position stays an int32
-            const int64_t p = static_cast<int64_t>(ctx) + (t - rows[seq]);
-            pos = p < INT32_MAX ? static_cast<int>(p) : INT32_MAX - 1;
-            len = pos + 1;
-            const int b = pos >> a.shift, have = blocks_of(a, ctx);
-            int page = -1;
+            const int64_t p = static_cast<int64_t>(ctx) + (t[k] - rows[seq[k]]);
+            pos[k] = p < INT32_MAX ? static_cast<int>(p) : INT32_MAX - 1;
+            const int b = pos[k] >> a.shift, have = blocks_of(a, ctx);
             if (b < have) {
-                page = a.table[seq * a.bt_stride + b];
+                page[k] = a.table[seq[k] * a.bt_stride + b];
             } else if (b < a.max_blocks) {
-                const int i = pages[seq] + (b - have);
-                if (i < a.n_free) page = a.free_pages[i];
+                const int i = pages[seq[k]] + (b - have);
+                if (i < a.n_free) page[k] = a.free_pages[i];
             }
-            if (page >= 0) slot = (page << a.shift) + (pos & ((1 << a.shift) - 1));
         }
-        a.seq_of[t] = seq;
-        a.pos[t] = pos;
-        a.slot[t] = slot;
-        a.kv_len[t] = len;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            if (k && t[k] == t[k - 1]) break;
+            const bool in = t[k] < n_rows;
+            a.seq_of[t[k]] = in ? seq[k] : -1;
+            a.pos[t[k]] = in ? pos[k] : -1;
+            a.slot[t[k]] = page[k] >= 0 ? (page[k] << a.shift) + (pos[k] & ((1 << a.shift) - 1)) : -1;
+            a.kv_len[t[k]] = in ? pos[k] + 1 : 0;
+        }
     }
 }
 
@@ -182,11 +198,11 @@ extern "C" b2q_status b2q_kv_plan(const int32_t* ctx_len, const int32_t* new_len
         return set_error(B2Q_ERR_INVALID, "null pointer");
     PlanArgs a{ctx_len, new_len, free_pages, block_table, bt_stride, seq_of, pos, slot, kv_len, counts, ds->err,
                n_seq, log2_of(page_size), n_free, max_blocks, max_tokens};
-    const size_t smem = 2 * sizeof(int) * (static_cast<size_t>(n_seq) + 1);
+    const size_t smem = sizeof(int) * (3 * static_cast<size_t>(n_seq) + 2);
     b2q_status st;
     if (smem > 40960 &&
         (st = cuda_check(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                              static_cast<int>(2 * sizeof(int) * (kPlanMaxSeq + 1))),
+                                              static_cast<int>(sizeof(int) * (3 * kPlanMaxSeq + 2))),
                          "plan shared memory")))
         return st;
     const int64_t work = max_tokens > n_seq ? max_tokens : n_seq;
