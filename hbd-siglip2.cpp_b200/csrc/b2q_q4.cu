@@ -571,8 +571,9 @@ int n_tiles_of(int rows, int pieces) {
 // operand tile leaves the registers for 24 or 32 warps, and what suits the number
 // of tiles costs least: 256000 x 1152 takes 37.8 us with 32 warps and 35.8 with 24,
 // 7 x 28672 x 8192 33.9 and 35.2.  16 warps start 0.7 us sooner: where an SM has no
-// more than four units for each (1 x 1152 x 4320: 4.4 against 5.1 us), and where two
-// or four operand tiles need the registers.
+// more than four units for each (1 x 1152 x 4320: 4.4 against 5.1 us), where two
+// or four operand tiles need the registers, and where long rows leave 24 warps a ring of
+// a single stage but 16 one of two (4 x 28672 x 8640, Q4_1, fp32: 41.0 against 73.5 us).
 struct Choice {
     int n_tiles, warps, split;
     Q4Plan plan;
@@ -582,9 +583,10 @@ Choice choose(int rows, int pieces, int64_t tiles, int units, int sms, bool min)
     const int n = n_tiles_of(rows, pieces);
     if (!n) return best;
     const bool few = n > 1 || (tiles + sms - 1) / sms * units <= 64;
+    const bool shallow = !few && plan_of(rows, pieces, 24, units, min).stages < 2;
     int64_t best_cost = INT64_MAX;
     for (int warps : {16, 24, 32}) {
-        if ((warps == 16) != few) continue;
+        if (warps == 16 ? !few && !shallow : few) continue;
         const Q4Plan p = plan_of(rows, pieces, warps, units, min);
         if (!p.stages || p.stages < best.plan.stages) continue;
         for (int split = 1; warps % split == 0 && split <= units; split *= 2) {
