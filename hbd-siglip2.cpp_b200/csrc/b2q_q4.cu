@@ -550,7 +550,7 @@ Q4Plan plan_of(int rows, int pieces, int warps, int units, bool min) {
     p.red_at = static_cast<int>(round_up(rows * pieces * p.pitch, 128));
     p.sum_at = p.red_at + static_cast<int>(round_up(2 * warps * 16 * red_pitch(rows * pieces) * 4, 128));
     p.ring_at = p.sum_at + (min ? static_cast<int>(round_up((units * rows + 1) * 32, 128)) : 0);
-    constexpr int kRings[][2] = {{2, 3}, {2, 2}, {1, 2}, {1, 1}};   // units of a group, stages; the last for long rows only
+    constexpr int kRings[][2] = {{2, 3}, {2, 2}, {1, 2}};   // units of a group, stages
     for (const auto& r : kRings) {
         if (warps > 16 && r[1] == 3) continue;   // (as many warps fill shared memory with two)
         p.bytes = p.ring_at + warps * unit_bytes(min) * r[0] * r[1];
@@ -572,8 +572,9 @@ int n_tiles_of(int rows, int pieces) {
 // of tiles costs least: 256000 x 1152 takes 37.8 us with 32 warps and 35.8 with 24,
 // 7 x 28672 x 8192 33.9 and 35.2.  16 warps start 0.7 us sooner: where an SM has no
 // more than four units for each (1 x 1152 x 4320: 4.4 against 5.1 us), where two
-// or four operand tiles need the registers, and where long rows leave 24 warps a ring of
-// a single stage but 16 one of two (4 x 28672 x 8640, Q4_1, fp32: 41.0 against 73.5 us).
+// or four operand tiles need the registers, and where long rows leave no room for 24
+// warps' rings of two stages (4 x 28672 x 8640, Q4_1, fp32: 41.0 us; 24 warps with one
+// stage each 73.5).
 struct Choice {
     int n_tiles, warps, split;
     Q4Plan plan;
@@ -583,10 +584,10 @@ Choice choose(int rows, int pieces, int64_t tiles, int units, int sms, bool min)
     const int n = n_tiles_of(rows, pieces);
     if (!n) return best;
     const bool few = n > 1 || (tiles + sms - 1) / sms * units <= 64;
-    const bool shallow = !few && plan_of(rows, pieces, 24, units, min).stages < 2;
+    const bool full = !few && !plan_of(rows, pieces, 24, units, min).stages;
     int64_t best_cost = INT64_MAX;
     for (int warps : {16, 24, 32}) {
-        if (warps == 16 ? !few && !shallow : few) continue;
+        if (warps == 16 ? !few && !full : few) continue;
         const Q4Plan p = plan_of(rows, pieces, warps, units, min);
         if (!p.stages || p.stages < best.plan.stages) continue;
         for (int split = 1; warps % split == 0 && split <= units; split *= 2) {
@@ -691,7 +692,7 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
     auto choice = [&](int rows) { return choose(rows, pieces, w->tiles, units, ds->num_sms, min); };
     // the most rows that a launch takes (operand tiles and shared memory), then as even launches as that allows
     int most = 1;
-    while (most < M && choice(most + 1).plan.stages >= 2) ++most;
+    while (most < M && choice(most + 1).plan.stages) ++most;
     const int64_t launches = (M + most - 1) / most;
     for (int64_t i = 0, m0 = 0; i < launches; ++i) {
         const int rows = static_cast<int>((M - m0 + launches - i - 1) / (launches - i));
@@ -724,9 +725,7 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
             if (p.group == 2 && p.stages == 3) {
                 if constexpr (decltype(wp)::value == 16) return go(mn, nt, two, std::integral_constant<int, 3>{}, wp);
             }
-            return p.group == 2    ? go(mn, nt, two, two, wp)
-                   : p.stages == 2 ? go(mn, nt, one, two, wp)
-                                   : go(mn, nt, one, one, wp);
+            return p.group == 2 ? go(mn, nt, two, two, wp) : go(mn, nt, one, two, wp);
         };
         constexpr std::integral_constant<int, 16> w16{};
         constexpr std::integral_constant<int, 24> w24{};

@@ -242,3 +242,9 @@ def test_refusals():
         assert e.value.status == status
     assert b2q.lib().b2q_mul_vec_q4(None, None, 0, 1, 32, 32, None, 0, 4, None, None, None) == b2q.ERR_INVALID
     assert b2q.lib().b2q_weight_q4_release(None) == b2q.OK
+
+
+@pytest.mark.parametrize("m, k, typ, dt", [(4, 8640, Q4_1, F32), (3, 12800, Q4_0, F32), (8, 12800, Q4_0, F32),
+                                           (7, 9600, Q4_1, BF16), (9, 14336, Q4_0, F16)])
+def test_long_rows_that_fill_shared_memory(m, k, typ, dt):
+    check(m, 70, k, typ, dt, bias=True)
