@@ -79,7 +79,8 @@ class Decoder:
         self.seq_of, self.pos, self.slot, self.kv_len, self.counts = i32(r), i32(r), i32(r), i32(r), i32(2)
         self.x, self.y, self.qkv, self.attn = f32(r, h), f32(r, h), f32(r, cfg.qkv), f32(r, h)
         self.q = torch.empty((r, h), dtype=torch.float16, device=dev)
-        self.act_h, self.act_f = b2q.act_empty(r, h), b2q.act_empty(r, cfg.ffn)
+        # the layers' rows, and at the end one row per request
+        self.act_h, self.act_f = b2q.act_empty(max(r, max_requests), h), b2q.act_empty(r, cfg.ffn)
         self.last, self.logits = f32(max_requests, h), f32(max_requests, cfg.vocab)
         self.last_n = f32(max_requests, h)
         self.scratch = b2q.attention_paged_scratch(cfg.n_head, self.caches[0])

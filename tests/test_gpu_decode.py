@@ -191,3 +191,15 @@ def test_a_request_alone_and_in_company():
     b = many.step(len(flat))[1].double()
     # the same arithmetic in another order: what the roundings to 16 and 8 bits make of that
     assert ((a - b).norm() / a.norm()).item() <= 0.02
+
+
+def test_more_requests_than_rows_of_a_step():
+    # the last LayerNorm has a row per request: its activations need room for them
+    w, rng = Weights(CFG), np.random.default_rng(10)
+    dec = w.decoder(max_requests=70, max_rows=5, n_pages=40)
+    assert dec.act_h.numel() >= b2q.act_empty(70, CFG.hidden).numel()
+    seqs = [np.zeros((0, CFG.hidden), np.float32) for _ in range(70)]
+    for busy in ({3: 4, 69: 1}, {69: 5}, {0: 1, 3: 1, 40: 2, 69: 1}):
+        new = [busy.get(s, 0) for s in range(70)]
+        check(w, run(dec, seqs, new, 5, rng), seqs, new)
+        assert b2q.check_device() == 0
