@@ -91,8 +91,10 @@ class Decoder:
         (their sum at most rows; rows beyond it are padding).  Returns the
         logits [requests][vocab] after each request's last new token (rows of
         idle requests are those of whatever they had last), valid until the
-        next step."""
+        next step.  B2QError where rows is not in 1..max_rows."""
         import torch
+        if not 1 <= rows <= self.max_rows:
+            raise b2q.B2QError(b2q.ERR_SHAPE, f"a step takes 1 to {self.max_rows} rows, not {rows}")
         c, r = self.cfg, rows
         x, y, qkv, q, attn = self.x[:r], self.y[:r], self.qkv[:r], self.q[:r], self.attn[:r]
         seq_of, pos, slot, kv_len = self.seq_of[:r], self.pos[:r], self.slot[:r], self.kv_len[:r]
