@@ -50,6 +50,18 @@ class DecoderConfig:
         return (self.n_head + 2 * self.n_kv_head) * self.d_head
 
 
+def placed_tokens(seq_of, pos, slot, new_len, max_pos: int):
+    """What a plan (its seq_of, pos and slot of a step's rows) has done for each
+    request: how many of its new tokens have a row and a cache slot, and the row of
+    the last of them.  Rows, pages and positions run out from the end, so these are
+    the first of the tokens that the request brings."""
+    import torch
+    ok = ((slot >= 0) & (pos < max_pos)).to(torch.int32)
+    count = torch.zeros_like(new_len).index_add_(0, seq_of.clamp(min=0), ok)
+    new = new_len.clamp(min=0)
+    return count, (torch.cumsum(new, 0) - new + count - 1).clamp(0, seq_of.numel() - 1)
+
+
 class Decoder:
     """layers: a list of dicts with "qkv", "out" (b2q.WeightQ4), "fc1", "fc2"
     (b2q.Weight), their fp32 biases "qkv_b", "out_b", "fc1_b", "fc2_b", fp32
@@ -76,6 +88,7 @@ class Decoder:
         self.table = torch.full((max_requests, -(-cfg.max_pos // page_size)), -1, dtype=torch.int32, device=dev)
         self.free = torch.arange(n_pages, dtype=torch.int32, device=dev)
         self._iota = torch.arange(n_pages, device=dev)
+        self._block = torch.arange(self.table.shape[1], dtype=torch.int32, device=dev)
         self.seq_of, self.pos, self.slot, self.kv_len, self.counts = i32(r), i32(r), i32(r), i32(r), i32(2)
         self.x, self.y, self.qkv, self.attn = f32(r, h), f32(r, h), f32(r, cfg.qkv), f32(r, h)
         self.q = torch.empty((r, h), dtype=torch.float16, device=dev)
@@ -91,7 +104,11 @@ class Decoder:
         (their sum at most rows; rows beyond it are padding).  Returns the
         logits [requests][vocab] after each request's last new token (rows of
         idle requests are those of whatever they had last), valid until the
-        next step.  B2QError where rows is not in 1..max_rows."""
+        next step.  B2QError where rows is not in 1..max_rows.
+
+        Tokens that get no row, page or position are left out and reported by
+        b2q.check_device: self.ctx_len grows by what was cached, no page is taken for
+        the others, and logits are those after the last token that was."""
         import torch
         if not 1 <= rows <= self.max_rows:
             raise b2q.B2QError(b2q.ERR_SHAPE, f"a step takes 1 to {self.max_rows} rows, not {rows}")
@@ -100,8 +117,13 @@ class Decoder:
         seq_of, pos, slot, kv_len = self.seq_of[:r], self.pos[:r], self.slot[:r], self.kv_len[:r]
         b2q.kv_plan(self.ctx_len, self.new_len, self.page_size, self.free, self.table, seq_of, pos, slot, kv_len,
                     self.counts)
-        # the list moves up by what was taken; -1 ends it
-        after = self._iota + self.counts[1]
+        placed, at = placed_tokens(seq_of, pos, slot, self.new_len, c.max_pos)
+        grown = self.ctx_len + placed
+        # the list moves up by the pages that hold a token (those planned for tokens
+        # without a row are the last ones: they stay in it); -1 ends it
+        had, has = ((n + self.page_size - 1) // self.page_size for n in (self.ctx_len, grown))
+        self.table.masked_fill_(self._block[None] >= has[:, None], -1)
+        after = self._iota + (has - had).sum()
         self.free.copy_(torch.where(after < after.numel(), self.free[after.clamp(max=after.numel() - 1)], -1))
         for w, cache in zip(self.layers, self.caches):
             b2q.ln_quantize(x, w["ln1_w"], w["ln1_b"], c.eps, r, c.hidden, self.act_h, y)
@@ -112,10 +134,9 @@ class Decoder:
             b2q.ln_quantize(x, w["ln2_w"], w["ln2_b"], c.eps, r, c.hidden, self.act_h)
             b2q.mul_mat(w["fc1"], self.act_h, r, kind=b2q.EPI_BIAS_GELU_Q8, bias=w["fc1_b"], act_out=self.act_f)
             b2q.mul_mat(w["fc2"], self.act_f, r, x, kind=b2q.EPI_BIAS_RESIDUAL, bias=w["fc2_b"], residual=x)
-        self.ctx_len += self.new_len
+        self.ctx_len.copy_(grown)
         n = self.ctx_len.numel()
-        at = (torch.cumsum(self.new_len, 0) - 1).clamp(min=0)
-        self.last.copy_(torch.where((self.new_len > 0)[:, None], self.x[at], self.last))
+        self.last.copy_(torch.where((placed > 0)[:, None], x[at], self.last))
         b2q.ln_quantize(self.last, *self.final, c.eps, n, c.hidden, self.act_h, self.last_n)
         b2q.mul_vec_q4(self.head, self.last_n, n, self.logits)
         return self.logits

@@ -1,8 +1,10 @@
 """What the decode operators' binding and the decoder refuse or work out on the host: no GPU."""
+import random
+
 import pytest
 
 import b2q
-from b2q.decode import Decoder
+from b2q.decode import Decoder, placed_tokens
 
 torch = pytest.importorskip("torch")
 
@@ -14,3 +16,40 @@ def test_a_step_refuses_rows_that_its_buffers_do_not_hold(rows):
     with pytest.raises(b2q.B2QError) as e:
         dec.step(rows)
     assert e.value.status == b2q.ERR_SHAPE
+
+
+def plan(ctx, new, page, n_free, width, rows):
+    """seq_of, pos, slot of a step's rows as b2q_kv_plan gives them, token by token."""
+    seq, pos, slot, taken = [-1] * rows, [-1] * rows, [-1] * rows, 0
+    t = 0
+    for s, (c, n) in enumerate(zip(ctx, new)):
+        have = min(-(-c // page), width)
+        for i in range(max(n, 0)):
+            p = c + i
+            if t < rows:
+                seq[t], pos[t] = s, p
+                first = taken + p // page - have
+                if p // page < width and (p // page < have or first < n_free):
+                    slot[t] = (1000 + first) * page + p % page
+            t += 1
+        taken += max(min(-(-(c + max(n, 0)) // page), width) - have, 0)
+    return seq, pos, slot
+
+
+def test_tokens_without_a_row_a_page_or_a_position_do_not_count():
+    rng = random.Random(3)
+    for _ in range(300):
+        n, page, rows = rng.randint(1, 6), rng.choice([1, 4, 16]), rng.randint(1, 40)
+        ctx = [rng.randint(0, 40) for _ in range(n)]
+        new = [rng.choice([0, 1, rng.randint(0, 30), -3]) for _ in range(n)]
+        width, n_free, max_pos = rng.randint(12, 60), rng.randint(0, 20), rng.choice([45, 10 ** 6])
+        ctx = [min(c, width * page, max_pos) for c in ctx]
+        seq, pos, slot = plan(ctx, new, page, n_free, width, rows)
+        count, last = placed_tokens(*(torch.tensor(v, dtype=torch.int32) for v in (seq, pos, slot, new)), max_pos)
+        for s in range(n):
+            good = [t for t in range(rows) if seq[t] == s and slot[t] >= 0 and pos[t] < max_pos]
+            assert count[s] == len(good)
+            assert 0 <= last[s] < rows          # an index that is always there to be read
+            assert [pos[t] for t in good] == list(range(ctx[s], ctx[s] + len(good)))
+            if good:
+                assert last[s] == good[-1]

@@ -203,3 +203,57 @@ def test_more_requests_than_rows_of_a_step():
         new = [busy.get(s, 0) for s in range(70)]
         check(w, run(dec, seqs, new, 5, rng), seqs, new)
         assert b2q.check_device() == 0
+
+
+def pages_of(dec):
+    """Every page that a request owns or that is free, and nothing behind a request's length."""
+    owned = [p for r in dec.table.tolist() for p in r if p >= 0]
+    assert len(owned) == sum(-(-n // dec.page_size) for n in dec.ctx_len.tolist())
+    free = dec.free.tolist()
+    left = [p for p in free if p >= 0]
+    assert free[:len(left)] == left             # no hole
+    return sorted(owned + left)
+
+
+def test_tokens_without_a_row_are_reported_and_not_counted():
+    w, rng = Weights(CFG), np.random.default_rng(11)
+    dec = w.decoder(max_requests=4, max_rows=20, n_pages=40)
+    seqs = [np.zeros((0, CFG.hidden), np.float32) for _ in range(4)]
+    check(w, run(dec, seqs, [6, 0, 3, 0], 9, rng), seqs, [6, 0, 3, 0])
+    # 54 tokens, 20 rows: 15 of the first request's, 5 of the second's, none of the others
+    flat = rng.standard_normal((20, CFG.hidden)).astype(np.float32)
+    dec.x[:] = torch.from_numpy(flat).cuda()
+    dec.new_len.copy_(torch.tensor([15, 35, 4, 0], dtype=torch.int32))
+    logits = dec.step(20)
+    with pytest.raises(b2q.B2QError) as e:
+        b2q.check_device()
+    assert "code 8" in str(e.value)
+    seqs[0], seqs[1] = np.concatenate([seqs[0], flat[:15]]), flat[15:]
+    check(w, logits, seqs, [1, 1, 1, 0])        # (the third one's last token is still its last)
+    assert dec.ctx_len.tolist() == [21, 5, 3, 0] and pages_of(dec) == list(range(40))
+    check(w, run(dec, seqs, [1, 14, 2, 3], 20, rng), seqs, [1, 14, 2, 3])
+    assert b2q.check_device() == 0 and pages_of(dec) == list(range(40))
+
+
+def test_tokens_without_a_page_or_a_position_are_not_counted():
+    w, rng = Weights(CFG), np.random.default_rng(12)
+    dec = w.decoder(max_requests=2, max_rows=64, n_pages=3)
+    seqs = [np.zeros((0, CFG.hidden), np.float32) for _ in range(2)]
+    check(w, run(dec, seqs, [20, 10], 30, rng), seqs, [20, 10])
+    run(dec, seqs, [15, 1], 16, rng)
+    with pytest.raises(b2q.B2QError):
+        b2q.check_device()
+    assert dec.ctx_len.tolist() == [32, 11] and pages_of(dec) == [0, 1, 2]
+    seqs[0] = seqs[0][:32]
+    check(w, run(dec, seqs, [0, 5], 5, rng), seqs, [0, 5])
+    assert b2q.check_device() == 0 and dec.ctx_len.tolist() == [32, 16]
+    # the block table ends at position 256, before the pages do
+    dec = w.decoder(max_requests=1, max_rows=64, n_pages=40)
+    seqs = [np.zeros((0, CFG.hidden), np.float32)]
+    for _ in range(4):
+        run(dec, seqs, [63], 63, rng)
+    assert b2q.check_device() == 0
+    run(dec, seqs, [9], 9, rng)
+    with pytest.raises(b2q.B2QError):
+        b2q.check_device()
+    assert dec.ctx_len.tolist() == [256] and pages_of(dec) == list(range(40))
