@@ -120,7 +120,7 @@ class Decoder:
         placed, at = placed_tokens(seq_of, pos, slot, self.new_len, c.max_pos)
         grown = self.ctx_len + placed
         # the list moves up by the pages that hold a token (those planned for tokens
-        # without a row are the last ones: they stay in it); -1 ends it
+        # without a row are the last ones: they stay in it), with -1 behind its last
         had, has = ((n + self.page_size - 1) // self.page_size for n in (self.ctx_len, grown))
         self.table.masked_fill_(self._block[None] >= has[:, None], -1)
         after = self._iota + (has - had).sum()
@@ -143,8 +143,9 @@ class Decoder:
 
     def release(self, request: int):
         """Ends a request: its pages are free again (synchronises)."""
-        have, left = -(-int(self.ctx_len[request]) // self.page_size), int((self.free >= 0).sum())
-        self.free[left:left + have] = self.table[request, :have]
+        row = self.table[request]
+        pages, left = row[row >= 0], int((self.free >= 0).sum())
+        self.free[left:left + pages.numel()] = pages
         self.ctx_len[request] = 0
         self.table[request] = -1
 

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
         find_seqs(pages, a.n_seq, one, s);
         const int b = blocks_of(a, ctxs[s[0]]) + (i - pages[s[0]]);
         const int page = i < a.n_free ? a.free_pages[i] : -1;
-        if (page < 0) report(a.err, kDevPlanFull);   // a negative entry ends the list
+        if (page < 0) report(a.err, kDevPlanFull);   // a negative entry is no page; those behind it are still taken
         a.table[s[0] * a.bt_stride + b] = page < 0 ? -1 : page;
     }
     // Four rows of a thread at a time, so that their searches and page reads overlap.

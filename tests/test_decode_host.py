@@ -53,3 +53,17 @@ def test_tokens_without_a_row_a_page_or_a_position_do_not_count():
             assert [pos[t] for t in good] == list(range(ctx[s], ctx[s] + len(good)))
             if good:
                 assert last[s] == good[-1]
+
+
+def test_a_released_request_leaves_no_hole_in_the_free_list():
+    dec = Decoder.__new__(Decoder)
+    dec.page_size = 16
+    dec.table = torch.tensor([[4, 5, -1, 7], [1, -1, -1, -1], [6, 2, 3, -1]], dtype=torch.int32)
+    dec.ctx_len = torch.tensor([64 + 20, 9, 48], dtype=torch.int32)     # the first one's past its table row
+    dec.free = torch.tensor([0] + [-1] * 7, dtype=torch.int32)
+    for s, free in [(0, [0, 4, 5, 7]), (2, [0, 4, 5, 7, 6, 2, 3]), (1, [0, 4, 5, 7, 6, 2, 3, 1]), (1, None)]:
+        dec.release(s)
+        assert dec.ctx_len[s] == 0 and (dec.table[s] == -1).all()
+        if free:
+            assert dec.free.tolist() == free + [-1] * (8 - len(free))
+    assert sorted(dec.free.tolist()) == list(range(8))

@@ -257,3 +257,35 @@ def test_tokens_without_a_page_or_a_position_are_not_counted():
     with pytest.raises(b2q.B2QError):
         b2q.check_device()
     assert dec.ctx_len.tolist() == [256] and pages_of(dec) == list(range(40))
+
+
+def test_pages_after_they_ran_out():
+    # run out, release, go on, release twice: every page is owned or free, exactly once
+    w, rng = Weights(CFG), np.random.default_rng(13)
+    dec = w.decoder(max_requests=3, max_rows=64, n_pages=6)
+    seqs = [np.zeros((0, CFG.hidden), np.float32) for _ in range(3)]
+
+    def out_of_pages(new):
+        run(dec, seqs, new, sum(new), rng)
+        with pytest.raises(b2q.B2QError):
+            b2q.check_device()
+        for s in range(3):
+            seqs[s] = seqs[s][:int(dec.ctx_len[s])]
+        assert pages_of(dec) == list(range(6))
+
+    def release(s):
+        dec.release(s)
+        seqs[s] = seqs[s][:0]
+        assert pages_of(dec) == list(range(6))
+
+    check(w, run(dec, seqs, [20, 10, 30], 60, rng), seqs, [20, 10, 30])
+    out_of_pages([31, 15, 10])
+    assert dec.ctx_len.tolist() == [48, 16, 32]
+    release(1)
+    check(w, run(dec, seqs, [10, 0, 0], 10, rng), seqs, [10, 0, 0])
+    out_of_pages([10, 3, 0])
+    assert dec.ctx_len.tolist() == [64, 0, 32]
+    release(0)
+    release(2)
+    check(w, run(dec, seqs, [20, 30, 14], 64, rng), seqs, [20, 30, 14])
+    assert b2q.check_device() == 0 and pages_of(dec) == list(range(6))
