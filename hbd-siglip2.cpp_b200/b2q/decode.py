@@ -94,7 +94,8 @@ class Decoder:
         self.q = torch.empty((r, h), dtype=torch.float16, device=dev)
         # the layers' rows, and at the end one row per request
         self.act_h, self.act_f = b2q.act_empty(max(r, max_requests), h), b2q.act_empty(r, cfg.ffn)
-        self.last, self.logits = f32(max_requests, h), f32(max_requests, cfg.vocab)
+        # a request that has brought nothing yet has a last row of zeros
+        self.last, self.logits = f32(max_requests, h).zero_(), f32(max_requests, cfg.vocab)
         self.last_n = f32(max_requests, h)
         self.scratch = b2q.attention_paged_scratch(cfg.n_head, self.caches[0])
 

@@ -289,3 +289,14 @@ def test_pages_after_they_ran_out():
     release(2)
     check(w, run(dec, seqs, [20, 30, 14], 64, rng), seqs, [20, 30, 14])
     assert b2q.check_device() == 0 and pages_of(dec) == list(range(6))
+
+
+def test_requests_that_have_brought_nothing_have_the_logits_of_zeros():
+    w, rng = Weights(CFG), np.random.default_rng(14)
+    taken = [torch.full((3, CFG.hidden), float("nan"), device="cuda") for _ in range(64)]
+    del taken                                   # memory that the decoder's buffers may get
+    dec = w.decoder(max_requests=3, max_rows=8, n_pages=8)
+    logits = run(dec, [np.zeros((0, CFG.hidden), np.float32)] * 3, [0, 4, 0], 4, rng).double().cpu().numpy()
+    ref = w.final[1].astype(np.float64) @ w.head_exact.T     # the last LayerNorm of zeros is its bias
+    for s in (0, 2):
+        assert np.linalg.norm(logits[s] - ref) <= 1e-5 * np.linalg.norm(ref)
