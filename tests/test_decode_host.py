@@ -67,3 +67,17 @@ def test_a_released_request_leaves_no_hole_in_the_free_list():
         if free:
             assert dec.free.tolist() == free + [-1] * (8 - len(free))
     assert sorted(dec.free.tolist()) == list(range(8))
+
+
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_an_expanded_cache_is_refused(dim):
+    # a stride of 0 reads as "contiguous order": the kernels would run past the tensor
+    shape = [6, 4, 16, 64]
+    shape[dim] = 1
+    one = torch.zeros(shape, dtype=torch.float16)
+    full = torch.zeros((6, 4, 16, 64), dtype=torch.float16)
+    for k, v in ((one.expand(6, 4, 16, 64),) * 2, (one.expand(6, 4, 16, 64), full), (full, one.expand(6, 4, 16, 64))):
+        with pytest.raises(b2q.B2QError) as e:
+            b2q.KVCache(k, v)
+        assert e.value.status == b2q.ERR_SHAPE
+    b2q.KVCache(full, full)
