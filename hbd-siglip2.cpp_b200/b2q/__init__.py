@@ -580,6 +580,7 @@ class KVCache:
     def __init__(self, k, v):
         _require(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype,
                  "k and v must be alike, [n_pages][n_kv_head][page_size][d_head]")
+        _require(k.device == v.device, f"k on {k.device}, v on {v.device}", ERR_INVALID)
         _require(k.stride(3) == 1, "the elements of a head must be contiguous")
         # (to the library a stride of 0 means the contiguous order)
         _require(all(st or n <= 1 for n, st in zip(k.shape, k.stride())), "k and v must not be expanded")

@@ -81,3 +81,12 @@ def test_an_expanded_cache_is_refused(dim):
             b2q.KVCache(k, v)
         assert e.value.status == b2q.ERR_SHAPE
     b2q.KVCache(full, full)
+
+
+def test_keys_and_values_on_two_devices_are_refused():
+    k = torch.zeros((2, 4, 16, 64), dtype=torch.float16)
+    v = torch.zeros((2, 4, 16, 64), dtype=torch.float16, device="meta")
+    for pair in ((k, v), (v, k)):
+        with pytest.raises(b2q.B2QError) as e:
+            b2q.KVCache(*pair)
+        assert e.value.status == b2q.ERR_INVALID

@@ -202,3 +202,12 @@ def test_without_a_device_nothing_is_accepted():
     assert b2q._native_plan(n, n, 4, n, n, n, n, n, n, n, None) is None
     assert b2q._native_rope(x, 1, None, 0, x, n, n, None, None, 1e-6, None, False, None) is None
     assert b2q._native_paged(x, None, 0, n, n, x, x, None, None, 0, None, None) is None
+
+
+@pytest.mark.gpu
+def test_a_cache_with_one_half_on_the_host_is_refused():
+    device()
+    k = torch.zeros((2, 4, 16, 64), dtype=F16, device="cuda")
+    for pair in ((k, k.cpu()), (k.cpu(), k)):
+        with pytest.raises(b2q.B2QError):
+            b2q.KVCache(*pair)
