@@ -578,17 +578,20 @@ class KVCache:
     dimensions (a permuted view is described by its strides)."""
 
     def __init__(self, k, v):
-        _require(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype,
+        _require(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype
+                 and all(a == b or n == 1 for n, a, b in zip(k.shape, k.stride(), v.stride())),
                  "k and v must be alike, [n_pages][n_kv_head][page_size][d_head]")
         _require(k.device == v.device, f"k on {k.device}, v on {v.device}", ERR_INVALID)
-        _require(k.stride(3) == 1, "the elements of a head must be contiguous")
+        _require(k.stride(3) == 1 or k.shape[3] == 1, "the elements of a head must be contiguous")
         # (to the library a stride of 0 means the contiguous order)
         _require(all(st or n <= 1 for n, st in zip(k.shape, k.stride())), "k and v must not be expanded")
         self.k, self.v = k, v
         self.n_pages, self.n_kv_head, self.page_size, self.d_head = k.shape
         self.dtype, self.device = k.dtype, k.get_device()
+        # a dimension of one entry may have any stride: none is passed on
+        strides = [0 if n == 1 else st for n, st in zip(k.shape[:3], k.stride())]
         self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _type_of(k), self.n_pages, self.page_size, self.n_kv_head,
-                                self.d_head, k.stride(0), k.stride(1), k.stride(2))
+                                self.d_head, *strides)
         self.ref = C.addressof(self.desc)
         self.scratch_bytes: dict[int, int] = {}   # attention_paged scratch by n_head
 

@@ -276,3 +276,21 @@ def test_refusals():
                                          None, None)
     assert null == b2q.ERR_INVALID
     assert b2q.check_device() == 0
+
+
+@pytest.mark.parametrize("shape", [(5, 1, 16, 64), (5, 2, 1, 64), (1, 2, 16, 64), (1, 1, 1, 64)])
+def test_dimensions_of_one_entry_may_have_any_stride(shape):
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(shape, generator=g).half().cuda() for _ in range(2))
+    q, lens = torch.randn((1, shape[1] * 64), generator=g).half().cuda(), i32([shape[0] * shape[2]])
+    table = i32(range(shape[0])).view(1, -1)
+    outs = []
+    for st in (None, 3, 0, 65):     # legal strides of such a dimension, none of a legal cache row
+        kv = [t if st is None else t.as_strided(shape, [st if n == 1 else s for n, s in zip(shape, t.stride())])
+              for t in (k, v)]
+        c = b2q.KVCache(*kv)
+        outs.append(torch.full((1, shape[1] * 64), NAN, device="cuda"))
+        b2q.attention_paged(q, c, table, lens, outs[-1], b2q.attention_paged_scratch(shape[1], c))
+    b2q.KVCache(k, kv[1])
+    assert b2q.check_device() == 0
+    assert torch.isfinite(outs[0]).all() and all(torch.equal(outs[0], o) for o in outs)
