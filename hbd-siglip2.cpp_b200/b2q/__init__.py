@@ -738,6 +738,10 @@ class WeightQ4:
         size = buf.nbytes if host else buf.numel() * buf.element_size()
         _require(size >= n * row_bytes and (host or (buf.is_cuda and buf.is_contiguous())),
                  "blocks must be contiguous and hold n rows")
+        if not host:
+            if _device is None:
+                _setup()
+            _refuse_device(_device(), buf)
         check(lib().b2q_weight_q4_register(buf.ctypes.data if host else buf.data_ptr(), ggml_type, n, k, row_bytes,
                                            int(host), _stream(stream), C.byref(self.handle)))
         self.n, self.k, self.ggml_type = n, k, ggml_type

@@ -90,3 +90,21 @@ def test_keys_and_values_on_two_devices_are_refused():
         with pytest.raises(b2q.B2QError) as e:
             b2q.KVCache(*pair)
         assert e.value.status == b2q.ERR_INVALID
+
+
+def test_weight_blocks_of_another_gpu_are_refused(monkeypatch):
+    class Blocks:                               # a tensor of the second GPU, as far as it is looked at
+        is_cuda, device = True, "cuda:1"
+        numel, element_size, is_contiguous = (lambda self: 4 * 36), (lambda self: 1), (lambda self: True)
+        get_device, data_ptr = (lambda self: 1), (lambda self: 4096)
+
+    registered = []
+    monkeypatch.setattr(b2q, "_device", lambda: 0)
+    monkeypatch.setattr(b2q, "_stream", lambda s: None)
+    monkeypatch.setattr(b2q.lib(), "b2q_weight_q4_register", lambda *a: registered.append(a) or 0)
+    with pytest.raises(b2q.B2QError) as e:
+        b2q.WeightQ4(Blocks(), 4, 64)
+    assert e.value.status == b2q.ERR_INVALID and not registered
+    monkeypatch.setattr(Blocks, "get_device", lambda self: 0)
+    b2q.WeightQ4(Blocks(), 4, 64)
+    assert len(registered) == 1
