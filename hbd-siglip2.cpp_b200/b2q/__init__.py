@@ -710,8 +710,8 @@ def attention_paged(q, cache: KVCache, block_table, kv_len, out, scratch, seq_of
     rows, width = shape
     n_head = width // d
     ldq, ldo = _rows(q, n_head * d, "q"), _rows(out, width, "out")
-    if scratch.numel() < _paged_scratch_bytes(n_head, cache):
-        raise B2QError(ERR_SHAPE, "scratch smaller than attention_paged_scratch")
+    if scratch.numel() < _paged_scratch_bytes(n_head, cache) or not scratch.is_contiguous():
+        raise B2QError(ERR_SHAPE, "scratch smaller than attention_paged_scratch, or not contiguous")
     table, stride, blocks, requests = _table(block_table)
     if not (dev == q.get_device() == cache.device == block_table.get_device() == kv_len.get_device()
             == out.get_device() == scratch.get_device() and (seq_of is None or seq_of.get_device() == dev)

@@ -243,7 +243,7 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
         auto* pe = static_cast<float*>(g.entries(lse, at::kFloat, rows * n_head));
         if (!g.ok) return nullptr;
         const size_t need = f_scratch(n_head, c->n_kv_head, c->d_head);
-        if (!need || static_cast<size_t>(scratch->numel()) < need) return nullptr;
+        if (!need || static_cast<size_t>(scratch->numel()) < need || !scratch->is_contiguous()) return nullptr;
         return result(unlocked([&] {
             return f_paged(q->data_ptr(), ldq, rows, n_head, c, static_cast<const int32_t*>(table->data_ptr()), stride,
                            blocks, requests, ps, pl, static_cast<float>(scale), window, out->data_ptr(), type, ldo, pe,

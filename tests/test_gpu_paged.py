@@ -294,3 +294,16 @@ def test_dimensions_of_one_entry_may_have_any_stride(shape):
     b2q.KVCache(k, kv[1])
     assert b2q.check_device() == 0
     assert torch.isfinite(outs[0]).all() and all(torch.equal(outs[0], o) for o in outs)
+
+
+def test_scratch_that_is_not_contiguous_is_refused():
+    # an expanded view has the entries, not the bytes
+    c = b2q.KVCache(*(torch.zeros((2, 2, 16, 64), dtype=F16, device="cuda") for _ in range(2)))
+    q, out = torch.zeros((1, 256), dtype=F16, device="cuda"), torch.zeros((1, 256), device="cuda")
+    n = b2q.attention_paged_scratch(4, c).numel()
+    buf = torch.zeros(2 * n, dtype=torch.uint8, device="cuda")
+    b2q.attention_paged(q, c, i32([0]).view(1, 1), i32([1]), out, buf)
+    for scratch in (buf[:1].expand(n), buf[::2], buf.view(2, n)[:, :n // 2 + 8]):
+        with pytest.raises(b2q.B2QError) as e:
+            b2q.attention_paged(q, c, i32([0]).view(1, 1), i32([1]), out, scratch)
+        assert e.value.status == b2q.ERR_SHAPE
