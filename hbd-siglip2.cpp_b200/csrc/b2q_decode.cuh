@@ -14,6 +14,11 @@
 namespace b2q {
 
 inline bool ptr_aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+// Arrays of 32-bit entries (null ones too).
+template <class... P>
+inline bool words(const P*... p) {
+    return (ptr_aligned(p, 4) && ...);
+}
 inline int log2_of(int p) { return p <= 1 ? 0 : 1 + log2_of(p >> 1); }
 
 __device__ __forceinline__ float to_f32(float x) { return x; }

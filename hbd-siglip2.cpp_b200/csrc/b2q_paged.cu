@@ -760,6 +760,7 @@ b2q_status b2q_attention_paged(const void* q, int64_t ldq, int64_t n_rows, int32
     if (!ptr_aligned(scratch, 256)) return set_error(B2Q_ERR_ALIGN, "scratch must be 256-byte aligned");
     if (ldq % 8 || !ptr_aligned(q, 16)) return set_error(B2Q_ERR_ALIGN, "query rows need 16-byte alignment");
     if (!ptr_aligned(out, out_dtype == B2Q_TYPE_F32 ? 4 : 2)) return set_error(B2Q_ERR_ALIGN, "misaligned out");
+    if (!words(block_table, seq_of, kv_len, lse)) return set_error(B2Q_ERR_ALIGN, "misaligned array");
     const int group = n_head / c.n_kv_head;
     auto go = [&](auto t, auto to) {
         using T = decltype(t);

@@ -196,6 +196,8 @@ extern "C" b2q_status b2q_kv_plan(const int32_t* ctx_len, const int32_t* new_len
     if (!counts || (n_seq > 0 && (!ctx_len || !new_len)) || (n_seq > 0 && max_blocks > 0 && !block_table) ||
         (n_free > 0 && !free_pages) || (max_tokens > 0 && (!seq_of || !pos || !slot || !kv_len)))
         return set_error(B2Q_ERR_INVALID, "null pointer");
+    if (!words(ctx_len, new_len, free_pages, block_table, seq_of, pos, slot, kv_len, counts))
+        return set_error(B2Q_ERR_ALIGN, "misaligned array");
     PlanArgs a{ctx_len, new_len, free_pages, block_table, bt_stride, seq_of, pos, slot, kv_len, counts, ds->err,
                n_seq, log2_of(page_size), n_free, max_blocks, max_tokens};
     const size_t smem = sizeof(int) * (3 * static_cast<size_t>(n_seq) + 2);

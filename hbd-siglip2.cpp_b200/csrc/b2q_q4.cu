@@ -682,7 +682,7 @@ b2q_status b2q_mul_vec_q4(const b2q_weight_q4* w, const void* x, int32_t x_dtype
     if (M == 0) return B2Q_OK;
     if (!x || !y) return set_error(B2Q_ERR_INVALID, "null pointer");
     if (!ptr_aligned(x, x_dtype == B2Q_TYPE_F32 ? 4 : 2) || !ptr_aligned(y, y_dtype == B2Q_TYPE_F32 ? 4 : 2) ||
-        !ptr_aligned(bias, 4) || !ptr_aligned(residual, 4))
+        !words(bias, residual))
         return set_error(B2Q_ERR_ALIGN, "misaligned rows");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool min = w->type == B2Q_TYPE_Q4_1;

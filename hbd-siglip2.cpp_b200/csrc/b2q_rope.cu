@@ -380,6 +380,7 @@ extern "C" b2q_status b2q_qk_norm_rope(const void* qkv, int32_t dtype, int64_t l
     if (!qkv || !pos || !slot || !q_out || (rot_dim > 0 && !rope)) return set_error(B2Q_ERR_INVALID, "null pointer");
     const size_t es = dtype == B2Q_TYPE_F32 ? 4 : 2;
     if (!ptr_aligned(qkv, es) || !ptr_aligned(q_out, 2)) return set_error(B2Q_ERR_ALIGN, "misaligned rows");
+    if (!words(q_weight, k_weight, rope, pos, slot)) return set_error(B2Q_ERR_ALIGN, "misaligned array");
     if (n_rows * heads > (int64_t(1) << 33)) return set_error(B2Q_ERR_SHAPE, "too many heads in one call");
     auto go = [&](auto tin, auto tc) {
         using Tin = decltype(tin);

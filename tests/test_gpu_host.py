@@ -211,3 +211,37 @@ def test_a_cache_with_one_half_on_the_host_is_refused():
     for pair in ((k, k.cpu()), (k.cpu(), k)):
         with pytest.raises(b2q.B2QError):
             b2q.KVCache(*pair)
+
+
+@pytest.mark.gpu
+def test_misaligned_arrays_are_refused_at_the_c_entry():
+    # 32-bit entries at an odd address would fault: the call says so and launches nothing
+    device()
+    L, c = b2q.lib(), cache(F16)
+    n = 3
+    ints = [i32([0] * 16) for _ in range(9)]
+    pi = [t.data_ptr() for t in ints]
+    x, q = torch.zeros((n, 6 * 16), device="cuda"), torch.zeros((n, 32), dtype=F16, device="cuda")
+    out, lse, w = torch.zeros((n, 32), device="cuda"), torch.zeros((n, 2), device="cuda"), torch.ones(32, device="cuda")
+    rope, scratch = b2q.rope_table(4, 16), b2q.attention_paged_scratch(2, c)
+
+    def plan(p):
+        return L.b2q_kv_plan(p[0], p[1], n, 4, p[2], 4, p[3], 5, 5, n, p[4], p[5], p[6], p[7], p[8], None)
+
+    def turn(p):
+        return L.b2q_qk_norm_rope(x.data_ptr(), 0, 96, n, 2, p[0], p[1], 1e-6, p[2], 4, 16, 0, p[3], p[4],
+                                  q.data_ptr(), 32, c.ref, None)
+
+    def attend(p):
+        return L.b2q_attention_paged(q.data_ptr(), 32, n, 2, c.ref, p[0], 1, 1, n, p[1], p[2], 1.0, 0, out.data_ptr(),
+                                     0, 32, p[3], scratch.data_ptr(), None)
+
+    for call, good in ((plan, pi), (turn, [w.data_ptr(), w.data_ptr(), rope.data_ptr(), pi[0], pi[1]]),
+                       (attend, [pi[0], pi[1], pi[2], lse.data_ptr()])):
+        before = L.b2q_launch_count()
+        for i in range(len(good)):
+            assert call([a + 2 * (i == j) for j, a in enumerate(good)]) == b2q.ERR_ALIGN, (call.__name__, i)
+        assert L.b2q_launch_count() == before
+        if call is not turn:    # (its three rows would share a slot)
+            assert call(good) == b2q.OK
+    torch.cuda.synchronize()
