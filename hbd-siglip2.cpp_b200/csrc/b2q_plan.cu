@@ -56,6 +56,12 @@ __device__ __forceinline__ int blocks_of(const PlanArgs& a, int64_t tokens) {
     return static_cast<int>(b < a.max_blocks ? b : a.max_blocks);
 }
 
+// Whether a page has slots of its own: not negative, and its slots fit an int32 (those
+// of a larger one would wrap round to other pages' slots).
+__device__ __forceinline__ bool is_page(const PlanArgs& a, int page) {
+    return static_cast<uint32_t>(page) <= static_cast<uint32_t>(INT32_MAX >> a.shift);
+}
+
 // last s < n with base[s] <= i of each i (base ascending, base[0] = 0 <= i); searched
 // side by side, as every step is one read from shared memory
 template <int kN>
@@ -138,8 +144,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
         find_seqs(pages, a.n_seq, one, s);
         const int b = blocks_of(a, ctxs[s[0]]) + (i - pages[s[0]]);
         const int page = i < a.n_free ? a.free_pages[i] : -1;
-        if (page < 0) report(a.err, kDevPlanFull);   // a negative entry is no page; those behind it are still taken
-        a.table[s[0] * a.bt_stride + b] = page < 0 ? -1 : page;
+        const bool ok = is_page(a, page);
+        if (!ok) report(a.err, kDevPlanFull);   // such an entry is no page; those behind it are still taken
+        a.table[s[0] * a.bt_stride + b] = ok ? page : -1;
     }
     // Four rows of a thread at a time, so that their searches and page reads overlap.
     constexpr int kEach = 4;
@@ -162,6 +169,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
             } else if (b < a.max_blocks) {
                 const int i = pages[seq[k]] + (b - have);
                 if (i < a.n_free) page[k] = a.free_pages[i];
+            }
+            if (!is_page(a, page[k])) {
+                if (page[k] >= 0) report(a.err, kDevPlanFull);
+                page[k] = -1;
             }
         }
 #pragma unroll

@@ -330,8 +330,9 @@ typedef struct b2q_kv_cache {
  * new_len[s]; block_table[s * bt_stride + b] (max_blocks entries) is the page
  * of its tokens b * page_size ...  Pages that the new tokens need are taken
  * from free_pages in order (requests in order, each request's pages in order;
- * a negative entry is no page) and entered into the table.  The new tokens of all requests back to back are
- * the step's rows; row t receives
+ * an entry that is negative or whose slots pass an int32 is no page) and entered
+ * into the table.  The new tokens of all requests back to back are the step's
+ * rows; row t receives
  *   seq_of[t] its request, pos[t] its position, slot[t] its cache slot,
  *   kv_len[t] = pos + 1 (what b2q_attention_paged reads for a causal row);
  * rows from the number of tokens up to max_tokens get -1, -1, -1, 0, so that a

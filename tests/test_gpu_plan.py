@@ -144,3 +144,33 @@ def test_refusals():
     null = b2q.lib().b2q_kv_plan(None, None, 1, 16, None, 0, None, 1, 1, 1, None, None, None, None, None, None)
     assert null == b2q.ERR_INVALID
     assert b2q.check_device() == 0
+
+
+@pytest.mark.parametrize("page", [1, 16, 1024])
+def test_pages_whose_slots_would_wrap_are_no_pages(page):
+    # slots are int32: 2^28 pages of 16 on, a page's slots would be those of page 0 again
+    top = (2 ** 31 - 1) // page                 # the last page whose slots all fit
+    table = np.full((3, 3), -1, np.int32)
+    ctx, new = [page, page, 0], [page, 1, 1]
+    table[:2, 0] = [7, 3]
+    _, out, counts = run(ctx, new, page, [top - 1, top - 1, 5], table, page + 2)
+    last = page + 1
+    np.testing.assert_array_equal(out["slot"][:page], (top - 1) * page + np.arange(page))
+    assert out["slot"][last] == 5 * page and counts == [page + 2, 3] and b2q.check_device() == 0
+    if page == 1:
+        return                                  # every int32 is a page of one token
+    for bad in (top + 1, 2 ** 28, 2 ** 31 - 1):
+        if bad <= top:
+            continue
+        got, out, counts = run(ctx, new, page, [bad, 9, 5], table, page + 2)
+        assert (out["slot"][:page] == -1).all() and out["slot"][page] == 9 * page and out["slot"][last] == 5 * page
+        np.testing.assert_array_equal(got, [[7, -1, -1], [3, 9, -1], [5, -1, -1]])
+        with pytest.raises(b2q.B2QError) as e:
+            b2q.check_device()
+        assert "code 8" in str(e.value)
+        # and one that the table holds already
+        held = np.array([[bad, -1, -1]], np.int32)
+        _, out, _ = run([1], [1], page, [4], held, 1)
+        assert (out["slot"] == -1).all() and (out["pos"] == 1).all()
+        with pytest.raises(b2q.B2QError):
+            b2q.check_device()
