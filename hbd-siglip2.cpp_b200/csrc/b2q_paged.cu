@@ -77,7 +77,7 @@ struct Shape {
 template <int DP, int kRows>
 constexpr int smem_bytes() {
     constexpr int ring = Shape<DP>::kWarps * Shape<DP>::kStages * Shape<DP>::kStageBytes;
-    constexpr int join = 2 * kRows * (kMaxCtas + 2) * 4 + Shape<DP>::kThreads * 16;
+    constexpr int join = 2 * kRows * (kMaxCtas + 2) * 4 + 2 * Shape<DP>::kThreads * 16;
     return ring > join ? ring : join;
 }
 // floats of one partial result: output rows, then refs and sums
@@ -596,9 +596,12 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
             constexpr int kTeamFloats = 2 * kRows * (kMaxCtas + 2);
             float* wt = reinterpret_cast<float*>(smem) + (x ? 2 * kRows * (n0 ? n0 : 0) : 0);
             float* sm = wt + n_parts * pt.rows;
-            float4* red = reinterpret_cast<float4*>(smem + kTeamFloats * 4);
-            // Few outputs: the parts too are dealt to threads, and added up in a second step.
-            const int subs = n_out < team_threads ? min(team_threads / n_out, n_parts) : 1;
+            float4* red = reinterpret_cast<float4*>(smem + kTeamFloats * 4) + team * kThreads;
+            // Few outputs: the parts too are dealt to `subs` sums of an output, added up in
+            // a second step.  Their number goes by the sizes alone and not by the team at
+            // hand, which depends on who reported last: half the threads take them in turns.
+            const int subs = 2 * n_out <= kThreads ? min(kThreads / n_out, n_parts) : 1;
+            const int at_once = subs > 1 ? min(team_threads / n_out, subs) : 1;
             const int sub = subs > 1 ? me / n_out : 0, e0 = subs > 1 ? me % n_out : me;
             constexpr int kEach = (kRows * DP / 4 + kThreads / 2 - 1) / (kThreads / 2);   // outputs of a thread, at most
             constexpr int kFirst = kEach <= 8 ? 2 : 1;   // its parts that are asked for at once, with the refs
@@ -608,7 +611,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
 #pragma unroll
                 for (int i = 0; i < kEach; ++i) {
                     const int p = sub + k * subs, e = e0 + i * team_threads;
-                    if (sub < subs && p < n_parts && e < n_out)
+                    if (sub < at_once && p < n_parts && e < n_out)
                         early[k][i] = __ldcg(reinterpret_cast<const float4*>(part_of(p)) + e);
                 }
             for (int i = me; i < n_parts * pt.rows; i += team_threads) {
@@ -646,7 +649,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
                 acc[i].z = fmaf(f, v.z, acc[i].z);
                 acc[i].w = fmaf(f, v.w, acc[i].w);
             };
-            if (sub < subs) {
+            if (sub < at_once) {
 #pragma unroll
                 for (int k = 0; k < kFirst; ++k)
 #pragma unroll
@@ -663,17 +666,28 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
                         if (e < n_out) add(i, p, e, __ldcg(q + e));
                     }
                 }
+                if (subs > 1) {
+                    red[sub * n_out + e0] = acc[0];
+                    for (int x = sub + at_once; x < subs; x += at_once) {
+                        acc[0] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                        for (int p = x; p < n_parts; p += subs)
+                            add(0, p, e0, __ldcg(reinterpret_cast<const float4*>(part_of(p)) + e0));
+                        red[x * n_out + e0] = acc[0];
+                    }
+                }
             }
-            if (subs > 1 && sub < subs) red[tid] = acc[0];
             __syncthreads();
-            if (subs > 1 && sub == 0)
+            if (subs > 1 && sub == 0) {
+                acc[0] = red[e0];
                 for (int k = 1; k < subs; ++k) {
-                    const float4 v = red[tid + k * n_out];
+                    const float4 v = red[k * n_out + e0];
                     acc[0].x += v.x;
                     acc[0].y += v.y;
                     acc[0].z += v.z;
                     acc[0].w += v.w;
                 }
+            }
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const int e = e0 + i * team_threads;

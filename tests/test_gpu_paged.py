@@ -307,3 +307,19 @@ def test_scratch_that_is_not_contiguous_is_refused():
         with pytest.raises(b2q.B2QError) as e:
             b2q.attention_paged(q, c, i32([0]).view(1, 1), i32([1]), out, scratch)
         assert e.value.status == b2q.ERR_SHAPE
+
+
+@pytest.mark.parametrize("lens", [[5000], [2000, 2100, 1900], [9001], [20011, 3, 700]])
+@pytest.mark.parametrize("hq, hk, d", [(16, 16, 72), (8, 8, 64), (8, 4, 64), (3, 1, 96), (4, 2, 128), (6, 6, 192), (8, 8, 256)])
+def test_bits_repeat_whoever_reports_last(hq, hk, d, lens):
+    # a CTA may come to join one group or two: the order of a group's sums must not know
+    g = torch.Generator(device="cuda").manual_seed(sum(lens) + d)
+    table, pages = deal_pages(np.random.default_rng(4), lens, 16)
+    c = b2q.KVCache(*(torch.randn(pages, hk, 16, d, device="cuda", generator=g).half() for _ in range(2)))
+    q = torch.randn(len(lens), hq * d, device="cuda", generator=g).half()
+    table, lens, scratch = torch.from_numpy(table).cuda(), i32(lens), b2q.attention_paged_scratch(hq, c)
+    outs = [torch.empty(q.shape, device="cuda") for _ in range(100)]
+    for out in outs:
+        b2q.attention_paged(q, c, table, lens, out, scratch)
+    torch.cuda.synchronize()
+    assert sum(not torch.equal(outs[0], o) for o in outs) == 0 and torch.isfinite(outs[0]).all()
