@@ -181,9 +181,25 @@ __device__ __forceinline__ uint32_t add_acq_rel(uint32_t* p, uint32_t v) {
     return old;
 }
 
-// v f, f = 1 / l, for a sum of l; no key: zeros
+// What stands for an element whose sum is NaN although every weight is a number: then
+// values that are none are among those weighted, and what they make is looked at again
+// at the end (no arithmetic or conversion yields this NaN).
+template <class To>
+__device__ __forceinline__ To open_mark();
+template <>
+__device__ __forceinline__ float open_mark<float>() { return __uint_as_float(0x7FC0B2B2u); }
+template <>
+__device__ __forceinline__ __half open_mark<__half>() { return __ushort_as_half(0x7EB2u); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 open_mark<__nv_bfloat16>() { return __ushort_as_bfloat16(0x7FD2u); }
+__device__ __forceinline__ bool is_open(float x) { return __float_as_uint(x) == 0x7FC0B2B2u; }
+__device__ __forceinline__ bool is_open(__half x) { return __half_as_ushort(x) == 0x7EB2u; }
+__device__ __forceinline__ bool is_open(__nv_bfloat16 x) { return __bfloat16_as_ushort(x) == 0x7FD2u; }
+
+// v f, f = 1 / l, for a sum of l; no key: zeros.  Sets *open where it leaves a mark.
 template <class To, class T>
-__device__ __forceinline__ void write_out(const PagedArgs<T>& a, int r, int head, int c, float4 v, float l, float f) {
+__device__ __forceinline__ void write_out(const PagedArgs<T>& a, int r, int head, int c, float4 v, float l, float f,
+                                          uint32_t* open) {
     if (c >= a.d) return;   // d is a multiple of 8
     To* o = static_cast<To*>(a.out) + r * a.ldo + static_cast<int64_t>(head) * a.d + c;
     v = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
@@ -191,6 +207,59 @@ __device__ __forceinline__ void write_out(const PagedArgs<T>& a, int r, int head
     o[1] = from_f32<To>(v.y);
     o[2] = from_f32<To>(v.z);
     o[3] = from_f32<To>(v.w);
+    if ((v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w) && l == l) {
+        *open = 1;
+        if (v.x != v.x) o[0] = open_mark<To>();
+        if (v.y != v.y) o[1] = open_mark<To>();
+        if (v.z != v.z) o[2] = open_mark<To>();
+        if (v.w != v.w) o[3] = open_mark<To>();
+    }
+}
+
+// The marks in the results of `rows` query heads from head0 of row r, all threads: a
+// probability's remainder is zero or negative as often as not, and makes NaN of an
+// infinity that the probability would leave alone.  By the definition infinities of one
+// sign make that infinity; both signs, or a NaN, make NaN.  Reads the row's values once
+// more, 16 loads of a thread in flight.
+template <class To, class T>
+__device__ __noinline__ void settle(const PagedArgs<T>& a, int r, int head0, int rows) {
+    constexpr int kTogether = 16;
+    const Span s = span_of<64>(a, r);
+    for (int i = threadIdx.x; i < rows * (a.d / 4); i += blockDim.x) {
+        const int head = head0 + i / (a.d / 4), c = i % (a.d / 4) * 4;
+        To* o = static_cast<To*>(a.out) + r * a.ldo + static_cast<int64_t>(head) * a.d + c;
+        if (!is_open(o[0]) && !is_open(o[1]) && !is_open(o[2]) && !is_open(o[3])) continue;
+        const T* col = a.c.v + head / a.group * a.c.head_stride + c;
+        uint32_t up = 0, down = 0, nan = 0;   // bit e: element e has such a value
+        for (int key0 = s.first; key0 < s.len && (nan | (up & down)) != 15u;
+             key0 = s.len - key0 > kTogether ? key0 + kTogether : s.len) {
+            uint2 raw[kTogether];
+#pragma unroll
+            for (int k = 0; k < kTogether; ++k) {   // (the last key again behind the end: nothing new)
+                const int key = k < s.len - key0 ? key0 + k : s.len - 1;
+                const int page = a.table[s.seq * a.bt_stride + (key >> a.c.page_shift)];
+                const bool ok = page >= 0 && page < a.c.n_pages;
+                const T* p = col + (ok ? page : 0) * a.c.page_stride + (key & a.c.page_mask) * a.c.token_stride;
+                raw[k] = ok ? *reinterpret_cast<const uint2*>(p) : make_uint2(0u, 0u);
+            }
+#pragma unroll
+            for (int k = 0; k < kTogether; ++k) {
+                const float2 x01 = unpack2<T>(raw[k].x), x23 = unpack2<T>(raw[k].y);
+                const float x[4] = {x01.x, x01.y, x23.x, x23.y};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    up |= static_cast<uint32_t>(x[e] == INFINITY) << e;
+                    down |= static_cast<uint32_t>(x[e] == -INFINITY) << e;
+                    nan |= static_cast<uint32_t>(x[e] != x[e]) << e;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool u = (up >> e) & 1, d = (down >> e) & 1, n = (nan >> e) & 1;
+            if (is_open(o[e])) o[e] = from_f32<To>(n || u == d ? __uint_as_float(0x7FFFFFFFu) : u ? INFINITY : -INFINITY);
+        }
+    }
 }
 template <class T>
 __device__ __forceinline__ void write_lse(const PagedArgs<T>& a, int r, int head, float ref, float l) {
@@ -200,7 +269,7 @@ __device__ __forceinline__ void write_lse(const PagedArgs<T>& a, int r, int head
 }
 
 template <class T, class To, int DP, int kRows>
-__global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_kernel(PagedArgs<T> a) {
+__global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_kernel(const __grid_constant__ PagedArgs<T> a) {
     using S = Shape<DP>;
     constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kTile = S::kTile;
     constexpr int kSteps = DP / 16;           // of 16 elements in q.k
@@ -217,7 +286,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
     __shared__ long long s_base[kWarps];
     __shared__ Start s_start;
     __shared__ Partial s_partial[2];
-    __shared__ uint32_t s_last[2];
+    __shared__ uint32_t s_last[2], s_open;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
@@ -233,6 +302,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
             *reinterpret_cast<uint4*>(smem + i / n * S::kPitch + (from + i % n) * 16) = make_uint4(0, 0, 0, 0);
     }
     if (tid < 2) s_partial[tid].live = 0;
+    if (tid == 0) s_open = 0;
     let_next_start();
     wait_for_previous();
 
@@ -539,7 +609,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
                         v.w = fmaf(f, x.w, v.w);
                     }
                     if (whole) {
-                        write_out<To>(a, cu.r, head0 + row, c, v, l, 1.0f / l);
+                        write_out<To>(a, cu.r, head0 + row, c, v, l, 1.0f / l, &s_open);
                         if (c == 0) write_lse(a, cu.r, head0 + row, m, l);
                     } else {
                         __stcg(reinterpret_cast<float4*>(part + row * DP + c), v);
@@ -693,8 +763,30 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
                 const int e = e0 + i * team_threads;
                 if (sub == 0 && e < n_out)
                     write_out<To>(a, pt.r, pt.head0 + e / (DP / 4), e % (DP / 4) * 4, acc[i], s_sum[x][e / (DP / 4)],
-                                  s_ref[x][e / (DP / 4)]);
+                                  s_ref[x][e / (DP / 4)], &s_open);
             }
+        }
+
+        // ---- infinities and NaN among the values: what they make of the results ----
+        __syncthreads();
+        if (s_open) {
+            const auto settle_group = [&](int r, int hm) {
+                const int q0 = hm % a.row_blocks * kRows;
+                settle<To>(a, r, hm / a.row_blocks * a.group + q0, min(kRows, a.group - q0));
+            };
+            Cursor c;   // the share's whole groups
+            c.r = s_start.r;
+            c.s = s_start.s;
+            c.hm = static_cast<int>(divide(s_start.in_row, c.s.nt));
+            for (long long u = u0 - (s_start.in_row - static_cast<long long>(c.hm) * c.s.nt); u < u0 + n_units;) {
+                const long long next = u + c.s.nt;
+                if (u >= u0 && next <= u0 + n_units) settle_group(c.r, c.hm);
+                u = next;
+                c.t = c.s.nt - 1;
+                next_unit<kTile>(a, c, per_row);
+            }
+            for (int x = 0; x < 2; ++x)   // and those that it joined
+                if (s_last[x]) settle<To>(a, s_partial[x].r, s_partial[x].head0, s_partial[x].rows);
         }
     }
 

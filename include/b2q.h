@@ -359,7 +359,7 @@ b2q_status b2q_kv_plan(const int32_t *ctx_len, const int32_t *new_len, int32_t n
  * slot out of range is reported through b2q_check_device (code 6; position 0 is
  * used, nothing is stored).  Slots of one call are distinct.  q_out may be
  * the Q columns of `qkv` itself when the types agree.  Arithmetic in fp32,
- * rounded once. */
+ * rounded once (past the range of an fp16 cache, 65504, to infinity). */
 b2q_status b2q_qk_norm_rope(const void *qkv, int32_t dtype, int64_t ld, int64_t n_rows, int32_t n_head,
                             const float *q_weight, const float *k_weight, float eps, const float *rope, int32_t n_pos,
                             int32_t rot_dim, int32_t interleaved, const int32_t *pos, const int32_t *slot,
@@ -375,6 +375,8 @@ b2q_status b2q_qk_norm_rope(const void *qkv, int32_t dtype, int64_t ld, int64_t 
  * stride ldo); a row with nothing to read gets zeros.  lse (fp32 [n_rows]
  * [n_head], NULL = not wanted) receives log sum exp(scale q.k), -inf for such
  * rows.  Nothing behind kv_len is read into a result, whatever bits it holds.
+ * Infinite or NaN values among those read make the elements that they belong to
+ * infinite (one sign) or NaN; a score that is NaN or +inf makes the row's head NaN.
  * A request, a page or a length out of range is reported through
  * b2q_check_device (code 7) and its keys are left out.
  * scratch: b2q_attention_paged_scratch_bytes(), 256-byte aligned, all zero

@@ -323,3 +323,79 @@ def test_bits_repeat_whoever_reports_last(hq, hk, d, lens):
         b2q.attention_paged(q, c, table, lens, out, scratch)
     torch.cuda.synchronize()
     assert sum(not torch.equal(outs[0], o) for o in outs) == 0 and torch.isfinite(outs[0]).all()
+
+
+@pytest.mark.parametrize("dt, out_dt", [(F16, F32), (F16, F16), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("hq, hk, d, lens, window", [(4, 2, 64, [1, 33, 200, 0], 0), (16, 16, 72, [997, 40], 0),
+                                                     (8, 1, 256, [700, 3000], 500), (20, 1, 128, [2500, 7], 0),
+                                                     (3, 3, 96, [20, 6001], 0)])
+def test_infinite_and_nan_values_reach_the_result(dt, out_dt, hq, hk, d, lens, window):
+    # a value of +inf or -inf with weight is the result, both signs and NaN are NaN; other
+    # columns, heads and rows keep their sums, and what lies outside the window is not read
+    rng = np.random.default_rng(hq + d)
+    table, pages = deal_pages(rng, lens, 16)
+    kc, vc = (torch.full((pages, hk, 16, d), NAN, dtype=dt, device="cuda") for _ in range(2))
+    q = torch.from_numpy(rng.standard_normal((len(lens), hq * d)).astype(np.float32)).to(dt)
+    keys, vals, inf = [], [], float("inf")
+    for i, n in enumerate(lens):
+        k, v = (torch.from_numpy(rng.standard_normal((n, hk, d)).astype(np.float32)).to(dt) for _ in range(2))
+        lo = max(0, n - window) if window else 0
+        if n:
+            at = lambda: int(rng.integers(lo, n))
+            v[at(), 0, 1] = inf
+            v[at(), 0, 2] = -inf
+            v[n - 1, hk - 1, 5] = inf
+            v[lo, hk - 1, 5] = inf
+            v[at(), hk - 1, 8] = NAN
+            v[at(), hk - 1, 8] = inf if n > 1 else NAN
+            if n > lo + 1:
+                v[lo, 0, 11], v[n - 1, 0, 11] = inf, -inf
+            v[at(), 0, d - 1] = -inf
+            if lo:
+                v[lo - 1, 0, 20] = inf
+            j = np.arange(n)
+            pg, row = torch.from_numpy(table[i, j // 16].astype(np.int64)).cuda(), torch.from_numpy(j % 16).cuda()
+            kc[pg, :, row], vc[pg, :, row] = k.cuda(), v.cuda()
+        keys.append(k.double().numpy())
+        vals.append(v.double().numpy())
+    out = torch.zeros((len(lens), hq * d), dtype=out_dt, device="cuda")
+    c = b2q.KVCache(kc, vc)
+    scratch = b2q.attention_paged_scratch(hq, c)
+    lse = torch.zeros((len(lens), hq), device="cuda")
+    for _ in range(2):          # (the second time on scratch that has seen them)
+        b2q.attention_paged(q.cuda(), c, torch.from_numpy(table).cuda(), i32(lens), out, scratch, window=window, lse=lse)
+    assert b2q.check_device() == 0
+    got = out.double().cpu().numpy().reshape(len(lens), hq, d)
+    more = 2.0 ** -20 if out_dt == F32 else 2.0 ** -15
+    for r, n in enumerate(lens):
+        lo = max(0, n - window) if window else 0
+        k, v = keys[r][lo:n], vals[r][lo:n]
+        plain = np.where(np.isfinite(v), v, 0.0)
+        ref, rl, tol, lt = reference(q[r].double().numpy().reshape(hq, d), k, plain, d ** -0.5)
+        per = hq // hk
+        up, down, nan = (f(v).any(0).repeat(per, 0) if n else np.zeros((hq, d), bool)
+                         for f in (np.isposinf, np.isneginf, np.isnan))
+        nan |= up & down
+        np.testing.assert_array_equal(np.isnan(got[r]), nan)
+        np.testing.assert_array_equal(np.isposinf(got[r]), up & ~nan)
+        np.testing.assert_array_equal(np.isneginf(got[r]), down & ~nan)
+        good = ~(up | down | nan)
+        tol = tol + more * np.abs(plain).max(axis=0, initial=0.0).repeat(per, 0) + UNIT[out_dt] * 1.01 * np.abs(ref) \
+            + TINY[out_dt]
+        within(got[r][good], ref[good], tol[good])
+        if n:
+            within(lse[r].double().cpu().numpy(), rl, lt)
+
+
+def test_scores_that_are_no_numbers_make_the_row_none():
+    # a NaN or infinite key: no weight of the row is a number, whatever the values are
+    k, v = (torch.ones((2, 1, 16, 64), dtype=F16, device="cuda") for _ in range(2))
+    v[0, 0, 3, 7] = float("inf")
+    q, c = torch.ones((2, 64), dtype=F16, device="cuda"), None
+    for bad in (NAN, float("inf")):
+        k[0, 0, 5, 9] = bad
+        c = b2q.KVCache(k, v)
+        out = torch.zeros((2, 64), device="cuda")
+        b2q.attention_paged(q, c, i32([0, 1]).view(2, 1), i32([16, 16]), out, b2q.attention_paged_scratch(1, c))
+        assert torch.isnan(out[0]).all() and (out[1] == 1.0).all()
+    assert b2q.check_device() == 0
