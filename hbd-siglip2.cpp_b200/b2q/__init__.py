@@ -500,8 +500,14 @@ def _setup():
         from importlib import machinery, util
         spec = util.spec_from_file_location("b2q_host", HOST_PATH, loader=machinery.ExtensionFileLoader(
             "b2q_host", str(HOST_PATH)))
-        native = util.module_from_spec(spec)
-        spec.loader.exec_module(native)
+        try:
+            native = util.module_from_spec(spec)
+            spec.loader.exec_module(native)
+        except ImportError as e:     # built against another torch or Python than this one
+            import warnings
+            warnings.warn(f"{HOST_PATH.name} does not load, decode calls take the slower checks in Python: {e}",
+                          RuntimeWarning, stacklevel=3)
+            return
         native.setup(*(C.cast(f, C.c_void_p).value for f in (_plan, _rope, _paged, L.b2q_attention_paged_scratch_bytes,
                                                              _vec)))
         _native_plan, _native_rope = native.kv_plan, native.qk_norm_rope

@@ -108,3 +108,42 @@ def test_weight_blocks_of_another_gpu_are_refused(monkeypatch):
     monkeypatch.setattr(Blocks, "get_device", lambda self: 0)
     b2q.WeightQ4(Blocks(), 4, 64)
     assert len(registered) == 1
+
+
+def test_a_native_half_that_does_not_load_is_left_out(monkeypatch, tmp_path):
+    stale = tmp_path / "b2q_host.so"
+    stale.write_bytes(b"\x7fELF of another time")
+    monkeypatch.setattr(b2q, "HOST_PATH", stale)
+    natives = ("_native_plan", "_native_rope", "_native_paged", "_native_vec")
+    for n in natives:
+        monkeypatch.setattr(b2q, n, b2q._not_native)
+    for n in ("_plan", "_rope", "_paged", "_vec", "_device", "_raw_stream", "_INT32", "_F32"):
+        monkeypatch.setattr(b2q, n, None)
+    with pytest.warns(RuntimeWarning, match="does not load"):
+        b2q._setup()
+    assert b2q._plan is not None and b2q._vec is not None
+    assert all(getattr(b2q, n) is b2q._not_native for n in natives)
+
+
+def test_the_native_half_is_built_again_for_another_torch(tmp_path):
+    import os
+    import shutil
+    import subprocess
+    from pathlib import Path
+    csrc = Path(b2q.__file__).resolve().parents[1] / "csrc"
+    if not shutil.which("make"):
+        pytest.skip("no make")
+    stamp = tmp_path / "b2q_host.for"            # what b2q_host.so depends on
+
+    def make(*more):
+        subprocess.run(["make", "-s", "-C", str(csrc), f"OBJDIR={tmp_path}", str(stamp), *more], check=True)
+        return stamp.read_text(), stamp.stat().st_mtime_ns
+
+    first = make()
+    assert torch.__version__ in first[0]
+    os.utime(stamp, ns=(1, 1))
+    assert make() == (first[0], 1)               # the same: not touched
+    again = make("HOSTFOR=3.12.3 another torch")
+    assert "another torch" in again[0] and again[1] > 1
+    rules = (csrc / "Makefile").read_text()
+    assert "../lib/b2q_host.so: b2q_host.cpp ../../include/b2q.h $(OBJDIR)/b2q_host.for" in rules
