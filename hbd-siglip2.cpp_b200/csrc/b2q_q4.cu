@@ -20,11 +20,14 @@
 //    of 1e-5 beside a large activation.)
 //  * An activation row is scaled by a power of two and becomes fp16 operands: fp16 and
 //    bf16 values one, an fp32 value two, x rounded to 11 bits and the rest rounded to
-//    11 bits, which leaves at most 2^-24 |x|, what a rounding to fp32 may leave; they
-//    take as many of the eight activation columns.  The scale loses what lies 2^-35
-//    below the row's largest value.
+//    11 bits, which leaves nothing of three values in four and at most 2^-23 |x|; they
+//    take as many of the eight activation columns.  The row has one scale, so nothing
+//    is held closer than 2^-34 of its largest value (fp16 ends at 2^-24, and that value
+//    lies at 2^9 or above): beside one 1e6 times as large values keep 14 bits.
 //  * S leaves the tensor core once per block and is summed in fp32, d S.
-// Relative error of 1 x 1152 x 4320 against 64 bits: 9e-8 (plain fp32 products 2e-7).
+// Relative error against 64 bits: 1 x 1152 x 4320, Q4_0, 9e-8 (plain fp32 products
+// 1.9e-7); 1 x 256000 x 1152, Q4_1, 1.6e-7 (1.3e-7: with the minima apart, d S and m X are
+// each several times their sum, and so are their roundings).
 //
 // The weights are laid out at registration in the order the lanes want them:
 // per 16 rows a run of units of 128 columns, each 1024 bytes of nibbles (lane l of
@@ -191,7 +194,7 @@ struct Eight {
 //
 // A warp takes 256 columns of a row at a time.  A row's power of two is a guess
 // from its first 32 values, the largest of them taken to [2^9, 2^10): that leaves
-// the row's largest value a factor of 32, and loses no more than 2^-35 of it.  The
+// the row's largest value a factor of 32, and loses no more than 2^-34 of it.  The
 // same pass takes the peaks; a row that needs more room is staged again with the
 // power that its peak gives (`again`).  Two CTAs of a cluster (`pair`) stage half of
 // the work each and store it in both shared memories.

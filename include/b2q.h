@@ -403,10 +403,13 @@ b2q_status b2q_weight_q4_release(b2q_weight_q4 *w);
  * x[M][ldx] (x_dtype F32, F16 or BF16) of x_cols columns, x_cols rounded up to
  * 32 = K (columns x_cols..K-1 read as zero).  y (y_dtype F32 or x_dtype) and
  * residual (fp32, may be y) have row stride ldy; bias and residual may be
- * NULL; y overlaps neither x nor bias.  The activations are not quantized:
- * products and sums are in fp32, rounded once.  Meant for few rows: a launch
- * takes up to 32 fp16 or bf16 rows or 16 fp32 ones, fewer where their columns
- * do not fit shared memory, and reads the weights once. */
+ * NULL; y overlaps neither x nor bias.  Products and sums are in fp32, the
+ * result is rounded once.  The activations are not quantized to blocks of
+ * integers, but enter as fp16 pieces on one power of two a row: a finite x is
+ * held within 2^-34 of the row's largest finite |x| (fp32 x: plus 2^-23 |x|), so
+ * that values far below that one lose bits.  Infinities and NaN reach the result.
+ * Meant for few rows: a launch takes up to 32 fp16 or bf16 rows or 16 fp32 ones,
+ * fewer where their columns do not fit shared memory, and reads the weights once. */
 b2q_status b2q_mul_vec_q4(const b2q_weight_q4 *w, const void *x, int32_t x_dtype, int64_t M, int64_t x_cols,
                           int64_t ldx, void *y, int32_t y_dtype, int64_t ldy, const float *bias,
                           const float *residual, void *stream);

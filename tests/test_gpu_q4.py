@@ -248,3 +248,61 @@ def test_refusals():
                                            (7, 9600, Q4_1, BF16), (9, 14336, Q4_0, F16)])
 def test_long_rows_that_fill_shared_memory(m, k, typ, dt):
     check(m, 70, k, typ, dt, bias=True)
+
+
+@pytest.mark.parametrize("typ", [Q4_0, Q4_1], ids=["q4_0", "q4_1"])
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("at", [3, 700])
+def test_values_beside_a_far_larger_one(typ, dt, at):
+    """A value that no weight takes part in, up to 1e7 times the others (3e4 in fp16): what they
+    keep is 2^-34 of it, as the header says, and 2^-23 of themselves.  An X of 32 columns is held
+    within 2^-29 of it, which is 2^-34 a column again."""
+    rng = np.random.default_rng(21)
+    b, w, mag = blocks(rng, 200, 1152, typ)
+    blk, i = at // 32, at % 32
+    head = 2 if typ == Q4_0 else 4
+    nib = b[:, blk, head + i % 16]
+    zero = 8 if typ == Q4_0 else 0
+    b[:, blk, head + i % 16] = (nib & 0xF0) | zero if i < 16 else (nib & 0x0F) | zero << 4
+    w[:, at] = mag[:, at] = 0.0
+    if typ == Q4_1:      # ... nor the block's minimum
+        cols = slice(blk * 32, blk * 32 + 32)
+        m = b[:, blk, 2:4].copy().view(np.float16).astype(np.float64)
+        w[:, cols] -= m
+        w[:, at] = 0.0
+        mag[:, cols] -= np.abs(m)
+        mag[:, at] = 0.0
+        b[:, blk, 2:4] = 0
+    W = b2q.WeightQ4(b, 200, 1152, typ)
+    sizes = (1e2, 1e3, 1e4, 3e4) if dt == F16 else (1e2, 1e4, 1e5, 1e6, 1e7)
+    x = rng.standard_normal((len(sizes), 1152)).astype(np.float32)
+    x[:, at] = sizes
+    xd = torch.from_numpy(x).to(dt).cuda()
+    y = torch.zeros((len(sizes), 200), device="cuda")
+    b2q.mul_vec_q4(W, xd, len(sizes), y)
+    x64 = xd.double().cpu().numpy()
+    tol = (32 + 36 + 8 + 1) * 2.0 ** -23 * (np.abs(x64) @ mag.T) \
+        + 2.0 ** -34 * np.abs(x64).max(1, keepdims=True) * mag.sum(1)[None]
+    within(y.double().cpu().numpy(), x64 @ w.T, tol)
+    W.release()
+
+
+def test_a_row_of_one_scale_keeps_its_last_bits():
+    # one weight of 1 in each row of them: the result is the activation as it is held
+    k = 64
+    b = np.zeros((k, k // 32, 18), np.uint8)
+    b[..., 2:] = 0x88
+    for n in range(k):
+        b[n, n // 32, :2] = np.float16(1.0).view(np.uint16).reshape(1).view(np.uint8)
+        i = n % 32
+        b[n, n // 32, 2 + i % 16] = 0x89 if i < 16 else 0x98
+    W = b2q.WeightQ4(b, k, k)
+    rng = np.random.default_rng(22)
+    x = (rng.standard_normal((16, k)) * 2.0 ** rng.uniform(-30, 0, (16, k))).astype(np.float32)
+    x[:, 40] = 1.5
+    for dt, own in ((F32, 2.0 ** -23), (F16, 0.0), (BF16, 0.0)):
+        xd = torch.from_numpy(x).to(dt).cuda()
+        y = torch.zeros((16, k), device="cuda")
+        b2q.mul_vec_q4(W, xd, 16, y)
+        x64 = xd.double().cpu().numpy()
+        within(y.double().cpu().numpy(), x64, own * np.abs(x64) + 2.0 ** -34 * np.abs(x64).max(1, keepdims=True))
