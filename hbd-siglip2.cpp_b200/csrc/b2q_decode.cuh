@@ -103,13 +103,6 @@ __device__ __forceinline__ void cp_async_16(uint32_t smem, const void* gmem, boo
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(valid ? 16u : 0u)
                  : "memory");
 }
-// Untiled bulk copy of this GPU's memory to this CTA's (addresses and size
-// multiples of 16 bytes); its bytes count towards the barrier's transaction.
-__device__ __forceinline__ void bulk_load(uint32_t smem, const void* gmem, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem),
-                 "l"(gmem), "r"(bytes), "r"(bar)
-                 : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
