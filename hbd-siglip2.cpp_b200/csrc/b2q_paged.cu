@@ -367,10 +367,10 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
             Pending p{-1, 0u, 0};
             if (looked < n_units) {
                 ++looked;
-                const int key0 = (ld.s.t0 + ld.t) * kTile + warp * 16;
-                const int lo = max(ld.s.first - key0, 0), hi = min(ld.s.len - key0, 16);
+                const int tile0 = (ld.s.t0 + ld.t) * kTile;   // below len; a warp's keys may pass an int32 behind it
+                const int lo = max(ld.s.first - tile0 - warp * 16, 0), hi = min(ld.s.len - tile0 - warp * 16, 16);
                 if (lo < hi) p.live = ((1u << hi) - 1) & ~((1u << lo) - 1);
-                const int key = key0 + (one_page ? 0 : lane);
+                const int key = static_cast<int>(static_cast<uint32_t>(tile0) + warp * 16 + (one_page ? 0 : lane));
                 const bool mine = one_page ? p.live != 0 : lane < 16 && ((p.live >> lane) & 1);
                 if (mine) p.page = a.table[ld.s.seq * a.bt_stride + (key >> a.c.page_shift)];
                 const int head = a.row_blocks == 1 ? ld.hm : ld.hm / a.row_blocks;

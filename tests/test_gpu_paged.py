@@ -399,3 +399,22 @@ def test_scores_that_are_no_numbers_make_the_row_none():
         b2q.attention_paged(q, c, i32([0, 1]).view(2, 1), i32([16, 16]), out, b2q.attention_paged_scratch(1, c))
         assert torch.isnan(out[0]).all() and (out[1] == 1.0).all()
     assert b2q.check_device() == 0
+
+
+@pytest.mark.parametrize("d, page", [(64, 16), (256, 16), (256, 8), (192, 16)])
+def test_the_longest_context_an_int32_counts(d, page):
+    # 2^31 - page keys on five pages in turn, read through a window at their end
+    blocks = (2 ** 31 - 1) // page
+    n, window = blocks * page, 229
+    rng = np.random.default_rng(d + page)
+    k, v = (torch.from_numpy(rng.standard_normal((5, 1, page, d)).astype(np.float32)).half() for _ in range(2))
+    table = (torch.arange(blocks, dtype=torch.int32, device="cuda") % 5).view(1, blocks)
+    q = torch.from_numpy(rng.standard_normal((1, d)).astype(np.float32)).half()
+    out = torch.empty((1, d), device="cuda")
+    c = b2q.KVCache(k.cuda(), v.cuda())
+    b2q.attention_paged(q.cuda(), c, table, i32([n]), out, b2q.attention_paged_scratch(1, c), window=window)
+    assert b2q.check_device() == 0
+    j = np.arange(n - window, n, dtype=np.int64)
+    keys, vals = (t.double().numpy()[j // page % 5, :, j % page] for t in (k, v))
+    ref, _, tol, _ = reference(q.double().numpy(), keys, vals, d ** -0.5)
+    within(out.double().cpu().numpy(), ref, tol + 2.0 ** -20 * np.abs(vals).max(0) + 2.0 ** -24 * 1.01 * np.abs(ref))
