@@ -170,10 +170,6 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
                 const int i = pages[seq[k]] + (b - have);
                 if (i < a.n_free) page[k] = a.free_pages[i];
             }
-            if (!is_page(a, page[k])) {
-                if (page[k] >= 0) report(a.err, kDevPlanFull);
-                page[k] = -1;
-            }
         }
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
@@ -181,8 +177,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
             const bool in = t[k] < n_rows;
             a.seq_of[t[k]] = in ? seq[k] : -1;
             a.pos[t[k]] = in ? pos[k] : -1;
-            a.slot[t[k]] = page[k] >= 0 ? (page[k] << a.shift) + (pos[k] & ((1 << a.shift) - 1)) : -1;
+            const bool ok = is_page(a, page[k]);
+            a.slot[t[k]] = ok ? (page[k] << a.shift) + (pos[k] & ((1 << a.shift) - 1)) : -1;
             a.kv_len[t[k]] = in ? pos[k] + 1 : 0;
+            if (!ok && page[k] >= 0) report(a.err, kDevPlanFull);
         }
     }
 }
