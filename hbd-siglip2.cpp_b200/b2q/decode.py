@@ -50,16 +50,20 @@ class DecoderConfig:
         return (self.n_head + 2 * self.n_kv_head) * self.d_head
 
 
-def placed_tokens(seq_of, pos, slot, new_len, max_pos: int):
-    """What a plan (its seq_of, pos and slot of a step's rows) has done for each
-    request: how many of its new tokens have a row and a cache slot, and the row of
-    the last of them.  Rows, pages and positions run out from the end, so these are
-    the first of the tokens that the request brings."""
+def placed_tokens(seq_of, slot, new_len):
+    """What a plan (its seq_of and slot of a step's rows) has done for each request:
+    how many of its new tokens have a row and a cache slot, and the row of the last of
+    them.  Rows and pages run out from the end, so these are the first of the tokens
+    that the request brings."""
     import torch
-    ok = ((slot >= 0) & (pos < max_pos)).to(torch.int32)
-    count = torch.zeros_like(new_len).index_add_(0, seq_of.clamp(min=0), ok)
+    count = torch.zeros_like(new_len).index_add_(0, seq_of.clamp(min=0), (slot >= 0).to(torch.int32))
     new = new_len.clamp(min=0)
     return count, (torch.cumsum(new, 0) - new + count - 1).clamp(0, seq_of.numel() - 1)
+
+
+def entered_pages(slot, page_size: int):
+    """How many pages these rows are the first ones of: those of a plan that hold a token."""
+    return ((slot & (page_size - 1 - 2 ** 31)) == 0).sum()     # (the sign too: -1 is no slot)
 
 
 class Decoder:
@@ -83,12 +87,12 @@ class Decoder:
 
         self.caches = [b2q.KVCache(*(torch.zeros((n_pages, cfg.n_kv_head, page_size, cfg.d_head), dtype=torch.float16,
                                                  device=dev) for _ in range(2))) for _ in layers]
-        self.rope = b2q.rope_table(cfg.max_pos, cfg.d_head)
+        width = -(-cfg.max_pos // page_size)
+        self.rope = b2q.rope_table(width * page_size, cfg.d_head)   # every position that the table has a page for
         self.ctx_len, self.new_len = i32(max_requests), i32(max_requests)
-        self.table = torch.full((max_requests, -(-cfg.max_pos // page_size)), -1, dtype=torch.int32, device=dev)
+        self.table = torch.full((max_requests, width), -1, dtype=torch.int32, device=dev)
         self.free = torch.arange(n_pages, dtype=torch.int32, device=dev)
         self._iota = torch.arange(n_pages, device=dev)
-        self._block = torch.arange(self.table.shape[1], dtype=torch.int32, device=dev)
         self.seq_of, self.pos, self.slot, self.kv_len, self.counts = i32(r), i32(r), i32(r), i32(r), i32(2)
         self.x, self.y, self.qkv, self.attn = f32(r, h), f32(r, h), f32(r, cfg.qkv), f32(r, h)
         self.q = torch.empty((r, h), dtype=torch.float16, device=dev)
@@ -118,13 +122,11 @@ class Decoder:
         seq_of, pos, slot, kv_len = self.seq_of[:r], self.pos[:r], self.slot[:r], self.kv_len[:r]
         b2q.kv_plan(self.ctx_len, self.new_len, self.page_size, self.free, self.table, seq_of, pos, slot, kv_len,
                     self.counts)
-        placed, at = placed_tokens(seq_of, pos, slot, self.new_len, c.max_pos)
-        grown = self.ctx_len + placed
-        # the list moves up by the pages that hold a token (those planned for tokens
-        # without a row are the last ones: they stay in it), with -1 behind its last
-        had, has = ((n + self.page_size - 1) // self.page_size for n in (self.ctx_len, grown))
-        self.table.masked_fill_(self._block[None] >= has[:, None], -1)
-        after = self._iota + (has - had).sum()
+        placed, at = placed_tokens(seq_of, slot, self.new_len)
+        # the list moves up by the pages that hold a token, -1 behind its last; those
+        # planned for tokens without a row are the last ones and stay in it (their table
+        # entries are behind the request's length: the next plan enters them anew)
+        after = self._iota + entered_pages(slot, self.page_size)
         self.free.copy_(torch.where(after < after.numel(), self.free[after.clamp(max=after.numel() - 1)], -1))
         for w, cache in zip(self.layers, self.caches):
             b2q.ln_quantize(x, w["ln1_w"], w["ln1_b"], c.eps, r, c.hidden, self.act_h, y)
@@ -135,7 +137,7 @@ class Decoder:
             b2q.ln_quantize(x, w["ln2_w"], w["ln2_b"], c.eps, r, c.hidden, self.act_h)
             b2q.mul_mat(w["fc1"], self.act_h, r, kind=b2q.EPI_BIAS_GELU_Q8, bias=w["fc1_b"], act_out=self.act_f)
             b2q.mul_mat(w["fc2"], self.act_f, r, x, kind=b2q.EPI_BIAS_RESIDUAL, bias=w["fc2_b"], residual=x)
-        self.ctx_len.copy_(grown)
+        self.ctx_len += placed
         n = self.ctx_len.numel()
         self.last.copy_(torch.where((placed > 0)[:, None], x[at], self.last))
         b2q.ln_quantize(self.last, *self.final, c.eps, n, c.hidden, self.act_h, self.last_n)
@@ -144,7 +146,7 @@ class Decoder:
 
     def release(self, request: int):
         """Ends a request: its pages are free again (synchronises)."""
-        row = self.table[request]
+        row = self.table[request, :-(-int(self.ctx_len[request]) // self.page_size)]
         pages, left = row[row >= 0], int((self.free >= 0).sum())
         self.free[left:left + pages.numel()] = pages
         self.ctx_len[request] = 0

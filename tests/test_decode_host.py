@@ -4,7 +4,7 @@ import random
 import pytest
 
 import b2q
-from b2q.decode import Decoder, placed_tokens
+from b2q.decode import Decoder, entered_pages, placed_tokens
 
 torch = pytest.importorskip("torch")
 
@@ -30,24 +30,26 @@ def plan(ctx, new, page, n_free, width, rows):
                 seq[t], pos[t] = s, p
                 first = taken + p // page - have
                 if p // page < width and (p // page < have or first < n_free):
-                    slot[t] = (1000 + first) * page + p % page
+                    slot[t] = (1000 + first if p // page >= have else 50 * s + p // page) * page + p % page
             t += 1
         taken += max(min(-(-(c + max(n, 0)) // page), width) - have, 0)
     return seq, pos, slot
 
 
-def test_tokens_without_a_row_a_page_or_a_position_do_not_count():
+def test_tokens_without_a_row_or_a_page_do_not_count():
     rng = random.Random(3)
     for _ in range(300):
         n, page, rows = rng.randint(1, 6), rng.choice([1, 4, 16]), rng.randint(1, 40)
         ctx = [rng.randint(0, 40) for _ in range(n)]
         new = [rng.choice([0, 1, rng.randint(0, 30), -3]) for _ in range(n)]
-        width, n_free, max_pos = rng.randint(12, 60), rng.randint(0, 20), rng.choice([45, 10 ** 6])
-        ctx = [min(c, width * page, max_pos) for c in ctx]
+        width, n_free = rng.randint(12, 60), rng.randint(0, 20)
+        ctx = [min(c, width * page) for c in ctx]
         seq, pos, slot = plan(ctx, new, page, n_free, width, rows)
-        count, last = placed_tokens(*(torch.tensor(v, dtype=torch.int32) for v in (seq, pos, slot, new)), max_pos)
+        count, last = placed_tokens(*(torch.tensor(v, dtype=torch.int32) for v in (seq, slot, new)))
+        pages = {v // page for v in slot if v >= 1000 * page}       # taken in this step, and holding a token
+        assert entered_pages(torch.tensor(slot, dtype=torch.int32), page) == len(pages)
         for s in range(n):
-            good = [t for t in range(rows) if seq[t] == s and slot[t] >= 0 and pos[t] < max_pos]
+            good = [t for t in range(rows) if seq[t] == s and slot[t] >= 0]
             assert count[s] == len(good)
             assert 0 <= last[s] < rows          # an index that is always there to be read
             assert [pos[t] for t in good] == list(range(ctx[s], ctx[s] + len(good)))
