@@ -669,9 +669,10 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
             float4* red = reinterpret_cast<float4*>(smem + kTeamFloats * 4) + team * kThreads;
             // Few outputs: the parts too are dealt to `subs` sums of an output, added up in
             // a second step.  Their number goes by the sizes alone and not by the team at
-            // hand, which depends on who reported last: half the threads take them in turns.
-            const int subs = 2 * n_out <= kThreads ? min(kThreads / n_out, n_parts) : 1;
-            const int at_once = subs > 1 ? min(team_threads / n_out, subs) : 1;
+            // hand, which depends on who reported last: half the threads take two each.
+            const int half = kThreads / 2 / n_out;
+            const int subs = half ? min(2 * half, n_parts) : 1;
+            const int at_once = half ? min(team_threads / n_out, subs) : 1;
             const int sub = subs > 1 ? me / n_out : 0, e0 = subs > 1 ? me % n_out : me;
             constexpr int kEach = (kRows * DP / 4 + kThreads / 2 - 1) / (kThreads / 2);   // outputs of a thread, at most
             constexpr int kFirst = kEach <= 8 ? 2 : 1;   // its parts that are asked for at once, with the refs
@@ -727,8 +728,10 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
                         const int p = sub + k * subs, e = e0 + i * team_threads;
                         if (p < n_parts && e < n_out) add(i, p, e, early[k][i]);
                     }
+            }
+            if (subs == 1) {
 #pragma unroll 4
-                for (int p = sub + kFirst * subs; p < n_parts; p += subs) {
+                for (int p = kFirst; p < n_parts; ++p) {
                     const float4* q = reinterpret_cast<const float4*>(part_of(p));
 #pragma unroll
                     for (int i = 0; i < kEach; ++i) {
@@ -736,16 +739,34 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
                         if (e < n_out) add(i, p, e, __ldcg(q + e));
                     }
                 }
-                if (subs > 1) {
-                    red[sub * n_out + e0] = acc[0];
-                    for (int x = sub + at_once; x < subs; x += at_once) {
-                        acc[0] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                        for (int p = x; p < n_parts; p += subs)
-                            add(0, p, e0, __ldcg(reinterpret_cast<const float4*>(part_of(p)) + e0));
-                        red[x * n_out + e0] = acc[0];
+            } else if (sub < at_once) {
+                // eight loads in flight (the last part again behind the end, not added)
+                static_assert(kEach >= 2, "two sums of a thread");
+                const auto rest = [&](auto sums) {
+                    constexpr int kSums = decltype(sums)::value, kBatch = 8 / kSums;
+                    int at[2] = {sub + kFirst * subs, sub + at_once};   // next parts of the sums
+                    const int stop = kSums == 2 && at[1] >= subs ? 0 : n_parts;
+                    while (at[kSums - 1] < stop || at[0] < n_parts) {
+                        float4 v[kBatch][kSums];
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+                            for (int i = 0; i < kSums; ++i)
+                                v[k][i] = __ldcg(reinterpret_cast<const float4*>(
+                                                     part_of(min(at[i] + k * subs, n_parts - 1))) + e0);
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+                            for (int i = 0; i < kSums; ++i)
+                                if (at[i] + k * subs < (i ? stop : n_parts)) add(i, at[i] + k * subs, e0, v[k][i]);
+#pragma unroll
+                        for (int i = 0; i < kSums; ++i) at[i] += kBatch * subs;
                     }
-                }
+                    red[sub * n_out + e0] = acc[0];
+                    if (kSums == 2 && stop) red[(sub + at_once) * n_out + e0] = acc[1];
+                };
+                if (at_once < subs) rest(std::integral_constant<int, 2>{});
+                else rest(std::integral_constant<int, 1>{});
             }
             __syncthreads();
             if (subs > 1 && sub == 0) {
