@@ -18,7 +18,7 @@
 // the end of one group, whole groups, and the start of another; what is not
 // whole goes to scratch as a partial result.  At its end the CTA reports its one or
 // two partial groups, and the last to report a group joins the parts in their order
-// (so the bits repeat).  Nobody waits.
+// whichever CTA that is (so the bits repeat).  Nobody waits.
 //
 // Inside a CTA each of four to eight warps takes 16 keys of every tile and keeps its own
 // ref, sum and output; they meet only where a group ends, each leaving its output
@@ -40,10 +40,10 @@
 // thousands of keys would shrink it (131,071 keys: relative error 4.0e-6 against 1.1e-6).
 //
 // Measured on one B200 (copy bandwidth 6.53 TB/s), device time: 3 requests of 131,071
-// keys, 40/8 heads of 128, fp16, 1.61 GB: 268 us, 6.0 TB/s; 61 ragged ones of 17 to 8,191,
-// 32/8 heads of 128, bf16, 0.99 GB: 166 us, 6.0 TB/s; 256 rows with a window of 1,024, 8/1
+// keys, 40/8 heads of 128, fp16, 1.61 GB: 270 us, 6.0 TB/s; 61 ragged ones of 17 to 8,191,
+// 32/8 heads of 128, bf16, 0.99 GB: 167 us, 5.9 TB/s; 256 rows with a window of 1,024, 8/1
 // heads of 256, 264 MB: 62 us, 4.3 TB/s (with four warps and three stages 70, as one warp a
-// scheduler waits for its own products); one request of 997 keys, 16 heads of 72: 9.5 us,
+// scheduler waits for its own products); one request of 997 keys, 16 heads of 72: 9.1 us,
 // round trips one after the other.  Two stages or three a warp: 268 and 275, 166 and 169 us.
 #include "b2q_decode.cuh"
 
@@ -216,50 +216,58 @@ __device__ __forceinline__ void write_out(const PagedArgs<T>& a, int r, int head
     }
 }
 
-// The marks in the results of `rows` query heads from head0 of row r, all threads: a
-// probability's remainder is zero or negative as often as not, and makes NaN of an
-// infinity that the probability would leave alone.  By the definition infinities of one
-// sign make that infinity; both signs, or a NaN, make NaN.  Reads the row's values once
-// more, 16 loads of a thread in flight.
+// The marks in the results of `rows` query heads (of one key head) from head0 of row r,
+// all threads of the CTA: a probability's remainder is zero or negative as often as not,
+// and makes NaN of an infinity that the probability would leave alone.  By the definition
+// infinities of one sign make that infinity; both signs, or a NaN, make NaN.  Reads the
+// row's values once more where there is a mark (3 x 131,071 keys, one infinity: 3.7 ms
+// a call).  flags: one word a column, shared.
 template <class To, class T>
-__device__ __noinline__ void settle(const PagedArgs<T>& a, int r, int head0, int rows) {
-    constexpr int kTogether = 16;
+__device__ __noinline__ void settle(const PagedArgs<T>& a, int r, int head0, int rows, uint32_t* flags) {
+    constexpr int kTogether = 16;   // loads of a thread in flight
+    const int tid = threadIdx.x, n = rows * a.d;
+    To* out = static_cast<To*>(a.out) + r * a.ldo + static_cast<int64_t>(head0) * a.d;
+    bool any = false;
+    for (int i = tid; i < n; i += blockDim.x) any |= is_open(out[i]);
+    if (!__syncthreads_or(any)) return;
+    for (int c = tid; c < a.d; c += blockDim.x) flags[c] = 0;
+    __syncthreads();
     const Span s = span_of<64>(a, r);
-    for (int i = threadIdx.x; i < rows * (a.d / 4); i += blockDim.x) {
-        const int head = head0 + i / (a.d / 4), c = i % (a.d / 4) * 4;
-        To* o = static_cast<To*>(a.out) + r * a.ldo + static_cast<int64_t>(head) * a.d + c;
-        if (!is_open(o[0]) && !is_open(o[1]) && !is_open(o[2]) && !is_open(o[3])) continue;
-        const T* col = a.c.v + head / a.group * a.c.head_stride + c;
-        uint32_t up = 0, down = 0, nan = 0;   // bit e: element e has such a value
-        for (int key0 = s.first; key0 < s.len && (nan | (up & down)) != 15u;
-             key0 = s.len - key0 > kTogether ? key0 + kTogether : s.len) {
-            uint2 raw[kTogether];
+    const int chunks = a.d / 8, step = blockDim.x / chunks, c = tid % chunks * 8;
+    const T* col = a.c.v + head0 / a.group * a.c.head_stride + c;
+    uint32_t seen[8] = {};   // 1: +inf, 2: -inf, 4: NaN, of column c + e
+    if (tid / chunks < step && tid / chunks < s.len - s.first)
+        for (int key0 = s.first + tid / chunks; key0 < s.len;
+             key0 = s.len - key0 > kTogether * step ? key0 + kTogether * step : s.len) {
+            uint4 raw[kTogether];
 #pragma unroll
-            for (int k = 0; k < kTogether; ++k) {   // (the last key again behind the end: nothing new)
-                const int key = k < s.len - key0 ? key0 + k : s.len - 1;
+            for (int k = 0; k < kTogether; ++k) {   // (the first key again behind the end: nothing new)
+                const int key = k * step < s.len - key0 ? key0 + k * step : key0;
                 const int page = a.table[s.seq * a.bt_stride + (key >> a.c.page_shift)];
                 const bool ok = page >= 0 && page < a.c.n_pages;
                 const T* p = col + (ok ? page : 0) * a.c.page_stride + (key & a.c.page_mask) * a.c.token_stride;
-                raw[k] = ok ? *reinterpret_cast<const uint2*>(p) : make_uint2(0u, 0u);
+                raw[k] = ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
             }
 #pragma unroll
             for (int k = 0; k < kTogether; ++k) {
-                const float2 x01 = unpack2<T>(raw[k].x), x23 = unpack2<T>(raw[k].y);
-                const float x[4] = {x01.x, x01.y, x23.x, x23.y};
+                const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    up |= static_cast<uint32_t>(x[e] == INFINITY) << e;
-                    down |= static_cast<uint32_t>(x[e] == -INFINITY) << e;
-                    nan |= static_cast<uint32_t>(x[e] != x[e]) << e;
+                for (int e = 0; e < 8; ++e) {
+                    const float2 x2 = unpack2<T>(w[e / 2]);
+                    const float x = e % 2 ? x2.y : x2.x;
+                    seen[e] |= (x == INFINITY ? 1u : 0u) | (x == -INFINITY ? 2u : 0u) | (x != x ? 4u : 0u);
                 }
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const bool u = (up >> e) & 1, d = (down >> e) & 1, n = (nan >> e) & 1;
-            if (is_open(o[e])) o[e] = from_f32<To>(n || u == d ? __uint_as_float(0x7FFFFFFFu) : u ? INFINITY : -INFINITY);
+    for (int e = 0; e < 8; ++e)
+        if (seen[e]) atomicOr(flags + c + e, seen[e]);
+    __syncthreads();
+    for (int i = tid; i < n; i += blockDim.x)
+        if (is_open(out[i])) {
+            const uint32_t f = flags[i % a.d];
+            out[i] = from_f32<To>(f == 1 ? INFINITY : f == 2 ? -INFINITY : __uint_as_float(0x7FFFFFFFu));
         }
-    }
 }
 template <class T>
 __device__ __forceinline__ void write_lse(const PagedArgs<T>& a, int r, int head, float ref, float l) {
@@ -793,7 +801,8 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
         if (s_open) {
             const auto settle_group = [&](int r, int hm) {
                 const int q0 = hm % a.row_blocks * kRows;
-                settle<To>(a, r, hm / a.row_blocks * a.group + q0, min(kRows, a.group - q0));
+                settle<To>(a, r, hm / a.row_blocks * a.group + q0, min(kRows, a.group - q0),
+                           reinterpret_cast<uint32_t*>(smem));
             };
             Cursor c;   // the share's whole groups
             c.r = s_start.r;
@@ -807,7 +816,8 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas) paged_k
                 next_unit<kTile>(a, c, per_row);
             }
             for (int x = 0; x < 2; ++x)   // and those that it joined
-                if (s_last[x]) settle<To>(a, s_partial[x].r, s_partial[x].head0, s_partial[x].rows);
+                if (s_last[x])
+                    settle<To>(a, s_partial[x].r, s_partial[x].head0, s_partial[x].rows, reinterpret_cast<uint32_t*>(smem));
         }
     }
 
