@@ -3,7 +3,8 @@
 The towers encode; this runs what follows them, a decoder of the towers' block
 shape (pre-LN, GELU feed-forward, optionally fewer key heads) over a paged
 key-value cache.  A step takes any mix of requests: one new token each, whole
-prompts, image embeddings as a prefix, idle ones.  Per step
+prompts (rows of the hidden width: token embeddings, or features of the caller's;
+the towers give one pooled vector an image and no patch features), idle ones.  Per step
 
   kv_plan              block tables, positions and slots from the lengths
 
