@@ -26,8 +26,9 @@
 //    lies at 2^9 or above): beside one 1e6 times as large values keep 14 bits.
 //  * S leaves the tensor core once per block and is summed in fp32, d S.
 // Relative error against 64 bits: 1 x 1152 x 4320, Q4_0, 9e-8 (plain fp32 products
-// 1.9e-7); 1 x 256000 x 1152, Q4_1, 1.6e-7 (1.3e-7: with the minima apart, d S and m X are
-// each several times their sum, and so are their roundings).
+// 1.9e-7); 1 x 256000 x 1152, Q4_1, 1.6e-7 to 2.6e-7 by the row (1.3e-7: with the minima
+// apart, d S and m X are each several times their sum, and so are their roundings, of
+// which that of X is the same for every output).
 //
 // The weights are laid out at registration in the order the lanes want them:
 // per 16 rows a run of units of 128 columns, each 1024 bytes of nibbles (lane l of
